@@ -81,8 +81,9 @@ def draw(rng):
                 "kv_heads": kv_heads, "dim": dim, "page": page, "dtype": dtype}
     heads = kv_heads * rng.choice([1, 2, 4])
     batch, tk = rng.randint(1, 8), _log_int(rng, 1, 4096)
-    most = 8192 * 512 * 24 if dtype == "bf16" else 1024 * 512 * 24  # query rows x keys
-    tq = min(rng.choice([1, _log_int(rng, 1, 4096)]), max(1, most // (tk * batch * heads)))
+    most = 8192 * 400 * 24 if dtype == "bf16" else 1024 * 512 * 24  # query rows x keys
+    rows = min(most // tk, (8192 if dtype == "bf16" else 4096) * 24)
+    tq = min(rng.choice([1, _log_int(rng, 1, 4096)]), max(1, rows // (batch * heads)))
     return {"op": op, "batch": batch, "tq": tq, "tk": tk, "longest": tk, "shortest": rng.randint(1, tk),
             "heads": heads, "kv_heads": kv_heads, "dim": dim, "mask": rng.random() < 0.5, "dtype": dtype}
 
