@@ -371,6 +371,74 @@ int we_attention(we_ctx* ctx, const void* q, const void* k, const void* v, int32
 int we_attend(we_ctx* ctx, const void* q, const void* k, const void* v, int32_t dtype, int64_t tokens, int64_t heads,
               int64_t kv_heads, int64_t dim, int32_t causal, int32_t out_dtype, void** out);
 
+/* ---------------- single tokens: products with 4-bit weights (no reference counterpart) ----------------
+   we_matmul for few rows: the same descriptor with w_dtype = WE_INT4G64 and 1 <= m <= WE_MATVEC_MAX_ROWS (a decoder's
+   tokens of one step). y[i, n] = sum over groups g of s[n, g] sum over j in g of q[n, j] x[i, j], every product exact
+   and every sum in f32 (we_matmul rounds q s to bf16 first), then bias and the fused epilogue as we_matmul applies
+   them. x and y f32 or bf16 with row strides and offsets in values; w contiguous [n, k / 2] and 16-byte aligned, f16
+   group scales [n, k / 64], k a multiple of 64; scale, chan_scale and k_split do not apply (scale is ignored, the
+   others are refused). flags: WE_MM_ACCUMULATE. */
+#define WE_MATVEC_MAX_ROWS 16
+int we_matvec(we_ctx* ctx, const we_matmul_desc* desc, const void* x, const void* w, void* y);
+
+/* ---------------- single tokens: a paged 4-bit K/V cache (no reference counterpart) ----------------
+   One layer's cache: every (token, kv head) row of `dim` values is WE_INT4G64, i.e. two's complement codes packed two
+   per byte (low nibble = even value) and one f16 scale per 64 values: s = f16(max|x| / 7), at most 65504, and
+   q = clamp(rint(x / s), -8, 7), 0 where s is 0. Rows live in pages of `page` tokens, laid out
+   [pages, kv_heads, page, dim / 2] (scales [pages, kv_heads, page, dim / 64]); token t of sequence b is row t % page
+   of page page_table[b][t / page]. `lengths` holds each sequence's tokens BEFORE the current step; all three arrays
+   are read on the device, in stream order. A negative length marks an idle sequence: nothing is written for it and its
+   outputs are zero. A page id outside 0..pages-1, or a token past max_pages * page, is skipped and recorded in the
+   context's device error word (6: bad page id, 7: past the end of the page table); such keys are not attended.
+   dim: 64, 128 or 256; page a multiple of 16; k, v 16-byte and their scales 4-byte aligned. */
+typedef struct {
+  uint8_t* k;
+  uint8_t* v;
+  uint16_t* k_scale;
+  uint16_t* v_scale;
+  const int32_t* page_table; /* [batch, max_pages] */
+  int32_t* lengths;          /* [batch] */
+  int64_t pages, max_pages, batch, kv_heads, page, dim;
+} we_kv4_cache;
+/* Quantises k and v [batch, tokens, kv_heads, dim] (f32 or bf16; `stride` values from a token to the next, 0 =
+   kv_heads * dim; a sequence's tokens follow the previous sequence's) into rows lengths[b] .. lengths[b] + tokens - 1. */
+int we_kv4_append(we_ctx* ctx, const we_kv4_cache* cache, const void* k, const void* v, int32_t dtype, int64_t tokens,
+                  int64_t stride);
+/* The values of rows start[b] .. start[b] + tokens - 1 (device array; NULL: from lengths[b], what an append of `tokens`
+   has just written) into k and v [batch, tokens, kv_heads, dim], f32 or bf16: zeros for idle sequences and for rows
+   outside the page table. Either of k and v may be NULL. */
+int we_kv4_unpack(we_ctx* ctx, const we_kv4_cache* cache, void* k, void* v, int32_t dtype, int64_t tokens,
+                  const int32_t* start);
+/* Attention of each sequence's `tokens` newest tokens over its cache: query i of sequence b stands at position
+   lengths[b] + i and sees keys 0 .. lengths[b] + i, so the step's keys have been appended. q [batch, tokens, heads, dim]
+   and out alike (q_stride / out_stride values from a token to the next, 0 = heads * dim); heads a multiple of
+   kv_heads, as we_attention groups them; scale 0 = 1 / sqrt(dim). */
+int we_kv4_attention(we_ctx* ctx, const we_kv4_cache* cache, const void* q, int32_t dtype, int64_t tokens,
+                     int64_t heads, int64_t q_stride, float scale, void* out, int32_t out_dtype, int64_t out_stride);
+/* lengths[b] += tokens for every sequence that is not idle: the end of a step, after its last layer. */
+int we_kv4_advance(we_ctx* ctx, const we_kv4_cache* cache, int64_t tokens);
+
+/* ---------------- cross attention: queries of one sequence, keys and values of another ----------------
+   out = softmax(scale q k^T) v per head with grouped-query heads (as attention(), src/kernels/attention.ts:20-51, with
+   its own key count): q [batch, tq, heads, dim], k, v [batch, tk, kv_heads, dim], out as q. Strides are values from a
+   token to the next (0 = contiguous heads; k and v cut out of one fused projection have a larger one); a batch entry's
+   tokens follow the previous one's. A key j of entry b is seen when j < key_lengths[b] (device int32, NULL = tk) and
+   key_mask[b][j] != 0 (device bytes [batch, tk], NULL = all). A row that sees no key gives zeros; values of unseen keys
+   (NaN included) do not reach the output. scale 0 = 1 / sqrt(dim). dim 1..256, f32 or bf16. */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int32_t dtype, out_dtype;
+  int64_t batch, tq, tk, heads, kv_heads, dim;
+  int64_t q_stride, k_stride, v_stride, out_stride;
+  const int32_t* key_lengths;
+  const uint8_t* key_mask;
+  float scale;
+} we_cross_desc;
+int we_cross_attention(we_ctx* ctx, const we_cross_desc* desc);
+
 /* ---------------- layer streaming: src/model/weights.ts:94-131 (loadTransformer) ----------------
    The reference uploads every block once and keeps it resident. A streamer instead keeps `slots` device
    buffers and copies layer l (host[l], bytes[l]) into slot l % slots with cudaMemcpyAsync on its own copy

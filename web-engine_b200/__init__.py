@@ -5,8 +5,9 @@ mirror of the reference's operator API (src/model/ops.ts over src/gpu/graph.ts) 
 """
 from . import _lib
 from .graph import Binding, Buffer, Graph
-from .ops import Linear, Mod, Rope, attention, k_split_for, linear, linear_host, no_mod, norm, qk_norm_rotate, rotate
-from . import kernels, parallel
+from .ops import (Linear, Mod, Rope, attention, cross_attention, k_split_for, linear, linear_host, matvec, no_mod, norm,
+                  qk_norm_rotate, rotate)
+from . import kernels, kv4, parallel
 from .stream import Streamer
 from . import block as blocks
 from . import transformer
@@ -15,7 +16,7 @@ from . import sequence
 from . import comm
 
 __all__ = ["Graph", "Buffer", "Binding", "Linear", "Mod", "Rope", "linear", "linear_host", "norm", "no_mod", "rotate",
-           "qk_norm_rotate", "k_split_for", "kernels", "blocks", "transformer", "parallel", "Streamer", "weights", "sequence", "comm", "build"]
+           "qk_norm_rotate", "k_split_for", "matvec", "cross_attention", "kernels", "kv4", "blocks", "transformer", "parallel", "Streamer", "weights", "sequence", "comm", "build"]
 
 
 def build(verbose: bool = False) -> str:

@@ -100,6 +100,20 @@ class RopeDesc(C.Structure):
     _fields_ = [("cos", C.c_void_p), ("sin", C.c_void_p), ("pairs", C.c_int64), ("tokens", C.c_int64)]
 
 
+class KV4Desc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "page_table", "lengths")] + [
+        (n, C.c_int64) for n in ("pages", "max_pages", "batch", "kv_heads", "page", "dim")]
+
+
+class CrossDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out")] + [("dtype", C.c_int32), ("out_dtype", C.c_int32)] + [
+        (n, C.c_int64) for n in ("batch", "tq", "tk", "heads", "kv_heads", "dim", "q_stride", "k_stride", "v_stride",
+                                 "out_stride")] + [
+        ("key_lengths", C.c_void_p), ("key_mask", C.c_void_p), ("scale", C.c_float)]
+
+
+MATVEC_MAX_ROWS = 16
+
 _P = C.c_void_p
 _I64 = C.c_int64
 _SIGS = {
@@ -159,6 +173,13 @@ _SIGS = {
     "we_attention": (C.c_int, [_P, _P, _P, _P, C.c_int32, _I64, _I64, _I64, _I64, C.c_int32, _P, C.c_int32]),
     "we_attend": (C.c_int, [_P, _P, _P, _P, C.c_int32, _I64, _I64, _I64, _I64, C.c_int32, C.c_int32,
                             C.POINTER(C.c_void_p)]),
+    "we_matvec": (C.c_int, [_P, C.POINTER(MatmulDesc), _P, _P, _P]),
+    "we_kv4_append": (C.c_int, [_P, C.POINTER(KV4Desc), _P, _P, C.c_int32, _I64, _I64]),
+    "we_kv4_unpack": (C.c_int, [_P, C.POINTER(KV4Desc), _P, _P, C.c_int32, _I64, _P]),
+    "we_kv4_attention": (C.c_int, [_P, C.POINTER(KV4Desc), _P, C.c_int32, _I64, _I64, _I64, C.c_float, _P, C.c_int32,
+                                   _I64]),
+    "we_kv4_advance": (C.c_int, [_P, C.POINTER(KV4Desc), _I64]),
+    "we_cross_attention": (C.c_int, [_P, C.POINTER(CrossDesc)]),
     "we_streamer_create": (C.c_int, [_P, C.POINTER(C.c_void_p), C.POINTER(C.c_size_t), C.c_int32, C.c_int32,
                                      C.c_uint32, C.POINTER(C.c_void_p)]),
     "we_streamer_acquire": (C.c_int, [_P, C.c_int32, C.POINTER(C.c_void_p)]),

@@ -24,6 +24,8 @@ enum : uint32_t {
   DEV_ERR_TIMEOUT_EPILOGUE = 3,
   DEV_ERR_TIMEOUT_DRAIN = 4,
   DEV_ERR_TIMEOUT_PEER = 5,  // a peer exchange waited longer than its timeout for another rank's flag
+  DEV_ERR_KV_PAGE = 6,       // a page id outside the cache (the access was skipped)
+  DEV_ERR_KV_FULL = 7,       // a token past the end of a sequence's page table (the access was skipped)
 };
 
 // ---- element decode / encode ----

@@ -143,4 +143,25 @@ int64_t flash_attention_scratch_bytes(const AttnArgs& a, int splits);
 cudaError_t launch_flash_attention(const AttnArgs& a, int splits, void* scratch, uint32_t* err, cudaStream_t st);
 cudaError_t launch_attention_simt(const AttnArgs& a, int sms, cudaStream_t st);
 
+// ---- single-token decoding (k_matvec.cu, k_kv4.cu, k_cross.cu) ----
+// y[m, n] = x[m, k] . (q s)^T: int4 group-64 weights, few rows (strides and epilogue as in MatmulArgs; w 16-byte aligned)
+cudaError_t launch_matvec(const void* x, const void* w, void* y, const MatmulArgs& a, int sms, cudaStream_t st);
+
+cudaError_t launch_kv4_append(const we_kv4_cache& c, const void* k, const void* v, int dt, int64_t tokens,
+                              int64_t stride, uint32_t* err, int sms, cudaStream_t st);
+cudaError_t launch_kv4_unpack(const we_kv4_cache& c, void* k, void* v, int dt, int64_t tokens, const int32_t* start,
+                              uint32_t* err, int sms, cudaStream_t st);
+cudaError_t launch_kv4_advance(const we_kv4_cache& c, int64_t tokens, cudaStream_t st);
+struct Kv4AttnArgs {
+  we_kv4_cache c;
+  const void* q;
+  void* out;
+  int64_t tokens, heads, q_stride, out_stride;
+  float scale;
+  int dtype, out_dtype;
+};
+cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, uint32_t* err, int sms, cudaStream_t st);
+
+cudaError_t launch_cross_simt(const we_cross_desc& d, int sms, cudaStream_t st);
+
 }  // namespace we

@@ -19,6 +19,23 @@ THETA = 1000.0       # src/kernels/rope.ts:11
 TILE = 128           # src/kernels/matmul.ts:33
 
 
+class Call:
+    """One library call with its arguments converted once. A decoding loop keeps its buffers in place and runs the same
+    calls every token: calling this queues the op again at the cost of one foreign-function call. `keep` holds what the
+    arguments point to (descriptors, tensors)."""
+
+    __slots__ = ("fn", "args", "ctx", "keep")
+
+    def __init__(self, graph: Graph, fn, args: tuple, keep=()):
+        self.fn, self.ctx, self.keep = fn, graph.ctx, keep
+        self.args = (graph.ctx, *args)
+
+    def __call__(self) -> None:
+        rc = self.fn(*self.args)
+        if rc:
+            L.check(self.ctx, rc)
+
+
 def matmul_params(m: int, n: int, k: int, scale: float, x_stride=None, w_stride=None, y_stride=None, x_offset=0,
                   w_offset=0, y_offset=0, k_split=1) -> L.MatmulDesc:
     """matmulParams (src/kernels/matmul.ts:198-212): validates like the reference and returns the descriptor."""
@@ -53,6 +70,26 @@ def matmul(graph: Graph, x, w, y, m: int, n: int, k: int, scale: float = 1.0, *,
     d.flags = (L.MM_ACCUMULATE if accumulate else 0) | (L.MM_FP8_FAST if fast else 0) | (
         L.MM_FORCE_SIMT if force_simt else 0)
     L.check(graph.ctx, L.lib().we_matmul(graph.ctx, C.byref(d), addr(x), addr(w), addr(y)))
+
+
+def matvec_call(graph: Graph, x, w, y, m: int, n: int, k: int, *, group_scale, x_dtype="f32", y_dtype="f32", bias=None,
+                x_stride=None, y_stride=None, x_offset=0, y_offset=0, accumulate=False, act=None, aux_op=None, aux=None,
+                aux_dtype="f32", gate=None) -> Call:
+    """The prepared form of `matvec`."""
+    d = matmul_params(m, n, k, 1.0, x_stride, None, y_stride, x_offset, 0, y_offset)
+    d.epi = epilogue(act, aux_op, aux, aux_dtype, gate)
+    d.group_scale, d.bias = addr(group_scale).value, addr(bias).value
+    d.x_dtype, d.w_dtype, d.y_dtype = L.DTYPES[x_dtype], L.INT4G64, L.DTYPES[y_dtype]
+    d.flags = L.MM_ACCUMULATE if accumulate else 0
+    return Call(graph, L.lib().we_matvec, (C.pointer(d), addr(x), addr(w), addr(y)),
+                (d, x, w, y, group_scale, bias, aux, gate))
+
+
+def matvec(graph: Graph, x, w, y, m: int, n: int, k: int, **kw) -> None:
+    """y[m, n] = x[m, k] . W^T for 1 to 16 rows and int4 group-64 W (we_matvec): packed [n, k / 2] with f16
+    group_scale [n, k / 64]. q s stays exact (matmul rounds it to bf16). Keywords as in `matvec_call`: dtypes, row
+    strides and offsets in values, bias, the fused epilogue steps of `matmul`, accumulate."""
+    matvec_call(graph, x, w, y, m, n, k, **kw)()
 
 
 def matmul_workgroups(m: int, n: int) -> tuple:
@@ -269,6 +306,25 @@ def attention(graph: Graph, q, k, v, tokens: int, heads: int, kv_heads: int, dim
     """attention into a given output buffer (src/kernels/attention.ts:20-51)."""
     L.check(graph.ctx, L.lib().we_attention(graph.ctx, addr(q), addr(k), addr(v), L.DTYPES[dtype], tokens, heads,
                                             kv_heads, dim, int(causal), addr(out), L.DTYPES[out_dtype]))
+
+
+def cross_attention_call(graph: Graph, q, k, v, out, batch: int, tq: int, tk: int, heads: int, kv_heads: int, dim: int, *,
+                         key_lengths=None, key_mask=None, scale: float = 0.0, q_stride: int = 0, k_stride: int = 0,
+                         v_stride: int = 0, out_stride: int = 0, dtype: str = "f32", out_dtype: str = "f32") -> Call:
+    """The prepared form of `cross_attention`."""
+    d = L.CrossDesc(addr(q).value, addr(k).value, addr(v).value, addr(out).value, L.DTYPES[dtype], L.DTYPES[out_dtype],
+                    batch, tq, tk, heads, kv_heads, dim, q_stride, k_stride, v_stride, out_stride,
+                    addr(key_lengths).value, addr(key_mask).value, scale)
+    return Call(graph, L.lib().we_cross_attention, (C.pointer(d),), (d, q, k, v, out, key_lengths, key_mask))
+
+
+def cross_attention(graph: Graph, q, k, v, out, batch: int, tq: int, tk: int, heads: int, kv_heads: int, dim: int,
+                    **kw) -> None:
+    """out = softmax(scale q k^T) v per head, the keys and values another sequence's (we_cross_attention): q, out
+    [batch, tq, heads, dim], k, v [batch, tk, kv_heads, dim]. key_lengths: int32 [batch]; key_mask: bytes [batch, tk],
+    0 = unseen; a row that sees nothing gives zeros. scale 0 = 1 / sqrt(dim). Strides are values from a token to the
+    next (0 = contiguous)."""
+    cross_attention_call(graph, q, k, v, out, batch, tq, tk, heads, kv_heads, dim, **kw)()
 
 
 def norm_split(graph: Graph, x, weight, rows: int, d: int, hi, lo, row_scale, scale=None, shift=None, eps=1e-5,
