@@ -10,13 +10,16 @@
 //   u = q + 8, and (word & 0x00f000f0) ^ 0x00800080 are u 2^-20; a shift by 8 brings the other two pairs of a word
 //   there: 5 operations for 8 weights. The factor 16 is taken from the x of those places (x / 16), and the offset by
 //   starting each group's sum at -8 sum(x): sum u x - 8 sum x = sum q x.
-// - x is laid out once per CTA as f16 in the order of the tiles, times a power of two that brings its row's maximum to
-//   2^15. bf16 values keep all their bits down to 2^-24 of the maximum (below, an error of at most 2^-36 of it); an f32
-//   value is two columns, 11 bits and the next 11 times 2^10, together within 2^-22. So a product is exact or within
-//   2^-22, sums are f32, and the group scale is one f32 multiply-add per group and output.
-// - A warp takes 256 values of k of 32 channels at a time, through a ring of its own in shared memory (cp.async, no
-//   barrier between warps); the 8 warps of a CTA split k, clusters of up to 8 CTAs split it further when there are few
-//   channels or x does not fit; partial sums meet in shared memory in a fixed order, so a call always gives the same bits.
+// - x is laid out once per CTA as f16 in the order of the tiles, each group of 64 times a power of two that brings its
+//   maximum to 2^15. bf16 values keep all their bits down to 2^-24 of the maximum (below, an error of at most 2^-36 of
+//   it); an f32 value is two columns, 11 bits and the next 11 times 2^10, together within 2^-22. So a product is exact
+//   or within 2^-22, sums are f32, and a group's two scales are one f32 multiply-add per output.
+// - A lane reads 16 bytes of a channel at once, so the four lanes of a tile's row hold two groups of 64. A token
+//   therefore is two columns, one per group, each zero where the lane's values belong to the other group: one product
+//   gives both groups' sums side by side and each takes its own scale.
+// - Weights go from global memory to registers, 4 KB a warp ahead of their use. Warps split channels and k; clusters of up
+//   to 8 CTAs split k when there are few channels or x does not fit. Partial sums meet in shared memory in a fixed order,
+//   so a call always gives the same bits.
 #include <algorithm>
 
 #include "common.cuh"
@@ -84,365 +87,329 @@ __global__ void __launch_bounds__(256) matvec_long_kernel(const void* __restrict
 // ---------------- tensor-core tiles ----------------
 namespace mv {
 constexpr int WARPS = 8, THREADS = WARPS * 32;
-constexpr int RT = 2, ROWS = RT * 16;          // channels of a tile pair
-constexpr int KB_GROUPS = 4, KB = 256;         // a warp's step: 4 groups = 128 packed bytes of each channel
-constexpr int STAGE = ROWS * 128;              // bytes of one step
-#ifndef MV_DEPTH
-#define MV_DEPTH 2
-#endif
-constexpr int DEPTH = MV_DEPTH;                // steps in a warp's ring
-constexpr int RING = WARPS * DEPTH * STAGE;
-constexpr int MAX_PAIRS = 8;                   // tile pairs of one CTA (their sums wait in shared memory)
+constexpr int CHUNK = 128;       // values of k of a step: 64 packed bytes of each channel
 constexpr int MAX_CLUSTER = 8;
+constexpr int IN_FLIGHT = 4;  // row tiles x steps that a warp loads ahead (1 KB each)
+constexpr int NOTHING = IN_FLIGHT * 256; // bytes of zeros that lanes without a token read
 
 struct Plan {
-  int pairs;        // tile pairs per CTA
+  int wk;           // warps of a CTA that split k (a power of two); the others take further channels
   int cluster;      // CTAs that split k
-  int kb_per_cta;   // steps of 256 values per CTA
-  int x_pitch;      // bytes from one column of x to the next in shared memory
+  int per_cta;      // chunks of 128 values per CTA
+  int x_pitch;      // bytes from one token's piece to the next in shared memory
   int smem;
 };
 }  // namespace mv
 
-// d = a b + c: 16 x 8 x 16, f16 operands, f32 sums (the legacy warp-level tensor instruction; see the file's head)
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
-                                        const float (&c)[4]) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+// 16 bytes that are read once
+__device__ __forceinline__ uint4 load_once16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
 }
 
-// f16 pair of two floats, to nearest, and its values back
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
+// d += a b: 16 x 8 x 16, f16 operands, f32 sums (the legacy warp-level tensor instruction; see the file's head)
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// (v & mask) ^ flip in one operation
+__device__ __forceinline__ uint32_t and_xor(uint32_t v, uint32_t mask, uint32_t flip) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(v), "r"(mask), "r"(flip));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ float2 unpack_f16x2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
-// XT: type of x; NT: tiles of 8 columns. Column c is token c (bf16), or the leading (c < m) or following bits of token
-// c % m (f32).
-template <int XT, int NT>
-__global__ void __launch_bounds__(mv::THREADS) matvec_mma_kernel(const void* __restrict__ x, const uint8_t* __restrict__ w,
+// XT: type of x; NT: tiles of 8 columns; RT: row tiles of 16 channels of a warp; PER_SM: CTAs that fit an SM. Columns 2 t
+// and 2 t + 1 are the two groups of a chunk for piece t / m (f32: the leading bits, the following ones) of token t % m.
+template <int XT, int NT, int RT, int PER_SM>
+__global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const void* __restrict__ x, const uint8_t* __restrict__ w,
                                                                  void* y, const MatmulArgs a, const mv::Plan p) {
   using namespace mv;
   constexpr int XB = XT == WE_F32 ? 4 : 2, PIECES = XT == WE_F32 ? 2 : 1;
-  constexpr int COLS = NT * 8;
+  constexpr int TOKS = NT * 4, ROWS = RT * 16, DEPTH = IN_FLIGHT / RT, CHAINS = NT * RT <= 2 ? 2 : 1;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ uint32_t row_max[WE_MATVEC_MAX_ROWS];  // |x| of a row's slice, as bits of f32
-  const int m = (int)a.m, n = (int)a.n;
+  const int m = (int)a.m, n = (int)a.n, toks = m * PIECES;
   const int groups = (int)(a.k / 64);
-  uint8_t* xs = smem + RING;                                                    // [m * PIECES] columns of x_pitch bytes
-  float* start = reinterpret_cast<float*>(xs + m * PIECES * p.x_pitch);         // [groups of the slice][COLS]
-  float* red = start + p.kb_per_cta * KB_GROUPS * COLS;                         // [WARPS][ROWS][COLS]
-  float* part = red + WARPS * ROWS * COLS;                                      // [pairs][ROWS][m]
+  uint8_t* xs = smem + NOTHING;    // [toks][chunks][quad][lane of a row][16 bytes]
+  // [chunks of the slice][TOKS]: the two groups' starts (-8 sum of x) and powers of two
+  float4* base = reinterpret_cast<float4*>(xs + toks * p.x_pitch);
+  float* red = reinterpret_cast<float*>(base + p.per_cta * TOKS);  // [WARPS][ROWS][TOKS]
+  float* part = red + WARPS * ROWS * TOKS;                         // [m][channels of the CTA]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)tc::cluster_rank();
-  const int pair0 = (int)blockIdx.y * p.pairs;
-  const int all_pairs = (n + ROWS - 1) / ROWS;
-  const int pairs = min(p.pairs, all_pairs - pair0);
-  const int g0 = rank * p.kb_per_cta * KB_GROUPS;                               // first group of this CTA
-  const int my_groups = max(0, min(p.kb_per_cta * KB_GROUPS, groups - g0));
-  const int kbs = (my_groups + KB_GROUPS - 1) / KB_GROUPS;                      // steps of this CTA
-  const int my_kbs = kbs > warp ? (kbs - warp + WARPS - 1) / WARPS : 0;         // steps warp, warp + 8, ...
-  const int items = my_kbs * pairs;                                             // (pair, step), step fastest
-  if (threadIdx.x < WE_MATVEC_MAX_ROWS) row_max[threadIdx.x] = 0;
+  const int kpart = warp & (p.wk - 1);                             // this warp's part of k
+  const int cta_rows = WARPS / p.wk * ROWS;
+  const int first = (int)blockIdx.y * cta_rows;
+  const int g0 = rank * p.per_cta * 2;                             // first group of this CTA
+  const int my_groups = max(0, min(p.per_cta * 2, groups - g0));
+  const int chunks = (my_groups + 1) / 2;                          // of this CTA, the last one perhaps half
+  const int ch0 = chunks * kpart / p.wk, end = chunks * (kpart + 1) / p.wk;  // this warp's chunks
   pdl_launch_dependents();
   pdl_wait();
 
-  // Steps are fetched in the order of work. A lane copies 16 of 128 bytes of every fourth channel and loads the scales
-  // 32 j + lane = (channel, group of the step). Past the last channel it reads the last one again (not stored), past the
-  // last group the first one of the slice (its x is zero).
-  const uint32_t ring = tc::smem_u32(smem) + (uint32_t)(warp * DEPTH * STAGE);
-  const uint32_t lane_dst = ring + (lane >> 3) * 128 + (((((lane & 7) >> 1) ^ ((lane >> 3) & 3)) << 1) | (lane & 1)) * 16;
-  uint32_t w_off[ROWS / 4], s_off[2 * RT];  // this lane's channels: offsets in 16 bytes, in scales
+  // A step's weights and scales: of channels lane / 4 and + 8 of each row tile, the values 32 (lane % 4) and on of the
+  // chunk. Past the last channel the last one is read again (not stored); a lane whose group of the last chunk does not
+  // exist reads nothing there (its x is zero).
+  uint4 wq[DEPTH][2 * RT];
   uint32_t sc[DEPTH][2 * RT];
-  int f_pair = pair0, f_kb = warp, f_item = 0;
-  const uint32_t row16 = (uint32_t)(a.k / 32);
-  auto place = [&] {
-    const int c0 = f_pair * ROWS;
+  const uint8_t* wp[2 * RT];
+  const uint16_t* sp[2 * RT];
 #pragma unroll
-    for (int i = 0; i < ROWS / 4; i++) w_off[i] = (uint32_t)min(c0 + i * 4 + (lane >> 3), n - 1) * row16;
+  for (int j = 0; j < 2 * RT; j++) {
+    const int64_t at = (int64_t)min(first + warp / p.wk * ROWS + j * 8 + (lane >> 2), n - 1) * groups + g0 + 2 * ch0;
+    wp[j] = w + at * 32 + (lane & 3) * 16;
+    sp[j] = a.group_scale + at;
+  }
+  const bool pairs = (groups & 1) == 0 && (reinterpret_cast<uintptr_t>(a.group_scale) & 3) == 0;  // scales two at a time
+  // up to which chunk there are this lane's group, and two groups
+  const int lane_end = min(end, (my_groups - ((lane >> 1) & 1) + 1) / 2), two_end = min(end, my_groups / 2);
+  auto fetch = [&](int st, int c) {  // chunk c + st, where the pointers stand at chunk c
 #pragma unroll
-    for (int j = 0; j < 2 * RT; j++) s_off[j] = (uint32_t)min(c0 + j * 8 + (lane >> 2), n - 1) * (uint32_t)groups;
-  };
-  auto fetch = [&](int st) {
-    if (f_item < items) {
-      const int gw = f_kb * KB_GROUPS + ((lane & 7) >> 1), gs = f_kb * KB_GROUPS + (lane & 3);
-      const uint8_t* wp = w + (int64_t)(g0 + (gw < my_groups ? gw : 0)) * 32 + (lane & 1) * 16;
-      const uint16_t* sp = a.group_scale + g0 + (gs < my_groups ? gs : 0);
-#pragma unroll
-      for (int i = 0; i < ROWS / 4; i++) cp_async16(lane_dst + st * STAGE + i * 512, wp + (uint64_t)w_off[i] * 16);
-#pragma unroll
-      for (int j = 0; j < 2 * RT; j++) sc[st][j] = sp[s_off[j]];
-      f_item++;
-      f_kb += WARPS;
-      if (f_kb >= kbs) {
-        f_kb = warp;
-        f_pair++;
-        place();
+    for (int j = 0; j < 2 * RT; j++) {
+      if (c + st < lane_end) wq[st][j] = load_once16(wp[j] + st * 64);
+      if (pairs) {
+        if (c + st < end) sc[st][j] = __ldg(reinterpret_cast<const uint32_t*>(sp[j] + 2 * st));
+      } else {
+        if (c + st < end) sc[st][j] = __ldg(sp[j] + 2 * st);
+        if (c + st < two_end) sc[st][j] |= (uint32_t)__ldg(sp[j] + 2 * st + 1) << 16;
       }
     }
-    cp_async_commit();
   };
-  place();
 #pragma unroll
-  for (int d = 0; d < DEPTH; d++) fetch(d);
+  for (int d = 0; d < DEPTH; d++) {
+#pragma unroll
+    for (int j = 0; j < 2 * RT; j++) wq[d][j] = make_uint4(0, 0, 0, 0), sc[d][j] = 0;
+    fetch(d, ch0);
+  }
+  for (int u = threadIdx.x; u < NOTHING / 16; u += THREADS) reinterpret_cast<uint4*>(smem)[u] = make_uint4(0, 0, 0, 0);
 
-  // x: units of 16 values (a lane's share of a group in a tile). First as they are, with the rows' maxima; then scaled,
-  // as f16 pairs (v, v + 4) in the order of the codes, with the sums of each group.
-  const int units_row = kbs * KB / 16, units = m * units_row;
-  __syncthreads();
-  {
-    const char* src = static_cast<const char*>(x) + (int64_t)g0 * 64 * XB;
-    const bool wide = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)(a.x_stride * XB)) & 15) == 0;
-    for (int base = 0; base < units; base += THREADS) {
-      const int u = base + threadIdx.x;
-      const int i = min(u / units_row, m - 1), e = u - i * units_row;
-      uint32_t top = 0;
+  // x: units of 16 values (half of a lane's share of a chunk), four neighbouring lanes a group: scaled, and as f16 pairs
+  // (v, v + 4) in the order of the codes, with the sum of each group.
+  const int units_row = chunks * CHUNK / 16, units = m * units_row;
+  const char* src = static_cast<const char*>(x) + (int64_t)g0 * 64 * XB;
+  const bool wide = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)(a.x_stride * XB)) & 15) == 0;
+  for (int u0 = 0; u0 < units; u0 += THREADS) {
+    const int u = u0 + threadIdx.x;
+    const int i = min(u / units_row, m - 1), e = u - i * units_row;
+    uint32_t t[4 * XB];  // the values as they are
+#pragma unroll
+    for (int j = 0; j < 4 * XB; j++) t[j] = 0;
+    if (u < units && e * 16 < my_groups * 64) {
+      const char* from = src + ((int64_t)i * a.x_stride + e * 16) * XB;
+      if (wide) {
+#pragma unroll
+        for (int j = 0; j < XB; j++) {
+          const uint4 q = reinterpret_cast<const uint4*>(from)[j];
+          t[4 * j] = q.x, t[4 * j + 1] = q.y, t[4 * j + 2] = q.z, t[4 * j + 3] = q.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4 * XB; j++) {
+          if constexpr (XB == 4) t[j] = reinterpret_cast<const uint32_t*>(from)[j];
+          else t[j] = reinterpret_cast<const uint16_t*>(from)[2 * j] |
+                      (uint32_t)reinterpret_cast<const uint16_t*>(from)[2 * j + 1] << 16;
+        }
+      }
+    }
+    uint32_t top = 0;  // the largest magnitude's bits (bf16: of the halves, then as f32)
+#pragma unroll
+    for (int j = 0; j < 4 * XB; j++) top = XB == 4 ? max(top, t[j] & 0x7fffffffu) : __vmaxu2(top, t[j] & 0x7fff7fffu);
+    if (XB == 2) top = max(top & 0xffff0000u, top << 16);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    float v[16], sum[PIECES];
+#pragma unroll
+    for (int j = 0; j < 4 * XB; j++) {
+      if constexpr (XB == 4) {
+        v[j] = __uint_as_float(t[j]);
+      } else {
+        v[2 * j] = __uint_as_float(t[j] << 16);
+        v[2 * j + 1] = __uint_as_float(t[j] & 0xffff0000u);
+      }
+    }
+    // 2^E of the maximum in [2^E, 2^(E + 1)); below 2^-111 the values are first brought up by 2^64
+    uint32_t ex = top >> 23;
+    float power = __uint_as_float(min(ex, 254u) << 23);
+    if (ex < 16u) {
+#pragma unroll
+      for (int j = 0; j < 16; j++) v[j] *= 18446744073709551616.f;
+      ex = max(__float_as_uint(__uint_as_float(top) * 18446744073709551616.f) >> 23, 16u);
+      power = __uint_as_float(ex << 23) * 5.421010862427522e-20f;
+    }
+    const float up = __uint_as_float((269u - min(ex, 254u)) << 23);  // 2^(15 - E)
+#pragma unroll
+    for (int j = 0; j < 16; j++) v[j] *= up;
+    uint8_t* to = xs + i * p.x_pitch + (e >> 3) * 256 + (e & 1) * 128 + ((e >> 1) & 3) * 16;
+#pragma unroll
+    for (int c = 0; c < PIECES; c++) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; j++) s += v[j];
+      uint32_t o[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {  // pair (8 (j / 4) + j % 4, + 4); odd j: x / 16
+        float *l = v + (j >> 2) * 8 + (j & 3), *h = l + 4;
+        const float down = (j & 1) ? 0.0625f : 1.f, back = (j & 1) ? 16.f : 1.f;
+        if (c + 1 < PIECES) {  // the leading bits toward zero (2^16 is never reached), and what is left (below 2^5) times 2^10
+          o[j] = as_u32(__halves2half2(__float2half_rz(*l * down), __float2half_rz(*h * down)));
+          const float2 f = unpack_f16x2(o[j]);
+          *l -= f.x * back, *h -= f.y * back;
+          s -= *l + *h;
+          *l *= 1024.f, *h *= 1024.f;
+        } else {
+          o[j] = as_u32(__floats2half2_rn(*l * down, *h * down));
+        }
+      }
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
       if (u < units) {
-        uint4 v[XB];
+        uint4* piece = reinterpret_cast<uint4*>(to + c * m * p.x_pitch);
+        piece[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        piece[4] = make_uint4(o[4], o[5], o[6], o[7]);
+        if ((e & 3) == 0) {  // group (e / 4) % 2 of chunk e / 8; an infinity or NaN makes its row NaN
+          float* at = reinterpret_cast<float*>(base + (e >> 3) * TOKS + i + c * m) + ((e >> 2) & 1);
+          at[0] = ex == 255u ? __uint_as_float(0x7fc00000u) : s * -4.76837158203125e-07f;  // -8 2^-24
+          at[2] = power * (c ? 9.765625e-4f : 1.f);
+        }
+      }
+    }
+  }
+  if (toks < TOKS)  // places without a token
+    for (int u = threadIdx.x; u < chunks * (TOKS - toks); u += THREADS)
+      base[u / (TOKS - toks) * TOKS + toks + u % (TOKS - toks)] = make_float4(0.f, 0.f, 0.f, 0.f);
+  __syncthreads();
+
+  float acc[RT][NT][2];  // channels lane / 4 and + 8 of a row tile, token piece 4 nt + lane % 4
 #pragma unroll
-        for (int j = 0; j < XB; j++) v[j] = make_uint4(0, 0, 0, 0);
-        if (e * 16 < my_groups * 64) {
-          const char* from = src + ((int64_t)i * a.x_stride + e * 16) * XB;
+  for (int r = 0; r < RT; r++)
 #pragma unroll
-          for (int j = 0; j < XB; j++) {
-            if (wide) {
-              v[j] = reinterpret_cast<const uint4*>(from)[j];
-            } else {
-              uint32_t t[4];
+    for (int t = 0; t < NT; t++) acc[r][t][0] = acc[r][t][1] = 0.f;
+  // This lane's column holds a token only where its values belong to the column's group; other lanes read zeros.
+  const uint8_t* bp[NT];
+  int b_step[NT];
 #pragma unroll
-              for (int q = 0; q < 4; q++) {
-                if constexpr (XB == 4) t[q] = reinterpret_cast<const uint32_t*>(from)[4 * j + q];
-                else t[q] = reinterpret_cast<const uint16_t*>(from)[8 * j + 2 * q] |
-                            (uint32_t)reinterpret_cast<const uint16_t*>(from)[8 * j + 2 * q + 1] << 16;
-              }
-              v[j] = make_uint4(t[0], t[1], t[2], t[3]);
+  for (int t = 0; t < NT; t++) {
+    const int tok = t * 4 + (lane >> 3);
+    const bool some = ((lane >> 2) & 1) == ((lane >> 1) & 1) && tok < toks;
+    bp[t] = some ? xs + tok * p.x_pitch + ch0 * 256 + (lane & 3) * 16 : smem;
+    b_step[t] = some ? DEPTH * 256 : 0;
+  }
+  const float4* sp4 = base + ch0 * TOKS + (lane & 3);
+  // the masks in registers, so that a code pair is one operation with its other constant
+  uint32_t low = 0x000f000fu, high = 0x00f000f0u;
+  asm volatile("" : "+r"(low), "+r"(high));
+
+  for (int c0 = ch0; c0 < end; c0 += DEPTH) {
+#pragma unroll
+    for (int j = 0; j < 2 * RT; j++) wp[j] += DEPTH * 64, sp[j] += DEPTH * 2;  // DEPTH chunks on, fetched behind these
+#pragma unroll
+    for (int st = 0; st < DEPTH; st++) {
+      if (c0 + st < end) {
+        float d[RT][NT][4], e[RT][CHAINS == 2 ? NT : 1][4];  // one or two chains of products
+        float2 power[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          const float4 s = sp4[st * TOKS + t * 4];
+          power[t] = make_float2(s.z, s.w);
+#pragma unroll
+          for (int r = 0; r < RT; r++) {
+            d[r][t][0] = d[r][t][2] = s.x;
+            d[r][t][1] = d[r][t][3] = s.y;
+            if constexpr (CHAINS == 2) e[r][t][0] = e[r][t][1] = e[r][t][2] = e[r][t][3] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          uint4 b[NT];
+#pragma unroll
+          for (int t = 0; t < NT; t++) b[t] = *reinterpret_cast<const uint4*>(bp[t] + st * 256 + q * 64);
+#pragma unroll
+          for (int r = 0; r < RT; r++) {
+            const uint4 &l4 = wq[st][2 * r], &h4 = wq[st][2 * r + 1];
+            const uint32_t lo = q == 0 ? l4.x : q == 1 ? l4.y : q == 2 ? l4.z : l4.w, lo8 = lo >> 8;
+            const uint32_t hi = q == 0 ? h4.x : q == 1 ? h4.y : q == 2 ? h4.z : h4.w, hi8 = hi >> 8;
+            const uint32_t a0[4] = {and_xor(lo, low, 0x00080008u), and_xor(hi, low, 0x00080008u),
+                                    and_xor(lo, high, 0x00800080u), and_xor(hi, high, 0x00800080u)};
+            const uint32_t a1[4] = {and_xor(lo8, low, 0x00080008u), and_xor(hi8, low, 0x00080008u),
+                                    and_xor(lo8, high, 0x00800080u), and_xor(hi8, high, 0x00800080u)};
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+              mma_f16(d[r][t], a0, b[t].x, b[t].y);
+              mma_f16(CHAINS == 2 ? e[r][t] : d[r][t], a1, b[t].z, b[t].w);
             }
           }
         }
 #pragma unroll
-        for (int j = 0; j < XB; j++) {
-          const uint32_t t[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-#pragma unroll
-          for (int q = 0; q < 4; q++) {
-            if constexpr (XB == 4) top = max(top, t[q] & 0x7fffffffu);
-            else top = max(top, max((t[q] << 16) & 0x7fffffffu, t[q] & 0x7fff0000u));
-          }
-          *reinterpret_cast<uint4*>(xs + (i + (j >> 1) * m) * p.x_pitch + e * 32 + (j & 1) * 16) = v[j];
-        }
-      }
-      const int i0 = __shfl_sync(0xffffffffu, i, 0);
-      if (__all_sync(0xffffffffu, i == i0)) {
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0) atomicMax(&row_max[i0], top);
-      } else if (u < units) {
-        atomicMax(&row_max[i], top);
-      }
-    }
-  }
-  for (int u = threadIdx.x; u < kbs * KB_GROUPS * COLS; u += THREADS) start[u] = 0.f;  // columns without a token
-  __syncthreads();
-  for (int base = 0; base < units; base += THREADS) {
-    const int u = base + threadIdx.x;
-    const int i = min(u / units_row, m - 1), e = u - i * units_row;
-    float sum[PIECES];
-#pragma unroll
-    for (int c = 0; c < PIECES; c++) sum[c] = 0.f;
-    if (u < units) {
-      const uint32_t ex = min(max(row_max[i] >> 23, 16u), 254u);
-      const float up = __uint_as_float((269u - ex) << 23);  // 2^15 over the power of two of the maximum
-      float v[16];
-#pragma unroll
-      for (int j = 0; j < XB; j++) {
-        const uint4 q = *reinterpret_cast<const uint4*>(xs + (i + (j >> 1) * m) * p.x_pitch + e * 32 + (j & 1) * 16);
-        const uint32_t t[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int h = 0; h < 4; h++) {
-          if constexpr (XB == 4) {
-            v[4 * j + h] = __uint_as_float(t[h]) * up;
-          } else {
-            v[8 * j + 2 * h] = __uint_as_float(t[h] << 16) * up;
-            v[8 * j + 2 * h + 1] = __uint_as_float(t[h] & 0xffff0000u) * up;
-          }
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < PIECES; c++) {
-        uint32_t o[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {  // pair (8 (j / 4) + j % 4, + 4); odd j: x / 16
-          const int at = (j >> 2) * 8 + (j & 3);
-          const float down = (j & 1) ? 0.0625f : 1.f, back = (j & 1) ? 16.f : 1.f;
-          // the leading bits toward zero, so that 2^16 is never reached
-          const __half2 h = c + 1 < PIECES ? __halves2half2(__float2half_rz(v[at] * down), __float2half_rz(v[at + 4] * down))
-                                           : __floats2half2_rn(v[at] * down, v[at + 4] * down);
-          o[j] = *reinterpret_cast<const uint32_t*>(&h);
-          const float2 f = unpack_f16x2(o[j]);
-          sum[c] += f.x * back + f.y * back;
-          if (c + 1 < PIECES) {  // what is left (below 2^5), times 2^10; nothing of an infinity
-            v[at] = fabsf(v[at]) < 131072.f ? (v[at] - f.x * back) * 1024.f : 0.f;
-            v[at + 4] = fabsf(v[at + 4]) < 131072.f ? (v[at + 4] - f.y * back) * 1024.f : 0.f;
-          }
-        }
-        uint4* to = reinterpret_cast<uint4*>(xs + (i + c * m) * p.x_pitch + e * 32);
-        to[0] = make_uint4(o[0], o[1], o[2], o[3]);
-        to[1] = make_uint4(o[4], o[5], o[6], o[7]);
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < PIECES; c++) {
-      sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], 1);
-      sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], 2);
-      if (u < units && (e & 3) == 0) start[(e >> 2) * COLS + i + c * m] = sum[c] * -4.76837158203125e-07f;  // -8 2^-24
-    }
-  }
-  __syncthreads();
-
-  const int cols = m * PIECES;
-  float acc[RT][NT][4];
-  auto clear = [&] {
-#pragma unroll
-    for (int r = 0; r < RT; r++)
-#pragma unroll
-      for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc[r][t][e] = 0.f;
-  };
-  clear();
-
-  auto step = [&](int kb, int st) {  // the step's values are in stage st
-    const uint8_t* tile = smem + warp * DEPTH * STAGE + st * STAGE;
-#pragma unroll
-    for (int g = 0; g < KB_GROUPS; g++) {
-      const int gs = kb * KB_GROUPS + g;
-      uint4 b[NT][2];
-      float c[NT][4];
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-        const int col = t * 8 + (lane >> 2);
-        const uint4* src = reinterpret_cast<const uint4*>(xs + col * p.x_pitch + gs * 128 + (lane & 3) * 32);
-        b[t][0] = b[t][1] = make_uint4(0, 0, 0, 0);
-        if (col < cols) {
-          b[t][0] = src[0];
-          b[t][1] = src[1];
-        }
-        const float2 s = *reinterpret_cast<const float2*>(start + gs * COLS + t * 8 + (lane & 3) * 2);
-        c[t][0] = c[t][2] = s.x;
-        c[t][1] = c[t][3] = s.y;
-      }
-#pragma unroll
-      for (int r = 0; r < RT; r++) {
-        const int row = r * 16 + (lane >> 2);  // and row + 8 (the same swizzle)
-        const uint8_t* at = tile + row * 128 + ((g ^ (row & 3)) << 5) + (lane & 3) * 8;
-        const uint2 lo = *reinterpret_cast<const uint2*>(at);
-        const uint2 hi = *reinterpret_cast<const uint2*>(at + 8 * 128);
-        float d[NT][4];
-#pragma unroll
-        for (int s = 0; s < 4; s++) {
-          const uint32_t wl = (s < 2 ? lo.x : lo.y) >> ((s & 1) * 8), wh = (s < 2 ? hi.x : hi.y) >> ((s & 1) * 8);
-          const uint32_t av[4] = {(wl & 0x000f000fu) ^ 0x00080008u, (wh & 0x000f000fu) ^ 0x00080008u,
-                                  (wl & 0x00f000f0u) ^ 0x00800080u, (wh & 0x00f000f0u) ^ 0x00800080u};
+        for (int r = 0; r < RT; r++) {
+          // with 2^24 2^-15; the powers come last, in the addition, so that sums of tiny values are rounded once
+          const float2 s0 = __fmul2_rn(unpack_f16x2(sc[st][2 * r]), make_float2(512.f, 512.f));
+          const float2 s1 = __fmul2_rn(unpack_f16x2(sc[st][2 * r + 1]), make_float2(512.f, 512.f));
 #pragma unroll
           for (int t = 0; t < NT; t++) {
-            const uint4& bb = b[t][s >> 1];
-            mma_f16(d[t], av, (s & 1) ? bb.z : bb.x, (s & 1) ? bb.w : bb.y, s == 0 ? c[t] : d[t]);
+            float(&u)[4] = d[r][t];
+            if constexpr (CHAINS == 2) u[0] += e[r][t][0], u[1] += e[r][t][1], u[2] += e[r][t][2], u[3] += e[r][t][3];
+            acc[r][t][0] = fmaf(u[1] * s0.y, power[t].y, fmaf(u[0] * s0.x, power[t].x, acc[r][t][0]));
+            acc[r][t][1] = fmaf(u[3] * s1.y, power[t].y, fmaf(u[2] * s1.x, power[t].x, acc[r][t][1]));
           }
         }
-        const uint32_t both = __shfl_sync(0xffffffffu, sc[st][2 * r] | sc[st][2 * r + 1] << 16, (lane & ~3) | g);
-        const float2 s01 = unpack_f16x2(both);
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-          acc[r][t][0] = fmaf(s01.x, d[t][0], acc[r][t][0]);
-          acc[r][t][1] = fmaf(s01.x, d[t][1], acc[r][t][1]);
-          acc[r][t][2] = fmaf(s01.y, d[t][2], acc[r][t][2]);
-          acc[r][t][3] = fmaf(s01.y, d[t][3], acc[r][t][3]);
-        }
+        fetch(st, c0 + DEPTH);
       }
     }
-  };
-
-  // The pair's sums over this CTA's part of k: the warps' sums in turn, a token's pieces, and its power of two back.
-  auto reduce = [&](int pr) {
-    float* mine = red + warp * (ROWS * COLS);
-    __syncthreads();  // the pair before has been read
 #pragma unroll
-    for (int r = 0; r < RT; r++)
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-        const int row = r * 16 + (lane >> 2), col = t * 8 + (lane & 3) * 2;
-        *reinterpret_cast<float2*>(mine + row * COLS + col) = make_float2(acc[r][t][0], acc[r][t][1]);
-        *reinterpret_cast<float2*>(mine + (row + 8) * COLS + col) = make_float2(acc[r][t][2], acc[r][t][3]);
-      }
-    __syncthreads();
-    for (int u = threadIdx.x; u < ROWS * m; u += THREADS) {
-      const int row = u / m, i = u - row * m;
-      float v = 0.f;
-#pragma unroll
-      for (int c = PIECES - 1; c >= 0; c--) {
-        float s = 0.f;
-#pragma unroll
-        for (int k = 0; k < WARPS; k++) s += red[k * (ROWS * COLS) + row * COLS + c * m + i];
-        v = c ? s * 9.765625e-4f : v + s;  // 2^-10
-      }
-      const uint32_t ex = min(max(row_max[i] >> 23, 16u), 254u);
-      part[pr * (ROWS * m) + u] = v * 512.f * __uint_as_float(ex << 23);  // 2^24 2^-15 2^(ex - 127)
-    }
-  };
-
-  int pr = 0, left = my_kbs;  // the pair in work and its steps left (a warp without steps only joins the barriers)
-  for (int base = 0; base < items; base += DEPTH) {
-#pragma unroll
-    for (int d = 0; d < DEPTH; d++) {
-      if (base + d < items) {
-        cp_async_wait<DEPTH - 1>();
-        __syncwarp();
-        step(warp + (my_kbs - left) * WARPS, d);
-        __syncwarp();
-        fetch(d);
-        if (--left == 0) {
-          reduce(pr);
-          clear();
-          pr++;
-          left = my_kbs;
-        }
-      }
-    }
+    for (int t = 0; t < NT; t++) bp[t] += b_step[t];
+    sp4 += DEPTH * TOKS;
   }
-  if (items == 0)
-    for (; pr < pairs; pr++) reduce(pr);
+
+  // The sums over this CTA's part of k: the warps' parts in turn, a token's pieces.
+#pragma unroll
+  for (int r = 0; r < RT; r++)
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const int at = (warp * ROWS + r * 16 + (lane >> 2)) * TOKS + t * 4 + (lane & 3);
+      red[at] = acc[r][t][0];
+      red[at + 8 * TOKS] = acc[r][t][1];
+    }
   __syncthreads();
-
-  // the cluster's parts in rank order; rank q finishes the pairs q, q + size, ...
-  const int size = p.cluster;
-  if (size > 1) tc::cluster_sync_all();
-  const uint32_t part_addr = tc::smem_u32(part);
-  for (int q = rank; q < pairs; q += size) {
-    for (int u = threadIdx.x; u < ROWS * m; u += THREADS) {
-      const int i = u / ROWS, row = u - i * ROWS, c = (pair0 + q) * ROWS + row;
-      if (c >= n) continue;
-      const int at = q * (ROWS * m) + row * m + i;
-      float v = 0.f;
-      if (size == 1) {
-        v = part[at];
-      } else {
-        for (int s = 0; s < size; s++) {
-          float o;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(tc::map_rank(part_addr + 4u * at, s)));
-          v += o;
-        }
-      }
-      matvec_store(v, a, i, c, y);
-    }
+  const int outs = cta_rows * m;
+  for (int u = threadIdx.x; u < outs; u += THREADS) {
+    const int i = u / cta_rows, row = u - i * cta_rows;
+    const float* from = red + (row / ROWS * p.wk * ROWS + row % ROWS) * TOKS + i;
+    float v = 0.f;
+#pragma unroll
+    for (int c = PIECES - 1; c >= 0; c--)
+      for (int k = 0; k < p.wk; k++) v += from[k * (ROWS * TOKS) + c * m];
+    if (p.cluster > 1) part[u] = v;
+    else if (first + row < n) matvec_store(v, a, i, first + row, y);
   }
-  if (size > 1) tc::cluster_sync_all();  // no CTA leaves while another reads its part
+  if (p.cluster > 1) {  // the cluster's parts in rank order, each CTA a share of the outputs
+    tc::cluster_sync_all();
+    const uint32_t part_addr = tc::smem_u32(part);
+    for (int u = rank * THREADS + threadIdx.x; u < outs; u += p.cluster * THREADS) {
+      const int i = u / cta_rows, channel = first + u - i * cta_rows;
+      if (channel >= n) continue;
+      float v = 0.f;
+      for (int s = 0; s < p.cluster; s++) {
+        float o;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(tc::map_rank(part_addr + 4u * u, s)));
+        v += o;
+      }
+      matvec_store(v, a, i, channel, y);
+    }
+    tc::cluster_sync_all();  // no CTA leaves while another reads its part
+  }
 }
 
-template <int XT, int NT>
+template <int XT, int NT, int RT, int PER_SM>
 static cudaError_t matvec_mma(const void* x, const uint8_t* w, void* y, const MatmulArgs& a, const mv::Plan& p, int groups_y,
                               cudaStream_t st) {
-  auto kern = matvec_mma_kernel<XT, NT>;
+  auto kern = matvec_mma_kernel<XT, NT, RT, PER_SM>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -464,47 +431,50 @@ cudaError_t launch_matvec(const void* x, const void* wv, void* y, const MatmulAr
   using namespace mv;
   const uint8_t* w = static_cast<const uint8_t*>(wv);
   const bool f32 = a.x_dtype == WE_F32;
-  const int cols = (int)a.m * (f32 ? 2 : 1);
-  const int nt = (cols + 7) / 8;
-  const int64_t all_pairs = (a.n + ROWS - 1) / ROWS, kbs = (a.k + KB - 1) / KB;
+  const int toks = (int)a.m * (f32 ? 2 : 1);
+  const int nt = toks <= 4 ? 1 : (toks <= 8 ? 2 : (toks <= 16 ? 4 : 8));
+  const int per_sm = nt == 8 ? 1 : 2, rt = nt <= 2 ? 2 : 1;  // the instances below
+  const int64_t chunks = (a.k + CHUNK - 1) / CHUNK, tiles = (a.n + rt * 16 - 1) / (rt * 16);
+  // How k is split over clusters and warps: the shortest chain of instructions of an SM's warp slot (its share of x's
+  // layout, its steps, its sums and the cluster's, for as many waves of CTAs as it takes).
   Plan p{};
-  auto fill = [&](int cluster, int64_t pairs, int64_t limit) {
-    p.cluster = cluster;
-    p.pairs = (int)pairs;
-    p.kb_per_cta = (int)((kbs + cluster - 1) / cluster);
-    // columns 16 bytes past a multiple of 128: two columns' 16-byte reads fall into different banks
-    p.x_pitch = p.kb_per_cta * KB * 2 + 16;
-    const int64_t bytes = RING + cols * (int64_t)p.x_pitch +
-                          ((p.kb_per_cta * KB_GROUPS + WARPS * ROWS) * nt * 8 + pairs * ROWS * a.m) * 4;
-    p.smem = (int)std::min<int64_t>(bytes, 1 << 30);
-    return bytes <= limit;
-  };
-  // The fewest CTAs that split k (1, 2, 4, 8) which give every SM one, and more where x needs it for two CTAs (or else
-  // one) an SM; then as many tile pairs a CTA as put the whole product in one wave.
-  int least = 1;
-  while (least < MAX_CLUSTER && least * WARPS < kbs && all_pairs * least < sms) least *= 2;
-  bool ok = false;
-  for (int per_sm = 2; per_sm >= 1 && !ok; per_sm--)
-    for (int cluster = least; cluster <= MAX_CLUSTER && !ok; cluster *= 2) {
-      const int64_t slots = std::max<int64_t>(1, (int64_t)sms * per_sm / cluster);
-      ok = fill(cluster, std::min<int64_t>(MAX_PAIRS, (all_pairs + slots - 1) / slots), (per_sm == 2 ? 113 : 226) * 1024);
+  int64_t best = -1;
+  for (int cluster = 1; cluster <= MAX_CLUSTER; cluster *= 2)
+    for (int wk = 1; wk <= WARPS; wk *= 2) {
+      const int64_t per_cta = (chunks + cluster - 1) / cluster;
+      const int64_t depth = IN_FLIGHT / rt, blocks = (per_cta + depth - 1) / depth;
+      if (wk > 1 && wk > blocks) break;
+      const int64_t rows = WARPS / wk * rt * 16, ctas = (tiles * wk + WARPS - 1) / WARPS * cluster;
+      const int64_t waves = (ctas + sms * per_sm - 1) / (sms * per_sm);
+      const int64_t bytes = NOTHING + toks * per_cta * CHUNK * 2 +
+                            (per_cta * nt * 16 + WARPS * rt * 16 * nt * 4 + (cluster > 1 ? rows * a.m : 0)) * 4;
+      if (bytes > 226 * 1024 / per_sm) continue;
+      const int64_t units = (a.m * per_cta * 8 + THREADS - 1) / THREADS, outs = (rows * a.m + THREADS - 1) / THREADS;
+      const int64_t cost = waves * (300 + units * (f32 ? 250 : 110) + (blocks + wk - 1) / wk * depth * rt * (70 + 20 * nt) +
+                                    outs * (30 + 4 * wk) + (cluster > 1 ? 300 : 0));
+      if (best >= 0 && cost >= best) continue;
+      best = cost;
+      p = Plan{wk, cluster, (int)per_cta, (int)per_cta * CHUNK * 2, (int)bytes};
     }
-  // offsets of weights are held as 32 bits, in 16 bytes
-  if (!ok || (all_pairs + p.pairs - 1) / p.pairs > 65535 || a.n * (a.k / 32) > 0xffffffffLL) {
+  const bool ok = best >= 0;
+  const int64_t cta_rows = ok ? WARPS / p.wk * rt * 16 : 1, gy = (a.n + cta_rows - 1) / cta_rows;
+  if (!ok || gy > 65535) {
     const dim3 grid((unsigned)((a.n + 7) / 8));
     const cudaError_t e = f32 ? launch_pdl(matvec_long_kernel<WE_F32>, grid, 256, 0, st, x, w, y, a)
                               : launch_pdl(matvec_long_kernel<WE_BF16>, grid, 256, 0, st, x, w, y, a);
     return e == cudaSuccess ? cudaGetLastError() : e;
   }
-  const int gy = (int)((all_pairs + p.pairs - 1) / p.pairs);
+  const int ny = (int)gy;
   cudaError_t e;
   if (f32) {
-    e = nt == 1   ? matvec_mma<WE_F32, 1>(x, w, y, a, p, gy, st)
-        : nt == 2 ? matvec_mma<WE_F32, 2>(x, w, y, a, p, gy, st)
-        : nt == 3 ? matvec_mma<WE_F32, 3>(x, w, y, a, p, gy, st)
-                  : matvec_mma<WE_F32, 4>(x, w, y, a, p, gy, st);
+    e = nt == 1   ? matvec_mma<WE_F32, 1, 2, 2>(x, w, y, a, p, ny, st)
+        : nt == 2 ? matvec_mma<WE_F32, 2, 2, 2>(x, w, y, a, p, ny, st)
+        : nt == 4 ? matvec_mma<WE_F32, 4, 1, 2>(x, w, y, a, p, ny, st)
+                  : matvec_mma<WE_F32, 8, 1, 1>(x, w, y, a, p, ny, st);
   } else {
-    e = nt == 1 ? matvec_mma<WE_BF16, 1>(x, w, y, a, p, gy, st) : matvec_mma<WE_BF16, 2>(x, w, y, a, p, gy, st);
+    e = nt == 1   ? matvec_mma<WE_BF16, 1, 2, 2>(x, w, y, a, p, ny, st)
+        : nt == 2 ? matvec_mma<WE_BF16, 2, 2, 2>(x, w, y, a, p, ny, st)
+                  : matvec_mma<WE_BF16, 4, 1, 2>(x, w, y, a, p, ny, st);
   }
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
