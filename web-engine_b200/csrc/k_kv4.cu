@@ -1,4 +1,6 @@
 // A paged 4-bit K/V cache (we_kv4_cache): rows in, rows out, and the attention of a step's new tokens over it.
+#include <algorithm>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -91,50 +93,542 @@ __global__ void kv4_advance_kernel(int32_t* lengths, int64_t batch, int32_t toke
     if (lengths[b] >= 0) lengths[b] += tokens;
 }
 
-// One warp per (sequence, token, head): online softmax over the keys, a lane holding dims 2 lane, 2 lane + 1 of each 64.
-template <int DT, int OT, int D>
-__global__ void __launch_bounds__(128) kv4_attention_simple_kernel(const Kv4AttnArgs a, uint32_t* err) {
-  pdl_wait();
+// ---------------- attention ----------------
+// Per (sequence, kv head): q rows (the new tokens times the heads of the group) over that head's keys. The cache is read
+// once and bounds the call (dim / 2 + dim / 32 bytes per key, for k and for v); the products run on 16 x 8 x 16 tensor
+// tiles with KEYS (for v: dims) as the 16 rows and up to 8 q rows as the columns, so a tile has no more idle rows than
+// the group leaves of 8, and the codes go from the registers they are unpacked in straight into the tile:
+// - S^T = K Q^T. A lane holds 16 codes of 2 keys; a pair of codes becomes the f16 subnormals u 2^-24, u = q + 8, by one
+//   logical operation (and u 2^-20 for the next nibble, whose q is divided by 16); the sum of a group of 64 starts at
+//   -8 sum(q). The key's scale multiplies the group's sum in f32.
+// - O^T = V^T P^T. Two keys' words are interleaved by byte permutations, so that a pair is the same dim of two keys; p
+//   times the key's scale of v, times a power of two that keeps it in f16's range (2^15 at most), is the other operand,
+//   turned by movmatrix from S^T's layout. The offset 8 is taken out at the end with the sum of those weights, which one
+//   more tile of ones accumulates.
+// - f32 q or out (TERMS = 2): q and the weights are two f16 terms each (22 bits), and codes of v become exact signed f16
+//   by one more operation, because weights are all positive and the offset's sum would cost 3 to 5 bits.
+// - A warp takes 16 or 32 keys at a time through a ring of its own (cp.async), with its own running maximum; the O and
+//   sums are only rescaled when the maximum grows by more than 2^8 or v's scales outgrow their power of two. The 4 warps
+//   of a CTA and then the CTAs that split a long sequence are merged in a fixed order; the last CTA to finish merges.
+namespace kv {
+constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int MAX_SPLITS = 64;
+
+struct Params {
+  we_kv4_cache c;
+  const void* q;
+  void* out;
+  int tokens, heads, group, rows;  // group: heads per kv head; rows = tokens * group
+  int row_tiles;                   // tiles of 8 NQ rows
+  int chunk;                       // keys per CTA
+  int64_t q_stride, out_stride;
+  float scale_log2;
+  int dtype, out_dtype;
+  float* part;                     // [sequence, kv head, row tile][splits][8 NQ](dim values, maximum, sum), when split
+  uint32_t* done;                  // [sequence, kv head, row tile]: CTAs that have written, zero between calls
+  uint32_t* err;
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t and_xor(uint32_t v, uint32_t mask, uint32_t flip) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(v), "r"(mask), "r"(flip));
+  return r;
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {  // of an 8 x 8 f16 tile
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+__device__ __forceinline__ float2 halves(uint32_t u) { return __half22float2(as_half2(u)); }
+
+// Where the 32 bytes of group g of row `row` (0..15) of a tile lie: so that the rows that lanes read together
+// ({0 4 1 5}, {2 6 3 7} for k, {0 1 2 3}, {4 5 6 7} for v, and 8 more) are on different banks.
+template <int D>
+__device__ __forceinline__ int segment(int row, int g) {
+  const int h = (row & 1) | ((((row >> 1) ^ (row >> 2)) & 1) << 1);
+  if (D == 64) return ((row >> 2) * 4 + h) * 32;
+  if (D == 128) return ((row >> 1) * 4 + (row & 1) * 2 + (g ^ (h >> 1))) * 32;
+  return (row * 4 + (g ^ h)) * 32;
+}
+}  // namespace kv
+
+// D: dim; NQ: tiles of 8 q rows; KT: tiles of 16 keys of a step; TERMS: f16 terms of q and of the weights.
+template <int D, int NQ, int KT, int TERMS>
+__global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Params p) {
+  using namespace kv;
+  constexpr int G = D / 64, STEP = KT * 16, ROW = D / 2, TILE = 16 * ROW, QROWS = 8 * NQ;
+  constexpr int STAGE = KT * (2 * TILE + 2 * 16 * G * 2), DEPTH = 3;
+  constexpr int MTILES = D / 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3, u = lane >> 2;
+  const int split = blockIdx.x, b = blockIdx.z;
+  const int head = blockIdx.y / p.row_tiles, rtile = blockIdx.y % p.row_tiles;  // kv head, tile of q rows
+  const int unit = (b * gridDim.y) + blockIdx.y;
   pdl_launch_dependents();
-  constexpr int G = D / 64;
-  const we_kv4_cache& c = a.c;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= c.batch * a.tokens * a.heads) return;
-  const int64_t bt = row / a.heads, h = row % a.heads, b = bt / a.tokens, i = bt % a.tokens;
-  const int64_t kvh = h / (a.heads / c.kv_heads), have = c.lengths[b];
-  float q[2 * G], o[2 * G], m = -INFINITY, l = 0.f;
+  pdl_wait();
+
+  const int have = p.c.lengths[b];
+  const int64_t room = p.c.max_pages * p.c.page;
+  const int64_t want = (int64_t)have + min(p.tokens, (rtile * QROWS + QROWS - 1) / p.group + 1);  // keys of the tile's last row
+  const int keys = have < 0 ? 0 : (int)min(want, room);
+  if (have >= 0 && want > room && split == 0 && threadIdx.x == 0) atomicCAS(p.err, 0u, (uint32_t)DEV_ERR_KV_FULL);
+  const int splits = max(1, (keys + p.chunk - 1) / p.chunk);
+  if (split >= splits) return;
+  const int key0 = split * p.chunk, key1 = min(keys, key0 + p.chunk);
+
+  // this warp's steps: key0 + (warp + WARPS i) STEP
+  const int steps = (key1 - key0 + STEP - 1) / STEP;
+  const int mine = steps > warp ? (steps - warp + WARPS - 1) / WARPS : 0;
+  uint8_t* ring = smem + warp * (DEPTH * STAGE);
+  const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
+
+  // Page ids of this warp's next 32 tiles of 16 keys, a lane each; -1: not there.
+  int ids = -1;
+  const int page = (int)p.c.page;
+  auto load_ids = [&](int i) {  // from step i on
+    const int tile = i * KT + lane, key = key0 + (warp + WARPS * (tile / KT)) * STEP + (tile % KT) * 16;
+    ids = -1;
+    if (key < key1) {
+      ids = p.c.page_table[(int64_t)b * p.c.max_pages + key / page];
+      if (ids < 0 || ids >= p.c.pages) {
+        atomicCAS(p.err, 0u, (uint32_t)DEV_ERR_KV_PAGE);
+        ids = -1;
+      }
+    }
+  };
+  uint32_t there = 0;  // bit per tile of the ring's stages: its page exists
+  auto copy = [&](int i) {
+    if (i < mine) {
+      if ((i * KT) % 32 == 0) load_ids(i);
+      const uint32_t to = ring_addr + (i % DEPTH) * STAGE;
 #pragma unroll
-  for (int e = 0; e < 2 * G; e++) {
-    q[e] = load_act<DT>(a.q, bt * a.q_stride + h * D + (e / 2) * 64 + 2 * lane + (e & 1)) * a.scale;
-    o[e] = 0.f;
-  }
-  const int64_t keys = have < 0 ? 0 : have + i + 1;
-  for (int64_t t = 0; t < keys; t++) {
-    const int64_t r = kv4_row(c, b, kvh, t, err);
-    if (r < 0) continue;
-    float dot = 0.f, vv[2 * G];
+      for (int t = 0; t < KT; t++) {
+        const int id = __shfl_sync(0xffffffffu, ids, (i * KT + t) & 31);
+        const uint32_t bit = 1u << ((i % DEPTH) * KT + t);
+        there = id >= 0 ? there | bit : there & ~bit;
+        if (id < 0) continue;
+        const int key = key0 + (warp + WARPS * i) * STEP + t * 16;
+        const int64_t row = ((int64_t)id * p.c.kv_heads + head) * page + key % page;
+#pragma unroll
+        for (int side = 0; side < 2; side++) {
+          const uint8_t* from = (side ? p.c.v : p.c.k) + row * ROW;
+          const uint32_t dst = to + (t * 2 + side) * TILE;
+#pragma unroll
+          for (int j = 0; j < TILE / 512; j++) {
+            const int at = j * 32 + lane, r = at / (ROW / 16), ch = at % (ROW / 16);  // 16-byte piece `ch` of row r
+            cp_async16(dst + segment<D>(r, ch >> 1) + (ch & 1) * 16, from + at * 16);
+          }
+        }
+        // scales: 4-byte words, 8 G of k then 8 G of v
+        if (16 * G >= 32 || lane < 16 * G) {
+#pragma unroll
+          for (int j = 0; j < (16 * G + 31) / 32; j++) {
+            const int at = j * 32 + lane, side = at / (8 * G), word = at % (8 * G);
+            const uint16_t* from = (side ? p.c.v_scale : p.c.k_scale) + row * G + word * 2;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + KT * 2 * TILE + t * (64 * G) + at * 4), "l"(from)
+                         : "memory");
+          }
+        }
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < DEPTH - 1; i++) copy(i);
+
+  // q as the B operand: column lane / 4 of tile nq is row nq * 8 + lane / 4; of a group's 8 words a lane holds words 2 c and
+  // 2 c + 1 in the order of the codes: for word w and half h the pairs (q0, q4), (q1, q5) / 16 or (q2, q6), (q3, q7) / 16,
+  // times a power of two that brings the row's largest to 2^15.
+  uint32_t qf[NQ][G][4][2][TERMS];
+  float q_start[NQ][G][2], q_back[NQ][2];  // of the columns of S^T that a lane holds: 2 c, 2 c + 1
+#pragma unroll
+  for (int nq = 0; nq < NQ; nq++) {
+    const int r = rtile * QROWS + nq * 8 + u;
+    float x[G][16], top = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        x[g][e] = 0.f;
+        if (r < p.rows) {
+          const int64_t at = ((int64_t)b * p.tokens + r / p.group) * p.q_stride +
+                             (int64_t)(head * p.group + r % p.group) * D + g * 64 + c * 16 + e;
+          x[g][e] = p.dtype == WE_F32 ? static_cast<const float*>(p.q)[at] : bf16_bits_to_f32(static_cast<const uint16_t*>(p.q)[at]);
+        }
+        top = fmaxf(top, fabsf(x[g][e]));
+      }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const uint32_t ex = min(max(__float_as_uint(top) >> 23, 16u), 254u);
+    const float up = __uint_as_float((269u - ex) << 23);
+    float sum[G];
 #pragma unroll
     for (int g = 0; g < G; g++) {
-      const float ks = __half2float(__ushort_as_half(c.k_scale[r * G + g]));
-      const float vs = __half2float(__ushort_as_half(c.v_scale[r * G + g]));
-      const uint32_t kb = c.k[r * (D / 2) + g * 32 + lane], vb = c.v[r * (D / 2) + g * 32 + lane];
-      dot = fmaf((float)(int((kb & 15u) ^ 8u) - 8) * ks, q[2 * g], dot);
-      dot = fmaf((float)(int((kb >> 4) ^ 8u) - 8) * ks, q[2 * g + 1], dot);
-      vv[2 * g] = (float)(int((vb & 15u) ^ 8u) - 8) * vs;
-      vv[2 * g + 1] = (float)(int((vb >> 4) ^ 8u) - 8) * vs;
+      sum[g] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 2; w++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            const float down = k ? 0.0625f : 1.f;
+            float lo = x[g][w * 8 + h * 2 + k] * up, hi = x[g][w * 8 + h * 2 + k + 4] * up;
+            sum[g] += lo + hi;
+#pragma unroll
+            for (int t = 0; t < TERMS; t++) {
+              // the first of two terms toward zero, so that 2^16 is never reached
+              const __half2 v = t + 1 < TERMS ? __halves2half2(__float2half_rz(lo * down), __float2half_rz(hi * down))
+                                              : __floats2half2_rn(lo * down, hi * down);
+              qf[nq][g][w * 2 + h][k][t] = as_u32(v);
+              const float2 f = __half22float2(v);
+              lo -= f.x * (k ? 16.f : 1.f);
+              hi -= f.y * (k ? 16.f : 1.f);
+            }
+          }
+      sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
+      sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
     }
-    const float s = warp_sum(dot), mn = fmaxf(m, s);
-    const float corr = expf(m - mn), p = expf(s - mn);
-    l = l * corr + p;
+    const float back = p.scale_log2 * 512.f * __uint_as_float(ex << 23);  // 2^24 2^-15 2^E
 #pragma unroll
-    for (int e = 0; e < 2 * G; e++) o[e] = o[e] * corr + p * vv[e];
-    m = mn;
+    for (int k = 0; k < 2; k++) {
+      const int from = (c * 2 + k) * 4;
+      q_back[nq][k] = __shfl_sync(0xffffffffu, back, from);
+#pragma unroll
+      for (int g = 0; g < G; g++) q_start[nq][g][k] = __shfl_sync(0xffffffffu, sum[g], from) * -4.76837158203125e-07f;  // -8 2^-24
+    }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+
+  float o[NQ][MTILES][4], w_sum[NQ][G][4], m[NQ][2], l[NQ][2];
 #pragma unroll
-  for (int e = 0; e < 2 * G; e++)
-    store_out<OT>(a.out, bt * a.out_stride + h * D + (e / 2) * 64 + 2 * lane + (e & 1), o[e] * inv);
+  for (int nq = 0; nq < NQ; nq++) {
+#pragma unroll
+    for (int t = 0; t < MTILES; t++) o[nq][t][0] = o[nq][t][1] = o[nq][t][2] = o[nq][t][3] = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; g++) w_sum[nq][g][0] = w_sum[nq][g][1] = w_sum[nq][g][2] = w_sum[nq][g][3] = 0.f;
+    m[nq][0] = m[nq][1] = -INFINITY;
+    l[nq][0] = l[nq][1] = 0.f;
+  }
+  uint32_t v_top = 1u << 10;  // the largest scale of v so far, as f16 bits (at least the smallest normal one)
+  uint32_t low = 0x000f000fu, high = 0x00f000f0u;  // in registers: a pair of codes is one operation with its other constant
+  asm volatile("" : "+r"(low), "+r"(high));
+  const int full = have + (rtile * QROWS) / p.group + 1;  // keys below are seen by every row of the tile
+
+  for (int i = 0; i < mine; i++) {
+    copy(i + DEPTH - 1);
+    cp_async_wait<DEPTH - 1>();
+    __syncwarp();
+    const uint8_t* st = ring + (i % DEPTH) * STAGE;
+    const int first = key0 + (warp + WARPS * i) * STEP;
+    // S^T: rows are keys: row r of a tile is key r / 2 + 4 (r & 1) (+ 8)
+    float s[KT][NQ][4];
+    uint32_t vs[KT][2][(G + 1) / 2];  // scales of v of this lane's two keys
+#pragma unroll
+    for (int t = 0; t < KT; t++) {
+      const uint8_t* kt = st + (t * 2) * TILE;
+      const int k0 = (u >> 1) + 4 * (u & 1);  // this lane's key of the tile, and + 8
+      float d[NQ][G][4];
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) {
+          d[nq][g][0] = d[nq][g][2] = q_start[nq][g][0];
+          d[nq][g][1] = d[nq][g][3] = q_start[nq][g][1];
+        }
+        const uint2 a2 = *reinterpret_cast<const uint2*>(kt + segment<D>(k0, g) + c * 8);
+        const uint2 b2 = *reinterpret_cast<const uint2*>(kt + segment<D>(k0 + 8, g) + c * 8);
+#pragma unroll
+        for (int x = 0; x < 4; x++) {  // word x / 2, half x % 2
+          const uint32_t wa = (x < 2 ? a2.x : a2.y) >> ((x & 1) * 8), wb = (x < 2 ? b2.x : b2.y) >> ((x & 1) * 8);
+          const uint32_t av[4] = {and_xor(wa, low, 0x00080008u), and_xor(wb, low, 0x00080008u),
+                                  and_xor(wa, high, 0x00800080u), and_xor(wb, high, 0x00800080u)};
+#pragma unroll
+          for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+            for (int k = 0; k < TERMS; k++) mma_f16(d[nq][g], av, qf[nq][g][x][0][k], qf[nq][g][x][1][k]);
+        }
+      }
+      const bool page_there = (there >> ((i % DEPTH) * KT + t)) & 1;
+      const uint8_t* sc = st + KT * 2 * TILE + t * (64 * G);
+      float ks[2][G];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int key = k0 + 8 * h;
+        const bool valid = page_there && first + t * 16 + key < key1;
+        const uint8_t *kat = sc + key * (2 * G), *vat = kat + 32 * G;
+        if constexpr (G == 1) {
+          ks[h][0] = __half2float(__ushort_as_half(*reinterpret_cast<const uint16_t*>(kat)));
+          vs[t][h][0] = valid ? *reinterpret_cast<const uint16_t*>(vat) : 0u;
+        } else {
+#pragma unroll
+          for (int g = 0; g < G; g += 2) {
+            const float2 f = halves(*reinterpret_cast<const uint32_t*>(kat + g * 2));
+            ks[h][g] = f.x;
+            ks[h][g + 1] = f.y;
+            vs[t][h][g / 2] = valid ? *reinterpret_cast<const uint32_t*>(vat + g * 2) : 0u;
+          }
+        }
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            float x = d[nq][0][h * 2 + k] * ks[h][0];
+#pragma unroll
+            for (int g = 1; g < G; g++) x = fmaf(d[nq][g][h * 2 + k], ks[h][g], x);
+            x *= q_back[nq][k];
+            bool seen = valid;
+            if (first + STEP > full) {  // (uniform) some row stands before some key of the step
+              const int r = rtile * QROWS + nq * 8 + c * 2 + k;
+              seen = seen && first + t * 16 + key <= have + r / p.group;
+            }
+            s[t][nq][h * 2 + k] = seen ? x : -INFINITY;
+          }
+      }
+    }
+    // running maximum of each column, and of v's scales
+    bool grow = false;
+    float mt[NQ][2];
+#pragma unroll
+    for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        float x = fmaxf(s[0][nq][k], s[0][nq][2 + k]);
+#pragma unroll
+        for (int t = 1; t < KT; t++) x = fmaxf(x, fmaxf(s[t][nq][k], s[t][nq][2 + k]));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+        mt[nq][k] = x;
+        grow = grow || x > m[nq][k] + 8.f;
+      }
+    uint32_t vt = 0;
+#pragma unroll
+    for (int t = 0; t < KT; t++)
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int g = 0; g < (G + 1) / 2; g++) vt = __vmaxu2(vt, vs[t][h][g] & 0x7fff7fffu);
+    vt = __reduce_max_sync(0xffffffffu, max(vt & 0xffffu, vt >> 16));
+    const bool more = (vt >> 10) > (v_top >> 10);
+    if (__any_sync(0xffffffffu, grow) || more) {
+      // weights are kept times 2^(21 - exponent of the largest scale)
+      float f = 1.f;
+      if (more) {
+        f = __uint_as_float((127u + (v_top >> 10) - (vt >> 10)) << 23);
+        v_top = vt;
+      }
+#pragma unroll
+      for (int nq = 0; nq < NQ; nq++) {
+        float corr[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          corr[k] = 1.f;
+          if (mt[nq][k] > m[nq][k] + 8.f) {
+            corr[k] = ex2_ftz(m[nq][k] - mt[nq][k]);
+            m[nq][k] = mt[nq][k];
+          }
+          l[nq][k] *= corr[k];
+          corr[k] *= f;
+        }
+#pragma unroll
+        for (int t = 0; t < MTILES; t++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[nq][t][e] *= corr[e & 1];
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) w_sum[nq][g][e] *= corr[e & 1];
+      }
+    }
+    const float v_up = __uint_as_float((148u - (v_top >> 10)) << 23);  // 2^(21 - exponent field)
+#pragma unroll
+    for (int t = 0; t < KT; t++) {
+      float pw[NQ][4];
+#pragma unroll
+      for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float x = s[t][nq][e];
+          // a column that has seen nothing yet has m = -inf: no weight
+          pw[nq][e] = x == -INFINITY ? 0.f : ex2_ftz(x - m[nq][e & 1]);
+          l[nq][e & 1] += pw[nq][e];
+        }
+      const uint8_t* vt_ = st + (t * 2 + 1) * TILE;
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        // weights times scales as the B operand: S^T's rows (keys) become the 16 values of the product
+        uint32_t bw[NQ][TERMS][2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const uint32_t raw = vs[t][h][g / 2];
+          const float sv = __half2float(__ushort_as_half((uint16_t)((g & 1) ? raw >> 16 : raw))) * v_up;
+#pragma unroll
+          for (int nq = 0; nq < NQ; nq++) {
+            float x0 = pw[nq][h * 2] * sv, x1 = pw[nq][h * 2 + 1] * sv;
+#pragma unroll
+            for (int k = 0; k < TERMS; k++) {
+              const __half2 v = __floats2half2_rn(x0, x1);
+              bw[nq][k][h] = transposed(as_u32(v));
+              if (k + 1 < TERMS) {
+                const float2 f = __half22float2(v);
+                x0 -= f.x;
+                x1 -= f.y;
+              }
+            }
+          }
+        }
+        if constexpr (TERMS == 1) {
+          const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+#pragma unroll
+          for (int nq = 0; nq < NQ; nq++) mma_f16(w_sum[nq][g], ones, bw[nq][0][0], bw[nq][0][1]);
+        }
+        // v: word u (dims 8 u .. 8 u + 7 of the group) of the keys of rows 2 c, 2 c + 1, 2 c + 8, 2 c + 9
+        const uint32_t v0 = *reinterpret_cast<const uint32_t*>(vt_ + segment<D>(c, g) + u * 4);
+        const uint32_t v1 = *reinterpret_cast<const uint32_t*>(vt_ + segment<D>(c + 4, g) + u * 4);
+        const uint32_t v2 = *reinterpret_cast<const uint32_t*>(vt_ + segment<D>(c + 8, g) + u * 4);
+        const uint32_t v3 = *reinterpret_cast<const uint32_t*>(vt_ + segment<D>(c + 12, g) + u * 4);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {  // dims 8 u + 4 h ..
+          const uint32_t x = __byte_perm(v0, v1, h ? 0x7632 : 0x5410), y = __byte_perm(v2, v3, h ? 0x7632 : 0x5410);
+#pragma unroll
+          for (int j = 0; j < 2; j++) {  // rows u and u + 8 of the tile: dims 8 u + 4 h + 2 j and the next (for TERMS 1 times 16)
+            const uint32_t xs = x >> (8 * j), ys = y >> (8 * j);
+            uint32_t av[4];
+            if constexpr (TERMS == 1) {
+              av[0] = and_xor(xs, low, 0x00080008u), av[1] = and_xor(xs, high, 0x00800080u);
+              av[2] = and_xor(ys, low, 0x00080008u), av[3] = and_xor(ys, high, 0x00800080u);
+            } else {
+              // 1024 + u - 1032, and (1024 + 16 u) / 16 - 72: q exactly
+              const __half2 sub = __float2half2_rn(-1032.f), sixteenth = __float2half2_rn(0.0625f), sub2 = __float2half2_rn(-72.f);
+              av[0] = as_u32(__hadd2(as_half2(and_xor(xs, low, 0x64086408u)), sub));
+              av[1] = as_u32(__hfma2(as_half2(and_xor(xs, high, 0x64806480u)), sixteenth, sub2));
+              av[2] = as_u32(__hadd2(as_half2(and_xor(ys, low, 0x64086408u)), sub));
+              av[3] = as_u32(__hfma2(as_half2(and_xor(ys, high, 0x64806480u)), sixteenth, sub2));
+            }
+#pragma unroll
+            for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+              for (int k = 0; k < TERMS; k++) mma_f16(o[nq][g * 4 + h * 2 + j], av, bw[nq][k][0], bw[nq][k][1]);
+          }
+        }
+      }
+    }
+    __syncwarp();  // every lane has read the stage that is copied into next
+  }
+
+  // The warps' O, maxima and sums, merged in shared memory (the rings are done): [warp][row](D values, m, l)
+  cp_async_wait<0>();
+  __syncthreads();
+  constexpr int PITCH = D + 4;
+  float* mem = reinterpret_cast<float*>(smem);
+  const float v_down = __uint_as_float(((v_top >> 10) + 106u) << 23);  // 2^-(21 - exponent field)
+#pragma unroll
+  for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      float sum = l[nq][k];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      float* to = mem + (warp * QROWS + nq * 8 + c * 2 + k) * PITCH;
+#pragma unroll
+      for (int t = 0; t < MTILES; t++) {  // group t / 4, dims 8 u + 2 (t % 4) and the next
+        float x0 = o[nq][t][k], x1 = o[nq][t][2 + k];
+        if constexpr (TERMS == 1) {
+          const float off = 8.f * w_sum[nq][t / 4][k];
+          x0 = fmaf(x0, 16777216.f, -off);
+          x1 = fmaf(x1, 1048576.f, -off);
+        }
+        *reinterpret_cast<float2*>(to + (t / 4) * 64 + u * 8 + (t % 4) * 2) = make_float2(x0 * v_down, x1 * v_down);
+      }
+      if (u == 0) {
+        to[D] = m[nq][k];
+        to[D + 1] = sum;
+      }
+    }
+  __syncthreads();
+  float* part = p.part ? p.part + (int64_t)unit * gridDim.x * (QROWS * PITCH) : nullptr;
+  auto finish = [&](int r, int d, float4 acc, float sum) {  // 4 values of row r of the tile from dim d on
+    const int row = rtile * QROWS + r;
+    if (row >= p.rows) return;
+    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // no key seen: zeros; NaN stays
+    const int64_t at = ((int64_t)b * p.tokens + row / p.group) * p.out_stride + (int64_t)(head * p.group + row % p.group) * D + d;
+    const float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (p.out_dtype == WE_F32) store_out<WE_F32>(p.out, at + e, v[e]);
+      else store_out<WE_BF16>(p.out, at + e, v[e]);
+    }
+  };
+  for (int x = threadIdx.x; x < QROWS * (D / 4); x += THREADS) {
+    const int r = x / (D / 4), d = x % (D / 4) * 4;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) top = fmaxf(top, mem[(w * QROWS + r) * PITCH + D]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+      const float* from = mem + (w * QROWS + r) * PITCH;
+      if (from[D] == -INFINITY) continue;  // that warp saw no key of the row
+      const float f = ex2_ftz(from[D] - top);
+      const float4 v = *reinterpret_cast<const float4*>(from + d);
+      acc.x = fmaf(v.x, f, acc.x);
+      acc.y = fmaf(v.y, f, acc.y);
+      acc.z = fmaf(v.z, f, acc.z);
+      acc.w = fmaf(v.w, f, acc.w);
+      sum = fmaf(from[D + 1], f, sum);
+    }
+    if (splits == 1) {
+      finish(r, d, acc, sum);
+    } else {
+      float* to = part + ((int64_t)split * QROWS + r) * PITCH;
+      *reinterpret_cast<float4*>(to + d) = acc;
+      if (d == 0) {
+        to[D] = top;
+        to[D + 1] = sum;
+      }
+    }
+  }
+  if (splits == 1) return;
+  // the last CTA of the unit to get here merges all of its parts, in the order of the keys
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t before = atomicAdd(p.done + unit, 1u);
+    last = before == (uint32_t)splits - 1u;
+    if (last) p.done[unit] = 0u;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  for (int x = threadIdx.x; x < QROWS * (D / 4); x += THREADS) {
+    const int r = x / (D / 4), d = x % (D / 4) * 4;
+    if (rtile * QROWS + r >= p.rows) continue;
+    float top = -INFINITY;
+    for (int z = 0; z < splits; z++) top = fmaxf(top, part[((int64_t)z * QROWS + r) * PITCH + D]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll 8
+    for (int z = 0; z < splits; z++) {
+      const float* from = part + ((int64_t)z * QROWS + r) * PITCH;
+      const float f = from[D] == -INFINITY ? 0.f : ex2_ftz(from[D] - top);
+      const float4 v = *reinterpret_cast<const float4*>(from + d);
+      acc.x = fmaf(v.x, f, acc.x);
+      acc.y = fmaf(v.y, f, acc.y);
+      acc.z = fmaf(v.z, f, acc.z);
+      acc.w = fmaf(v.w, f, acc.w);
+      sum = fmaf(from[D + 1], f, sum);
+    }
+    finish(r, d, acc, sum);
+  }
 }
 
 static unsigned grid_of(int64_t work, int per_cta, int sms, int ctas_per_sm) {
@@ -164,18 +658,78 @@ cudaError_t launch_kv4_advance(const we_kv4_cache& c, int64_t tokens, cudaStream
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
-template <int DT, int OT>
-static cudaError_t attention_simple(const Kv4AttnArgs& a, uint32_t* err, cudaStream_t st) {
-  const dim3 grid((unsigned)((a.c.batch * a.tokens * a.heads + 3) / 4));
-  if (a.c.dim == 64) return launch_pdl(kv4_attention_simple_kernel<DT, OT, 64>, grid, 128, 0, st, a, err);
-  if (a.c.dim == 128) return launch_pdl(kv4_attention_simple_kernel<DT, OT, 128>, grid, 128, 0, st, a, err);
-  return launch_pdl(kv4_attention_simple_kernel<DT, OT, 256>, grid, 128, 0, st, a, err);
+namespace {
+// How the work of a call is cut: q rows into tiles of 8 or 16, keys into chunks of a CTA.
+struct Kv4Plan {
+  int nq, row_tiles, splits, chunk;
+  int64_t units, part_floats;
+};
+Kv4Plan kv4_plan(const Kv4AttnArgs& a, int sms) {
+  Kv4Plan q{};
+  const int64_t rows = a.tokens * (a.heads / a.c.kv_heads);
+  q.nq = rows <= 8 ? 1 : 2;
+  q.row_tiles = (int)((rows + 8 * q.nq - 1) / (8 * q.nq));
+  q.units = a.c.batch * a.c.kv_heads * q.row_tiles;
+  // Four CTAs an SM. A sequence's length is known on the device only, so chunks are cut for the longest possible one:
+  // about four waves of them, so that ragged lengths even out, or one wave where that would be too many parts to merge.
+  const int64_t cap = std::max<int64_t>(1, a.c.max_pages * a.c.page), slots = (int64_t)sms * 4;
+  int64_t want = (4 * slots + q.units - 1) / q.units;
+  if (want > 32) want = std::min<int64_t>(kv::MAX_SPLITS, std::max<int64_t>(32, slots / q.units));
+  const int64_t chunk = (((cap + want - 1) / want) + 127) / 128 * 128;
+  q.chunk = (int)std::min<int64_t>(chunk, 0x40000000);
+  q.splits = (int)((cap + q.chunk - 1) / q.chunk);
+  q.part_floats = q.splits > 1 ? q.units * q.splits * 8 * q.nq * (a.c.dim + 4) : 0;
+  return q;
 }
 
-cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, uint32_t* err, int sms, cudaStream_t st) {
-  const bool qf = a.dtype == WE_F32, of = a.out_dtype == WE_F32;
-  const cudaError_t e = qf ? (of ? attention_simple<WE_F32, WE_F32>(a, err, st) : attention_simple<WE_F32, WE_BF16>(a, err, st))
-                           : (of ? attention_simple<WE_BF16, WE_F32>(a, err, st) : attention_simple<WE_BF16, WE_BF16>(a, err, st));
+template <int D, int NQ, int KT, int TERMS>
+cudaError_t kv4_launch(const kv::Params& p, dim3 grid, cudaStream_t st) {
+  auto kern = kv4_attention_kernel<D, NQ, KT, TERMS>;
+  constexpr int ring = kv::WARPS * 3 * KT * (D * 16 + D);
+  constexpr int merge = kv::WARPS * 8 * NQ * (D + 4) * 4;
+  constexpr int bytes = ring > merge ? ring : merge;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kern, grid, kv::THREADS, bytes, st, p);
+}
+}  // namespace
+
+void kv4_attention_scratch(const Kv4AttnArgs& a, int sms, int64_t* part_bytes, int64_t* units) {
+  const Kv4Plan q = kv4_plan(a, sms);
+  *part_bytes = q.part_floats * 4;
+  *units = q.splits > 1 ? q.units : 0;
+}
+
+cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, void* part, uint32_t* done, uint32_t* err, int sms, cudaStream_t st) {
+  const Kv4Plan q = kv4_plan(a, sms);
+  kv::Params p{};
+  p.c = a.c;
+  p.q = a.q;
+  p.out = a.out;
+  p.tokens = (int)a.tokens;
+  p.heads = (int)a.heads;
+  p.group = (int)(a.heads / a.c.kv_heads);
+  p.rows = p.tokens * p.group;
+  p.row_tiles = q.row_tiles;
+  p.chunk = q.chunk;
+  p.q_stride = a.q_stride;
+  p.out_stride = a.out_stride;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.dtype = a.dtype;
+  p.out_dtype = a.out_dtype;
+  p.part = static_cast<float*>(part);
+  p.done = done;
+  p.err = err;
+  const dim3 grid((unsigned)q.splits, (unsigned)(a.c.kv_heads * q.row_tiles), (unsigned)a.c.batch);
+  const bool f32 = a.dtype == WE_F32 || a.out_dtype == WE_F32;
+  cudaError_t e;
+#define KV4_CASE(D)                                                                                             \
+  e = f32 ? (q.nq == 1 ? kv4_launch<D, 1, 1, 2>(p, grid, st) : kv4_launch<D, 2, 1, 2>(p, grid, st))             \
+          : (q.nq == 1 ? kv4_launch<D, 1, D == 256 ? 1 : 2, 1>(p, grid, st) : kv4_launch<D, 2, 1, 1>(p, grid, st))
+  if (a.c.dim == 64) KV4_CASE(64);
+  else if (a.c.dim == 128) KV4_CASE(128);
+  else KV4_CASE(256);
+#undef KV4_CASE
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
 

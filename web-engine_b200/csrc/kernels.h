@@ -160,7 +160,10 @@ struct Kv4AttnArgs {
   float scale;
   int dtype, out_dtype;
 };
-cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, uint32_t* err, int sms, cudaStream_t st);
+// scratch for the parts of split sequences, and how many counters (zero before and after a call) they need
+void kv4_attention_scratch(const Kv4AttnArgs& a, int sms, int64_t* part_bytes, int64_t* units);
+cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, void* part, uint32_t* done, uint32_t* err, int sms,
+                                 cudaStream_t st);
 
 cudaError_t launch_cross_simt(const we_cross_desc& d, int sms, cudaStream_t st);
 

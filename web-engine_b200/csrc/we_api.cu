@@ -13,6 +13,8 @@
 #include "common.cuh"
 #include "kernels.h"
 
+static constexpr int64_t kCounters = 1 << 16;
+
 struct we_ctx {
   int device = 0;
   int sms = 148;
@@ -26,6 +28,7 @@ struct we_ctx {
   we_stats stats{0, 0, 0, 0, 0, 0};
   uint32_t* dev_err = nullptr;  // device error word written by bounded waits
   unsigned int* amax_word = nullptr;
+  uint32_t* counters = nullptr;  // kCounters words, zero between launches (we_ctx_counters)
   // Pinned staging ring for host -> device uploads. Like WebGPU's queue.writeBuffer, an upload copies the
   // caller's data before returning and the DMA then runs in stream order: a copy straight from pageable
   // memory would first wait for the whole stream, and the GPU would idle while the host catches up.
@@ -217,6 +220,15 @@ int we_ctx_device(we_ctx* ctx) { return ctx->device; }
 uint32_t* we_ctx_dev_err(we_ctx* ctx) { return ctx->dev_err; }
 void we_ctx_count_launch(we_ctx* ctx) { ctx->stats.launches++; }
 bool we_ctx_capturing(const we_ctx* ctx) { return ctx->capturing; }
+// scratch of the translation units without the pool's types (as Scratch below: given back right after its work is queued)
+int we_ctx_scratch_take(we_ctx* ctx, size_t bytes, void** out) {
+  bool reused;
+  return pool_take(ctx, (bytes + 255) / 256 * 256, out, &reused);
+}
+void we_ctx_scratch_put(we_ctx* ctx, void* p) { pool_put(ctx, p); }
+// Arrival counters of kernels that merge split work: made zero with the context, and left zero by every launch, so that
+// the launches of the context's stream, captured ones included, take turns with the same words.
+uint32_t* we_ctx_counters(we_ctx* ctx, int64_t count) { return count <= kCounters ? ctx->counters : nullptr; }
 
 extern "C" {
 
@@ -242,7 +254,9 @@ int we_init(int device, uint32_t flags, we_ctx** out) {
   }
   ctx->sms = sms > 0 ? sms : 148;
   if (cudaStreamCreateWithFlags(&ctx->own, cudaStreamNonBlocking) != cudaSuccess ||
-      cudaMalloc(&ctx->dev_err, 16) != cudaSuccess || cudaMemset(ctx->dev_err, 0, 16) != cudaSuccess) {
+      cudaMalloc(&ctx->dev_err, 16) != cudaSuccess || cudaMemset(ctx->dev_err, 0, 16) != cudaSuccess ||
+      cudaMalloc(&ctx->counters, kCounters * 4) != cudaSuccess ||
+      cudaMemset(ctx->counters, 0, kCounters * 4) != cudaSuccess) {
     delete ctx;
     return WE_ECUDA;
   }
@@ -265,6 +279,7 @@ int we_destroy(we_ctx* ctx) {
   if (ctx->d2h) cudaStreamDestroy(ctx->d2h);
   for (auto& kv : ctx->sizes) cudaFree(kv.first);
   cudaFree(ctx->dev_err);
+  cudaFree(ctx->counters);
   cudaStreamDestroy(ctx->own);
   delete ctx;
   return WE_OK;

@@ -11,6 +11,9 @@ int we_ctx_fail(we_ctx* ctx, int code, const std::string& msg);
 cudaStream_t we_ctx_stream(we_ctx* ctx);
 uint32_t* we_ctx_dev_err(we_ctx* ctx);
 void we_ctx_count_launch(we_ctx* ctx);
+int we_ctx_scratch_take(we_ctx* ctx, size_t bytes, void** out);  // from the buffer pool, to be given back once queued
+void we_ctx_scratch_put(we_ctx* ctx, void* p);
+uint32_t* we_ctx_counters(we_ctx* ctx, int64_t count);  // zeroed device words that every user leaves zero, or NULL
 
 namespace {
 
@@ -152,7 +155,20 @@ int we_kv4_attention(we_ctx* ctx, const we_kv4_cache* c, const void* q, int32_t 
                     scale != 0.f ? scale : 1.f / sqrtf((float)c->dim),
                     dtype,
                     out_dtype};
-  DLK(we::launch_kv4_attention(a, we_ctx_dev_err(ctx), we_num_sms(ctx), we_ctx_stream(ctx)), "kv4 attention");
+  int64_t part_bytes, units;
+  we::kv4_attention_scratch(a, we_num_sms(ctx), &part_bytes, &units);
+  if (heads / c->kv_heads * tokens > 0x7fffffff / 16 || a.c.kv_heads * ((heads / c->kv_heads * tokens + 7) / 8) > 65535)
+    return we_ctx_fail(ctx, WE_EINVAL, "kv4: too many query rows in one call");
+  void* part = nullptr;
+  uint32_t* done = nullptr;
+  if (units > 0) {
+    done = we_ctx_counters(ctx, units);
+    if (!done) return we_ctx_fail(ctx, WE_EINVAL, "kv4: too many sequences and heads to split in one call");
+    if ((rc = we_ctx_scratch_take(ctx, (size_t)part_bytes, &part)) != WE_OK) return rc;
+  }
+  const cudaError_t e = we::launch_kv4_attention(a, part, done, we_ctx_dev_err(ctx), we_num_sms(ctx), we_ctx_stream(ctx));
+  if (part) we_ctx_scratch_put(ctx, part);
+  DLK(e, "kv4 attention");
   return WE_OK;
 }
 
