@@ -113,6 +113,10 @@ __global__ void kv4_advance_kernel(int32_t* lengths, int64_t batch, int32_t toke
 namespace kv {
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int MAX_SPLITS = 64;
+#ifndef KV_DEPTH_
+#define KV_DEPTH_ 4
+#endif
+constexpr int KV_DEPTH = KV_DEPTH_;  // steps in a warp's ring (a power of two)
 
 struct Params {
   we_kv4_cache c;
@@ -164,7 +168,7 @@ template <int D, int NQ, int KT, int TERMS>
 __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Params p) {
   using namespace kv;
   constexpr int G = D / 64, STEP = KT * 16, ROW = D / 2, TILE = 16 * ROW, QROWS = 8 * NQ;
-  constexpr int STAGE = KT * (2 * TILE + 2 * 16 * G * 2), DEPTH = 3;
+  constexpr int STAGE = KT * (2 * TILE + 2 * 16 * G * 2), DEPTH = KV_DEPTH;
   constexpr int MTILES = D / 16;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int last;
@@ -190,52 +194,52 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
   uint8_t* ring = smem + warp * (DEPTH * STAGE);
   const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
 
-  // Page ids of this warp's next 32 tiles of 16 keys, a lane each; -1: not there.
-  int ids = -1;
+  // Where this warp's next 32 tiles of 16 keys lie, a lane each: index of the tile in the cache, or -1: not there.
+  uint32_t at16 = 0xffffffffu;
   const int page = (int)p.c.page;
   auto load_ids = [&](int i) {  // from step i on
     const int tile = i * KT + lane, key = key0 + (warp + WARPS * (tile / KT)) * STEP + (tile % KT) * 16;
-    ids = -1;
+    at16 = 0xffffffffu;
     if (key < key1) {
-      ids = p.c.page_table[(int64_t)b * p.c.max_pages + key / page];
-      if (ids < 0 || ids >= p.c.pages) {
-        atomicCAS(p.err, 0u, (uint32_t)DEV_ERR_KV_PAGE);
-        ids = -1;
-      }
+      const int slot = key / page;
+      const int id = p.c.page_table[(int64_t)b * p.c.max_pages + slot];
+      if (id < 0 || id >= p.c.pages) atomicCAS(p.err, 0u, (uint32_t)DEV_ERR_KV_PAGE);
+      else at16 = ((uint32_t)id * (uint32_t)p.c.kv_heads + head) * (uint32_t)(page / 16) + (key - slot * page) / 16;
     }
   };
+  uint32_t copy_to[TILE / 512];  // where a lane's 16-byte pieces of a tile go
+#pragma unroll
+  for (int j = 0; j < TILE / 512; j++) {
+    const int at = j * 32 + lane, r = at / (ROW / 16), ch = at % (ROW / 16);  // piece `ch` of row r
+    copy_to[j] = segment<D>(r, ch >> 1) + (ch & 1) * 16;
+  }
   uint32_t there = 0;  // bit per tile of the ring's stages: its page exists
   auto copy = [&](int i) {
     if (i < mine) {
       if ((i * KT) % 32 == 0) load_ids(i);
-      const uint32_t to = ring_addr + (i % DEPTH) * STAGE;
+      const int stage = i & (DEPTH - 1);
+      const uint32_t to = ring_addr + stage * STAGE;
 #pragma unroll
       for (int t = 0; t < KT; t++) {
-        const int id = __shfl_sync(0xffffffffu, ids, (i * KT + t) & 31);
-        const uint32_t bit = 1u << ((i % DEPTH) * KT + t);
-        there = id >= 0 ? there | bit : there & ~bit;
-        if (id < 0) continue;
-        const int key = key0 + (warp + WARPS * i) * STEP + t * 16;
-        const int64_t row = ((int64_t)id * p.c.kv_heads + head) * page + key % page;
+        const uint32_t at = __shfl_sync(0xffffffffu, at16, (i * KT + t) & 31);
+        const uint32_t bit = 1u << (stage * KT + t);
+        there &= ~bit;
+        if (at == 0xffffffffu) continue;
+        there |= bit;
 #pragma unroll
         for (int side = 0; side < 2; side++) {
-          const uint8_t* from = (side ? p.c.v : p.c.k) + row * ROW;
-          const uint32_t dst = to + (t * 2 + side) * TILE;
+          const uint8_t* from = (side ? p.c.v : p.c.k) + (uint64_t)at * TILE + lane * 16;
 #pragma unroll
-          for (int j = 0; j < TILE / 512; j++) {
-            const int at = j * 32 + lane, r = at / (ROW / 16), ch = at % (ROW / 16);  // 16-byte piece `ch` of row r
-            cp_async16(dst + segment<D>(r, ch >> 1) + (ch & 1) * 16, from + at * 16);
-          }
+          for (int j = 0; j < TILE / 512; j++) cp_async16(to + (t * 2 + side) * TILE + copy_to[j], from + j * 512);
         }
         // scales: 4-byte words, 8 G of k then 8 G of v
-        if (16 * G >= 32 || lane < 16 * G) {
 #pragma unroll
-          for (int j = 0; j < (16 * G + 31) / 32; j++) {
-            const int at = j * 32 + lane, side = at / (8 * G), word = at % (8 * G);
-            const uint16_t* from = (side ? p.c.v_scale : p.c.k_scale) + row * G + word * 2;
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + KT * 2 * TILE + t * (64 * G) + at * 4), "l"(from)
+        for (int j = 0; j < (16 * G + 31) / 32; j++) {
+          const int word = j * 32 + lane, w = word % (8 * G);
+          const uint16_t* from = (word / (8 * G) ? p.c.v_scale : p.c.k_scale) + (uint64_t)at * (16 * G) + w * 2;
+          if (word < 16 * G)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + KT * 2 * TILE + t * (64 * G) + word * 4), "l"(from)
                          : "memory");
-          }
         }
       }
     }
@@ -321,19 +325,33 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
   asm volatile("" : "+r"(low), "+r"(high));
   const int full = have + (rtile * QROWS) / p.group + 1;  // keys below are seen by every row of the tile
 
+  // offsets of this lane's pieces of a tile: for k words 2 c, 2 c + 1 of a group of its key and (+ 8 rows) the other; for v
+  // word u of the keys of rows 2 c and (+ 8 rows) 2 c + 8, and of rows 2 c + 1 and 2 c + 9
+  const int k0 = (u >> 1) + 4 * (u & 1);  // row r of a tile of S^T is key r / 2 + 4 (r & 1) (+ 8)
+  int k_at[G], v_at[2][G];
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    k_at[g] = segment<D>(k0, g) + c * 8;
+    v_at[0][g] = TILE + segment<D>(c, g) + u * 4;
+    v_at[1][g] = TILE + segment<D>(c + 4, g) + u * 4;
+  }
+  const int s_at = KT * 2 * TILE + k0 * (2 * G);
+
   for (int i = 0; i < mine; i++) {
     copy(i + DEPTH - 1);
     cp_async_wait<DEPTH - 1>();
     __syncwarp();
-    const uint8_t* st = ring + (i % DEPTH) * STAGE;
+    const int stage = i & (DEPTH - 1);
+    const uint8_t* st = ring + stage * STAGE;
     const int first = key0 + (warp + WARPS * i) * STEP;
-    // S^T: rows are keys: row r of a tile is key r / 2 + 4 (r & 1) (+ 8)
-    float s[KT][NQ][4];
+    constexpr uint32_t TILES = (1u << KT) - 1u;
+    const uint32_t here = (there >> (stage * KT)) & TILES;
+    const bool whole = here == TILES && first + STEP <= min(full, key1);  // (uniform) every row sees every key
+    float s[KT][NQ][4];  // S^T in the units of the products
     uint32_t vs[KT][2][(G + 1) / 2];  // scales of v of this lane's two keys
 #pragma unroll
     for (int t = 0; t < KT; t++) {
       const uint8_t* kt = st + (t * 2) * TILE;
-      const int k0 = (u >> 1) + 4 * (u & 1);  // this lane's key of the tile, and + 8
       float d[NQ][G][4];
 #pragma unroll
       for (int g = 0; g < G; g++) {
@@ -342,8 +360,8 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
           d[nq][g][0] = d[nq][g][2] = q_start[nq][g][0];
           d[nq][g][1] = d[nq][g][3] = q_start[nq][g][1];
         }
-        const uint2 a2 = *reinterpret_cast<const uint2*>(kt + segment<D>(k0, g) + c * 8);
-        const uint2 b2 = *reinterpret_cast<const uint2*>(kt + segment<D>(k0 + 8, g) + c * 8);
+        const uint2 a2 = *reinterpret_cast<const uint2*>(kt + k_at[g]);
+        const uint2 b2 = *reinterpret_cast<const uint2*>(kt + k_at[g] + 8 * ROW);
 #pragma unroll
         for (int x = 0; x < 4; x++) {  // word x / 2, half x % 2
           const uint32_t wa = (x < 2 ? a2.x : a2.y) >> ((x & 1) * 8), wb = (x < 2 ? b2.x : b2.y) >> ((x & 1) * 8);
@@ -355,44 +373,52 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
             for (int k = 0; k < TERMS; k++) mma_f16(d[nq][g], av, qf[nq][g][x][0][k], qf[nq][g][x][1][k]);
         }
       }
-      const bool page_there = (there >> ((i % DEPTH) * KT + t)) & 1;
-      const uint8_t* sc = st + KT * 2 * TILE + t * (64 * G);
-      float ks[2][G];
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const int key = k0 + 8 * h;
-        const bool valid = page_there && first + t * 16 + key < key1;
-        const uint8_t *kat = sc + key * (2 * G), *vat = kat + 32 * G;
+        const uint8_t* kat = st + s_at + t * (64 * G) + h * (16 * G);
+        float ks[G];
         if constexpr (G == 1) {
-          ks[h][0] = __half2float(__ushort_as_half(*reinterpret_cast<const uint16_t*>(kat)));
-          vs[t][h][0] = valid ? *reinterpret_cast<const uint16_t*>(vat) : 0u;
+          ks[0] = __half2float(__ushort_as_half(*reinterpret_cast<const uint16_t*>(kat)));
+          vs[t][h][0] = *reinterpret_cast<const uint16_t*>(kat + 32);
         } else {
 #pragma unroll
           for (int g = 0; g < G; g += 2) {
             const float2 f = halves(*reinterpret_cast<const uint32_t*>(kat + g * 2));
-            ks[h][g] = f.x;
-            ks[h][g + 1] = f.y;
-            vs[t][h][g / 2] = valid ? *reinterpret_cast<const uint32_t*>(vat + g * 2) : 0u;
+            ks[g] = f.x;
+            ks[g + 1] = f.y;
+            vs[t][h][g / 2] = *reinterpret_cast<const uint32_t*>(kat + 32 * G + g * 2);
           }
         }
 #pragma unroll
         for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
           for (int k = 0; k < 2; k++) {
-            float x = d[nq][0][h * 2 + k] * ks[h][0];
+            float x = d[nq][0][h * 2 + k] * ks[0];
 #pragma unroll
-            for (int g = 1; g < G; g++) x = fmaf(d[nq][g][h * 2 + k], ks[h][g], x);
-            x *= q_back[nq][k];
-            bool seen = valid;
-            if (first + STEP > full) {  // (uniform) some row stands before some key of the step
-              const int r = rtile * QROWS + nq * 8 + c * 2 + k;
-              seen = seen && first + t * 16 + key <= have + r / p.group;
-            }
-            s[t][nq][h * 2 + k] = seen ? x : -INFINITY;
+            for (int g = 1; g < G; g++) x = fmaf(d[nq][g][h * 2 + k], ks[g], x);
+            s[t][nq][h * 2 + k] = x;
           }
       }
     }
-    // running maximum of each column, and of v's scales
+    if (!whole) {
+#pragma unroll
+      for (int t = 0; t < KT; t++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int key = first + t * 16 + k0 + 8 * h;
+          const bool valid = ((here >> t) & 1) && key < key1;
+#pragma unroll
+          for (int g = 0; g < (G + 1) / 2; g++) vs[t][h][g] = valid ? vs[t][h][g] : 0u;
+#pragma unroll
+          for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              const int r = rtile * QROWS + nq * 8 + c * 2 + k;
+              if (!(valid && key <= have + r / p.group)) s[t][nq][h * 2 + k] = -INFINITY;
+            }
+        }
+    }
+    // Does a score pass its column's maximum by 2^8, or a scale of v its power of two, in this lane? (q_back > 0)
     bool grow = false;
     float mt[NQ][2];
 #pragma unroll
@@ -402,11 +428,8 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
         float x = fmaxf(s[0][nq][k], s[0][nq][2 + k]);
 #pragma unroll
         for (int t = 1; t < KT; t++) x = fmaxf(x, fmaxf(s[t][nq][k], s[t][nq][2 + k]));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-        mt[nq][k] = x;
-        grow = grow || x > m[nq][k] + 8.f;
+        mt[nq][k] = x * q_back[nq][k];
+        grow = grow || mt[nq][k] > m[nq][k] + 8.f;
       }
     uint32_t vt = 0;
 #pragma unroll
@@ -415,24 +438,25 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
       for (int h = 0; h < 2; h++)
 #pragma unroll
         for (int g = 0; g < (G + 1) / 2; g++) vt = __vmaxu2(vt, vs[t][h][g] & 0x7fff7fffu);
-    vt = __reduce_max_sync(0xffffffffu, max(vt & 0xffffu, vt >> 16));
-    const bool more = (vt >> 10) > (v_top >> 10);
-    if (__any_sync(0xffffffffu, grow) || more) {
+    vt = max(vt & 0xffffu, vt >> 16);
+    if (__any_sync(0xffffffffu, grow || vt > (v_top | 0x3ffu))) {
       // weights are kept times 2^(21 - exponent of the largest scale)
-      float f = 1.f;
-      if (more) {
-        f = __uint_as_float((127u + (v_top >> 10) - (vt >> 10)) << 23);
-        v_top = vt;
-      }
+      vt = max(__reduce_max_sync(0xffffffffu, vt), v_top);
+      const float f = __uint_as_float((127u + (v_top >> 10) - (vt >> 10)) << 23);
+      v_top = vt;
 #pragma unroll
       for (int nq = 0; nq < NQ; nq++) {
         float corr[2];
 #pragma unroll
         for (int k = 0; k < 2; k++) {
+          float x = mt[nq][k];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
           corr[k] = 1.f;
-          if (mt[nq][k] > m[nq][k] + 8.f) {
-            corr[k] = ex2_ftz(m[nq][k] - mt[nq][k]);
-            m[nq][k] = mt[nq][k];
+          if (x > m[nq][k]) {
+            corr[k] = ex2_ftz(m[nq][k] - x);
+            m[nq][k] = x;
           }
           l[nq][k] *= corr[k];
           corr[k] *= f;
@@ -455,12 +479,11 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
       for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float x = s[t][nq][e];
-          // a column that has seen nothing yet has m = -inf: no weight
-          pw[nq][e] = x == -INFINITY ? 0.f : ex2_ftz(x - m[nq][e & 1]);
+          pw[nq][e] = ex2_ftz(fmaf(s[t][nq][e], q_back[nq][e & 1], -m[nq][e & 1]));
+          if (!whole && s[t][nq][e] == -INFINITY) pw[nq][e] = 0.f;  // (its column may have m = -inf)
           l[nq][e & 1] += pw[nq][e];
         }
-      const uint8_t* vt_ = st + (t * 2 + 1) * TILE;
+      const uint8_t* kt = st + (t * 2) * TILE;
 #pragma unroll
       for (int g = 0; g < G; g++) {
         // weights times scales as the B operand: S^T's rows (keys) become the 16 values of the product
@@ -490,10 +513,10 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
           for (int nq = 0; nq < NQ; nq++) mma_f16(w_sum[nq][g], ones, bw[nq][0][0], bw[nq][0][1]);
         }
         // v: word u (dims 8 u .. 8 u + 7 of the group) of the keys of rows 2 c, 2 c + 1, 2 c + 8, 2 c + 9
-        const uint32_t v0 = *reinterpret_cast<const uint32_t*>(vt_ + segment<D>(c, g) + u * 4);
-        const uint32_t v1 = *reinterpret_cast<const uint32_t*>(vt_ + segment<D>(c + 4, g) + u * 4);
-        const uint32_t v2 = *reinterpret_cast<const uint32_t*>(vt_ + segment<D>(c + 8, g) + u * 4);
-        const uint32_t v3 = *reinterpret_cast<const uint32_t*>(vt_ + segment<D>(c + 12, g) + u * 4);
+        const uint32_t v0 = *reinterpret_cast<const uint32_t*>(kt + v_at[0][g]);
+        const uint32_t v1 = *reinterpret_cast<const uint32_t*>(kt + v_at[1][g]);
+        const uint32_t v2 = *reinterpret_cast<const uint32_t*>(kt + v_at[0][g] + 8 * ROW);
+        const uint32_t v3 = *reinterpret_cast<const uint32_t*>(kt + v_at[1][g] + 8 * ROW);
 #pragma unroll
         for (int h = 0; h < 2; h++) {  // dims 8 u + 4 h ..
           const uint32_t x = __byte_perm(v0, v1, h ? 0x7632 : 0x5410), y = __byte_perm(v2, v3, h ? 0x7632 : 0x5410);
@@ -685,7 +708,7 @@ Kv4Plan kv4_plan(const Kv4AttnArgs& a, int sms) {
 template <int D, int NQ, int KT, int TERMS>
 cudaError_t kv4_launch(const kv::Params& p, dim3 grid, cudaStream_t st) {
   auto kern = kv4_attention_kernel<D, NQ, KT, TERMS>;
-  constexpr int ring = kv::WARPS * 3 * KT * (D * 16 + D);
+  constexpr int ring = kv::WARPS * kv::KV_DEPTH * KT * (D * 16 + D);
   constexpr int merge = kv::WARPS * 8 * NQ * (D + 4) * 4;
   constexpr int bytes = ring > merge ? ring : merge;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
