@@ -3,6 +3,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "tc_ptx.cuh"
 
 namespace we {
 
@@ -108,15 +109,13 @@ __global__ void kv4_advance_kernel(int32_t* lengths, int64_t batch, int32_t toke
 // - f32 q or out (TERMS = 2): q and the weights are two f16 terms each (22 bits), and codes of v become exact signed f16
 //   by one more operation, because weights are all positive and the offset's sum would cost 3 to 5 bits.
 // - A warp takes 16 or 32 keys at a time through a ring of its own (cp.async), with its own running maximum; the O and
-//   sums are only rescaled when the maximum grows by more than 2^8 or v's scales outgrow their power of two. The 4 warps
-//   of a CTA and then the CTAs that split a long sequence are merged in a fixed order; the last CTA to finish merges.
+//   sums are only rescaled when the maximum grows by more than 2^8 or v's scales outgrow their power of two.
+// - A cluster of 8 CTAs shares the keys of a sequence evenly and merges over distributed shared memory; a longer sequence
+//   takes several clusters, whose parts the last one to finish merges. Every merge is in a fixed order.
 namespace kv {
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int MAX_SPLITS = 64;
-#ifndef KV_DEPTH_
-#define KV_DEPTH_ 4
-#endif
-constexpr int KV_DEPTH = KV_DEPTH_;  // steps in a warp's ring (a power of two)
+constexpr int CLUSTER = 8;    // CTAs that share a run of keys and merge over distributed shared memory
+constexpr int KV_DEPTH = 2;   // steps in a warp's ring (a power of two)
 
 struct Params {
   we_kv4_cache c;
@@ -124,12 +123,13 @@ struct Params {
   void* out;
   int tokens, heads, group, rows;  // group: heads per kv head; rows = tokens * group
   int row_tiles;                   // tiles of 8 NQ rows
-  int chunk;                       // keys per CTA
+  int chunk;                       // keys per CTA at most
+  int wide_q;                      // rows of q are 16-byte aligned
   int64_t q_stride, out_stride;
   float scale_log2;
   int dtype, out_dtype;
-  float* part;                     // [sequence, kv head, row tile][splits][8 NQ](dim values, maximum, sum), when split
-  uint32_t* done;                  // [sequence, kv head, row tile]: CTAs that have written, zero between calls
+  float* part;                     // [sequence, kv head, row tile][clusters][8 NQ](dim values, maximum, sum), when more than one
+  uint32_t* done;                  // [sequence, kv head, row tile]: clusters that have written, zero between calls
   uint32_t* err;
 };
 
@@ -173,20 +173,49 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3, u = lane >> 2;
-  const int split = blockIdx.x, b = blockIdx.z;
+  const int rank = blockIdx.x % CLUSTER, run = blockIdx.x / CLUSTER, b = blockIdx.z;  // CTA of the cluster, run of keys
   const int head = blockIdx.y / p.row_tiles, rtile = blockIdx.y % p.row_tiles;  // kv head, tile of q rows
   const int unit = (b * gridDim.y) + blockIdx.y;
   pdl_launch_dependents();
   pdl_wait();
 
+  // this lane's q values (see below) come first: they need no length
+  uint4 q_raw[NQ][G][4];
+#pragma unroll
+  for (int nq = 0; nq < NQ; nq++) {
+    const int r = rtile * QROWS + nq * 8 + u;
+    const int64_t row = ((int64_t)b * p.tokens + r / p.group) * p.q_stride + (int64_t)(head * p.group + r % p.group) * D + c * 16;
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        q_raw[nq][g][j] = make_uint4(0, 0, 0, 0);
+        if (r >= p.rows || (p.dtype == WE_BF16 && j >= 2)) continue;
+        const int64_t at = row + g * 64 + j * (p.dtype == WE_F32 ? 4 : 8);
+        uint32_t w[4];
+        if (p.wide_q) {
+          const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.q) + at * (p.dtype == WE_F32 ? 4 : 2));
+          w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            if (p.dtype == WE_F32) w[e] = static_cast<const uint32_t*>(p.q)[at + e];
+            else w[e] = static_cast<const uint16_t*>(p.q)[at + 2 * e] | (uint32_t) static_cast<const uint16_t*>(p.q)[at + 2 * e + 1] << 16;
+          }
+        }
+        q_raw[nq][g][j] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+  }
+
   const int have = p.c.lengths[b];
   const int64_t room = p.c.max_pages * p.c.page;
   const int64_t want = (int64_t)have + min(p.tokens, (rtile * QROWS + QROWS - 1) / p.group + 1);  // keys of the tile's last row
   const int keys = have < 0 ? 0 : (int)min(want, room);
-  if (have >= 0 && want > room && split == 0 && threadIdx.x == 0) atomicCAS(p.err, 0u, (uint32_t)DEV_ERR_KV_FULL);
-  const int splits = max(1, (keys + p.chunk - 1) / p.chunk);
-  if (split >= splits) return;
-  const int key0 = split * p.chunk, key1 = min(keys, key0 + p.chunk);
+  if (have >= 0 && want > room && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(p.err, 0u, (uint32_t)DEV_ERR_KV_FULL);
+  const int runs = max(1, (keys + CLUSTER * p.chunk - 1) / (CLUSTER * p.chunk));
+  if (run >= runs) return;  // (the whole cluster)
+  const int share = ((keys + runs * CLUSTER - 1) / (runs * CLUSTER) + STEP - 1) / STEP * STEP;  // keys of each CTA
+  const int key0 = min(keys, (run * CLUSTER + rank) * share), key1 = min(keys, key0 + share);
 
   // this warp's steps: key0 + (warp + WARPS i) STEP
   const int steps = (key1 - key0 + STEP - 1) / STEP;
@@ -255,20 +284,25 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
   float q_start[NQ][G][2], q_back[NQ][2];  // of the columns of S^T that a lane holds: 2 c, 2 c + 1
 #pragma unroll
   for (int nq = 0; nq < NQ; nq++) {
-    const int r = rtile * QROWS + nq * 8 + u;
     float x[G][16], top = 0.f;
 #pragma unroll
-    for (int g = 0; g < G; g++)
+    for (int g = 0; g < G; g++) {
 #pragma unroll
-      for (int e = 0; e < 16; e++) {
-        x[g][e] = 0.f;
-        if (r < p.rows) {
-          const int64_t at = ((int64_t)b * p.tokens + r / p.group) * p.q_stride +
-                             (int64_t)(head * p.group + r % p.group) * D + g * 64 + c * 16 + e;
-          x[g][e] = p.dtype == WE_F32 ? static_cast<const float*>(p.q)[at] : bf16_bits_to_f32(static_cast<const uint16_t*>(p.q)[at]);
+      for (int j = 0; j < 4; j++) {
+        const uint32_t w[4] = {q_raw[nq][g][j].x, q_raw[nq][g][j].y, q_raw[nq][g][j].z, q_raw[nq][g][j].w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          if (p.dtype == WE_F32) {
+            x[g][4 * j + e] = __uint_as_float(w[e]);
+          } else if (j < 2) {
+            x[g][8 * j + 2 * e] = __uint_as_float(w[e] << 16);
+            x[g][8 * j + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+          }
         }
-        top = fmaxf(top, fabsf(x[g][e]));
       }
+#pragma unroll
+      for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(x[g][e]));
+    }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const uint32_t ex = min(max(__float_as_uint(top) >> 23, 16u), 254u);
@@ -577,7 +611,6 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
       }
     }
   __syncthreads();
-  float* part = p.part ? p.part + (int64_t)unit * gridDim.x * (QROWS * PITCH) : nullptr;
   auto finish = [&](int r, int d, float4 acc, float sum) {  // 4 values of row r of the tile from dim d on
     const int row = rtile * QROWS + r;
     if (row >= p.rows) return;
@@ -590,67 +623,117 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
       else store_out<WE_BF16>(p.out, at + e, v[e]);
     }
   };
+  struct Sum {  // of parts of a row: 4 values and the sum of weights, relative to the row's maximum over the parts
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    __device__ __forceinline__ void add(float4 x, float m, float sum, float top) {
+      const float f = m == -INFINITY ? 0.f : ex2_ftz(m - top);  // -inf: the part saw no key of the row
+      v.x = fmaf(x.x, f, v.x);
+      v.y = fmaf(x.y, f, v.y);
+      v.z = fmaf(x.z, f, v.z);
+      v.w = fmaf(x.w, f, v.w);
+      l = fmaf(sum, f, l);
+    }
+  };
+  // the CTA's warps, into a place of its own
+  float* cta = mem + WARPS * QROWS * PITCH;
   for (int x = threadIdx.x; x < QROWS * (D / 4); x += THREADS) {
     const int r = x / (D / 4), d = x % (D / 4) * 4;
+    const float* from = mem + r * PITCH;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < WARPS; w++) top = fmaxf(top, mem[(w * QROWS + r) * PITCH + D]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
+    for (int w = 0; w < WARPS; w++) top = fmaxf(top, from[w * QROWS * PITCH + D]);
+    Sum sum;
 #pragma unroll
-    for (int w = 0; w < WARPS; w++) {
-      const float* from = mem + (w * QROWS + r) * PITCH;
-      if (from[D] == -INFINITY) continue;  // that warp saw no key of the row
-      const float f = ex2_ftz(from[D] - top);
-      const float4 v = *reinterpret_cast<const float4*>(from + d);
-      acc.x = fmaf(v.x, f, acc.x);
-      acc.y = fmaf(v.y, f, acc.y);
-      acc.z = fmaf(v.z, f, acc.z);
-      acc.w = fmaf(v.w, f, acc.w);
-      sum = fmaf(from[D + 1], f, sum);
+    for (int w = 0; w < WARPS; w++, from += QROWS * PITCH) sum.add(*reinterpret_cast<const float4*>(from + d), from[D], from[D + 1], top);
+    *reinterpret_cast<float4*>(cta + r * PITCH + d) = sum.v;
+    if (d == 0) {
+      cta[r * PITCH + D] = top;
+      cta[r * PITCH + D + 1] = sum.l;
     }
-    if (splits == 1) {
-      finish(r, d, acc, sum);
+  }
+  __syncwarp();
+  tc::cluster_sync_all();
+  // the cluster's CTAs: a CTA takes an eighth of the values
+  constexpr int ITEMS = QROWS * (D / 4) / CLUSTER;
+  const uint32_t cta_addr = (uint32_t)__cvta_generic_to_shared(cta);
+  auto remote = [](uint32_t addr, int cta_rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(tc::map_rank(addr, cta_rank)) : "memory");
+    return v;
+  };
+  float* part = runs > 1 ? p.part + (int64_t)unit * (gridDim.x / CLUSTER) * (QROWS * PITCH) : nullptr;
+  for (int x = threadIdx.x; x < ITEMS; x += THREADS) {
+    const int r = (rank * ITEMS + x) / (D / 4), d = (rank * ITEMS + x) % (D / 4) * 4;
+    const uint32_t at = cta_addr + 4 * (r * PITCH);
+    float ms[CLUSTER], ls[CLUSTER], top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < CLUSTER; w++) {
+      ms[w] = remote(at + 4 * D, w);
+      ls[w] = remote(at + 4 * (D + 1), w);
+      top = fmaxf(top, ms[w]);
+    }
+    Sum sum;
+#pragma unroll
+    for (int w = 0; w < CLUSTER; w++) {
+      float4 v;
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                   : "r"(tc::map_rank(at + 4 * d, w))
+                   : "memory");
+      sum.add(v, ms[w], ls[w], top);
+    }
+    if (runs == 1) {
+      finish(r, d, sum.v, sum.l);
     } else {
-      float* to = part + ((int64_t)split * QROWS + r) * PITCH;
-      *reinterpret_cast<float4*>(to + d) = acc;
+      float* to = part + ((int64_t)run * QROWS + r) * PITCH;
+      *reinterpret_cast<float4*>(to + d) = sum.v;
       if (d == 0) {
         to[D] = top;
-        to[D + 1] = sum;
+        to[D + 1] = sum.l;
       }
     }
   }
-  if (splits == 1) return;
-  // the last CTA of the unit to get here merges all of its parts, in the order of the keys
   __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const uint32_t before = atomicAdd(p.done + unit, 1u);
-    last = before == (uint32_t)splits - 1u;
-    if (last) p.done[unit] = 0u;
+  __syncwarp();
+  tc::cluster_sync_all();  // no CTA leaves while another reads its place; the cluster's part is written
+  if (runs == 1) return;
+  // the last cluster of the unit to get here merges all of its parts, in the order of the keys, a CTA an eighth of the values
+  if (rank == 0 && threadIdx.x == 0) {
+    const int is_last = atomicAdd(p.done + unit, 1u) == (uint32_t)runs - 1u;
+    if (is_last) p.done[unit] = 0u;
+    __threadfence();
+    const uint32_t flag = (uint32_t)__cvta_generic_to_shared(&last);
+    for (int w = 0; w < CLUSTER; w++)
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::map_rank(flag, w)), "r"(is_last) : "memory");
   }
-  __syncthreads();
+  __syncwarp();
+  tc::cluster_sync_all();
   if (!last) return;
   __threadfence();
-  for (int x = threadIdx.x; x < QROWS * (D / 4); x += THREADS) {
-    const int r = x / (D / 4), d = x % (D / 4) * 4;
-    if (rtile * QROWS + r >= p.rows) continue;
+  // 4 threads share the runs of one item
+  for (int x = threadIdx.x / 4; x < ITEMS; x += THREADS / 4) {
+    const int r = (rank * ITEMS + x) / (D / 4), d = (rank * ITEMS + x) % (D / 4) * 4, sub = threadIdx.x & 3;
+    const float* from = part + (int64_t)r * PITCH;
     float top = -INFINITY;
-    for (int z = 0; z < splits; z++) top = fmaxf(top, part[((int64_t)z * QROWS + r) * PITCH + D]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-#pragma unroll 8
-    for (int z = 0; z < splits; z++) {
-      const float* from = part + ((int64_t)z * QROWS + r) * PITCH;
-      const float f = from[D] == -INFINITY ? 0.f : ex2_ftz(from[D] - top);
-      const float4 v = *reinterpret_cast<const float4*>(from + d);
-      acc.x = fmaf(v.x, f, acc.x);
-      acc.y = fmaf(v.y, f, acc.y);
-      acc.z = fmaf(v.z, f, acc.z);
-      acc.w = fmaf(v.w, f, acc.w);
-      sum = fmaf(from[D + 1], f, sum);
+    for (int z = 0; z < runs; z++) top = fmaxf(top, from[(int64_t)z * (QROWS * PITCH) + D]);
+    Sum sum;
+    const int z1 = runs * (sub + 1) / 4;
+#pragma unroll 4
+    for (int z = runs * sub / 4; z < z1; z++) {
+      const float* row = from + (int64_t)z * (QROWS * PITCH);
+      sum.add(*reinterpret_cast<const float4*>(row + d), row[D], row[D + 1], top);
     }
-    finish(r, d, acc, sum);
+#pragma unroll
+    for (int w = 1; w < 4; w *= 2) {
+      const uint32_t quad = 0xfu << (lane & ~3);
+      sum.v.x += __shfl_xor_sync(quad, sum.v.x, w);
+      sum.v.y += __shfl_xor_sync(quad, sum.v.y, w);
+      sum.v.z += __shfl_xor_sync(quad, sum.v.z, w);
+      sum.v.w += __shfl_xor_sync(quad, sum.v.w, w);
+      sum.l += __shfl_xor_sync(quad, sum.l, w);
+    }
+    if (sub == 0) finish(r, d, sum.v, sum.l);
   }
 }
 
@@ -684,7 +767,7 @@ cudaError_t launch_kv4_advance(const we_kv4_cache& c, int64_t tokens, cudaStream
 namespace {
 // How the work of a call is cut: q rows into tiles of 8 or 16, keys into chunks of a CTA.
 struct Kv4Plan {
-  int nq, row_tiles, splits, chunk;
+  int nq, row_tiles, runs, chunk;
   int64_t units, part_floats;
 };
 Kv4Plan kv4_plan(const Kv4AttnArgs& a, int sms) {
@@ -693,15 +776,13 @@ Kv4Plan kv4_plan(const Kv4AttnArgs& a, int sms) {
   q.nq = rows <= 8 ? 1 : 2;
   q.row_tiles = (int)((rows + 8 * q.nq - 1) / (8 * q.nq));
   q.units = a.c.batch * a.c.kv_heads * q.row_tiles;
-  // Four CTAs an SM. A sequence's length is known on the device only, so chunks are cut for the longest possible one:
-  // about four waves of them, so that ragged lengths even out, or one wave where that would be too many parts to merge.
-  const int64_t cap = std::max<int64_t>(1, a.c.max_pages * a.c.page), slots = (int64_t)sms * 4;
-  int64_t want = (4 * slots + q.units - 1) / q.units;
-  if (want > 32) want = std::min<int64_t>(kv::MAX_SPLITS, std::max<int64_t>(32, slots / q.units));
-  const int64_t chunk = (((cap + want - 1) / want) + 127) / 128 * 128;
-  q.chunk = (int)std::min<int64_t>(chunk, 0x40000000);
-  q.splits = (int)((cap + q.chunk - 1) / q.chunk);
-  q.part_floats = q.splits > 1 ? q.units * q.splits * 8 * q.nq * (a.c.dim + 4) : 0;
+  // Four CTAs an SM. A sequence's length is known on the device only, so runs are cut for the longest possible one: about
+  // four waves of CTAs, so that ragged lengths even out.
+  const int64_t cap = std::max<int64_t>(1, a.c.max_pages * a.c.page);
+  const int64_t chunk = (cap * q.units + sms * 16 - 1) / (sms * 16);
+  q.chunk = (int)std::min<int64_t>((std::max<int64_t>(chunk, 128) + 31) / 32 * 32, 0x4000000);
+  q.runs = (int)((cap + (int64_t)q.chunk * kv::CLUSTER - 1) / ((int64_t)q.chunk * kv::CLUSTER));
+  q.part_floats = q.runs > 1 ? q.units * q.runs * 8 * q.nq * (a.c.dim + 4) : 0;
   return q;
 }
 
@@ -709,18 +790,30 @@ template <int D, int NQ, int KT, int TERMS>
 cudaError_t kv4_launch(const kv::Params& p, dim3 grid, cudaStream_t st) {
   auto kern = kv4_attention_kernel<D, NQ, KT, TERMS>;
   constexpr int ring = kv::WARPS * kv::KV_DEPTH * KT * (D * 16 + D);
-  constexpr int merge = kv::WARPS * 8 * NQ * (D + 4) * 4;
+  constexpr int merge = (kv::WARPS + 1) * 8 * NQ * (D + 4) * 4;
   constexpr int bytes = ring > merge ? ring : merge;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kern, grid, kv::THREADS, bytes, st, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kv::THREADS);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kv::CLUSTER;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  pdl_attribute(attr[1]);
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, p);
 }
 }  // namespace
 
 void kv4_attention_scratch(const Kv4AttnArgs& a, int sms, int64_t* part_bytes, int64_t* units) {
   const Kv4Plan q = kv4_plan(a, sms);
   *part_bytes = q.part_floats * 4;
-  *units = q.splits > 1 ? q.units : 0;
+  *units = q.runs > 1 ? q.units : 0;
 }
 
 cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, void* part, uint32_t* done, uint32_t* err, int sms, cudaStream_t st) {
@@ -735,6 +828,7 @@ cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, void* part, uint32_t* don
   p.rows = p.tokens * p.group;
   p.row_tiles = q.row_tiles;
   p.chunk = q.chunk;
+  p.wide_q = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * (a.dtype == WE_F32 ? 4 : 2))) & 15) == 0;
   p.q_stride = a.q_stride;
   p.out_stride = a.out_stride;
   p.scale_log2 = a.scale * 1.4426950408889634f;
@@ -743,7 +837,7 @@ cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, void* part, uint32_t* don
   p.part = static_cast<float*>(part);
   p.done = done;
   p.err = err;
-  const dim3 grid((unsigned)q.splits, (unsigned)(a.c.kv_heads * q.row_tiles), (unsigned)a.c.batch);
+  const dim3 grid((unsigned)(q.runs * kv::CLUSTER), (unsigned)(a.c.kv_heads * q.row_tiles), (unsigned)a.c.batch);
   const bool f32 = a.dtype == WE_F32 || a.out_dtype == WE_F32;
   cudaError_t e;
 #define KV4_CASE(D)                                                                                             \
