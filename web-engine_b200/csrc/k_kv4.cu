@@ -1,6 +1,7 @@
 // A paged 4-bit K/V cache (we_kv4_cache): rows in, rows out, and the attention of a step's new tokens over it.
 #include <algorithm>
 
+#include "attn_merge.cuh"
 #include "common.cuh"
 #include "kernels.h"
 #include "tc_ptx.cuh"
@@ -138,6 +139,12 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// d = a b + c
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
 __device__ __forceinline__ uint32_t and_xor(uint32_t v, uint32_t mask, uint32_t flip) {
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(v), "r"(mask), "r"(flip));
@@ -170,6 +177,7 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
   constexpr int G = D / 64, STEP = KT * 16, ROW = D / 2, TILE = 16 * ROW, QROWS = 8 * NQ;
   constexpr int STAGE = KT * (2 * TILE + 2 * 16 * G * 2), DEPTH = KV_DEPTH;
   constexpr int MTILES = D / 16;
+  constexpr float UP = TERMS == 1 ? 6.f : 0.f;  // weights are kept times 2^UP
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3, u = lane >> 2;
@@ -281,7 +289,7 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
   // 2 c + 1 in the order of the codes: for word w and half h the pairs (q0, q4), (q1, q5) / 16 or (q2, q6), (q3, q7) / 16,
   // times a power of two that brings the row's largest to 2^15.
   uint32_t qf[NQ][G][4][2][TERMS];
-  float q_start[NQ][G][2], q_back[NQ][2];  // of the columns of S^T that a lane holds: 2 c, 2 c + 1
+  float q_start[NQ][G][4], q_back[NQ][2];  // of the columns of S^T that a lane holds: 2 c, 2 c + 1 (of two rows)
 #pragma unroll
   for (int nq = 0; nq < NQ; nq++) {
     float x[G][16], top = 0.f;
@@ -340,7 +348,7 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
       const int from = (c * 2 + k) * 4;
       q_back[nq][k] = __shfl_sync(0xffffffffu, back, from);
 #pragma unroll
-      for (int g = 0; g < G; g++) q_start[nq][g][k] = __shfl_sync(0xffffffffu, sum[g], from) * -4.76837158203125e-07f;  // -8 2^-24
+      for (int g = 0; g < G; g++) q_start[nq][g][k] = q_start[nq][g][2 + k] = __shfl_sync(0xffffffffu, sum[g], from) * -4.76837158203125e-07f;  // -8 2^-24
     }
   }
 
@@ -351,7 +359,7 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
     for (int t = 0; t < MTILES; t++) o[nq][t][0] = o[nq][t][1] = o[nq][t][2] = o[nq][t][3] = 0.f;
 #pragma unroll
     for (int g = 0; g < G; g++) w_sum[nq][g][0] = w_sum[nq][g][1] = w_sum[nq][g][2] = w_sum[nq][g][3] = 0.f;
-    m[nq][0] = m[nq][1] = -INFINITY;
+    m[nq][0] = m[nq][1] = NONE;
     l[nq][0] = l[nq][1] = 0.f;
   }
   uint32_t v_top = 1u << 10;  // the largest scale of v so far, as f16 bits (at least the smallest normal one)
@@ -389,11 +397,6 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
       float d[NQ][G][4];
 #pragma unroll
       for (int g = 0; g < G; g++) {
-#pragma unroll
-        for (int nq = 0; nq < NQ; nq++) {
-          d[nq][g][0] = d[nq][g][2] = q_start[nq][g][0];
-          d[nq][g][1] = d[nq][g][3] = q_start[nq][g][1];
-        }
         const uint2 a2 = *reinterpret_cast<const uint2*>(kt + k_at[g]);
         const uint2 b2 = *reinterpret_cast<const uint2*>(kt + k_at[g] + 8 * ROW);
 #pragma unroll
@@ -404,7 +407,10 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
 #pragma unroll
           for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
-            for (int k = 0; k < TERMS; k++) mma_f16(d[nq][g], av, qf[nq][g][x][0][k], qf[nq][g][x][1][k]);
+            for (int k = 0; k < TERMS; k++) {
+              if (x == 0 && k == 0) mma_f16(d[nq][g], av, qf[nq][g][x][0][k], qf[nq][g][x][1][k], q_start[nq][g]);
+              else mma_f16(d[nq][g], av, qf[nq][g][x][0][k], qf[nq][g][x][1][k]);
+            }
         }
       }
 #pragma unroll
@@ -474,7 +480,7 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
         for (int g = 0; g < (G + 1) / 2; g++) vt = __vmaxu2(vt, vs[t][h][g] & 0x7fff7fffu);
     vt = max(vt & 0xffffu, vt >> 16);
     if (__any_sync(0xffffffffu, grow || vt > (v_top | 0x3ffu))) {
-      // weights are kept times 2^(21 - exponent of the largest scale)
+      // O and the sums of weights are kept over 2^(exponent of the largest scale)
       vt = max(__reduce_max_sync(0xffffffffu, vt), v_top);
       const float f = __uint_as_float((127u + (v_top >> 10) - (vt >> 10)) << 23);
       v_top = vt;
@@ -505,7 +511,10 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
           for (int e = 0; e < 4; e++) w_sum[nq][g][e] *= corr[e & 1];
       }
     }
-    const float v_up = __uint_as_float((148u - (v_top >> 10)) << 23);  // 2^(21 - exponent field)
+    // scales of v times 2^(15 - e) (TERMS 2: 2^(21 - e)), e the exponent field of the largest: below 2, so that a weight of
+    // 2^(8 + UP) at most times it stays below 2^15 (2^15)
+    const float v_up = __uint_as_float((148u - (v_top >> 10)) << 23);
+    const __half2 v_up2 = __float2half2_rn(v_up * 0.015625f);
 #pragma unroll
     for (int t = 0; t < KT; t++) {
       float pw[NQ][4];
@@ -513,31 +522,42 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
       for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          pw[nq][e] = ex2_ftz(fmaf(s[t][nq][e], q_back[nq][e & 1], -m[nq][e & 1]));
-          if (!whole && s[t][nq][e] == -INFINITY) pw[nq][e] = 0.f;  // (its column may have m = -inf)
+          pw[nq][e] = ex2_ftz(fmaf(s[t][nq][e], q_back[nq][e & 1], UP - m[nq][e & 1]));
           l[nq][e & 1] += pw[nq][e];
         }
       const uint8_t* kt = st + (t * 2) * TILE;
+      // TERMS 1: weights and scales as f16, their products rounded once more (2^-11 each)
+      __half2 ph[NQ][2];
+      uint32_t vn[2][(G + 1) / 2];
+      if constexpr (TERMS == 1) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+          for (int nq = 0; nq < NQ; nq++) ph[nq][h] = __floats2half2_rn(pw[nq][h * 2], pw[nq][h * 2 + 1]);
+#pragma unroll
+          for (int g = 0; g < (G + 1) / 2; g++) vn[h][g] = as_u32(__hmul2(as_half2(vs[t][h][g]), v_up2));
+        }
+      }
 #pragma unroll
       for (int g = 0; g < G; g++) {
         // weights times scales as the B operand: S^T's rows (keys) become the 16 values of the product
         uint32_t bw[NQ][TERMS][2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          const uint32_t raw = vs[t][h][g / 2];
-          const float sv = __half2float(__ushort_as_half((uint16_t)((g & 1) ? raw >> 16 : raw))) * v_up;
+          if constexpr (TERMS == 1) {
+            const __half2 both = as_half2(vn[h][g / 2]), sv = (g & 1) ? __high2half2(both) : __low2half2(both);
 #pragma unroll
-          for (int nq = 0; nq < NQ; nq++) {
-            float x0 = pw[nq][h * 2] * sv, x1 = pw[nq][h * 2 + 1] * sv;
+            for (int nq = 0; nq < NQ; nq++) bw[nq][0][h] = transposed(as_u32(__hmul2(ph[nq][h], sv)));
+          } else {
+            const uint32_t raw = vs[t][h][g / 2];
+            const float sv = __half2float(__ushort_as_half((uint16_t)((g & 1) ? raw >> 16 : raw))) * v_up;
 #pragma unroll
-            for (int k = 0; k < TERMS; k++) {
+            for (int nq = 0; nq < NQ; nq++) {
+              const float x0 = pw[nq][h * 2] * sv, x1 = pw[nq][h * 2 + 1] * sv;
               const __half2 v = __floats2half2_rn(x0, x1);
-              bw[nq][k][h] = transposed(as_u32(v));
-              if (k + 1 < TERMS) {
-                const float2 f = __half22float2(v);
-                x0 -= f.x;
-                x1 -= f.y;
-              }
+              const float2 f = __half22float2(v);
+              bw[nq][0][h] = transposed(as_u32(v));
+              bw[nq][1][h] = transposed(as_u32(__floats2half2_rn(x0 - f.x, x1 - f.y)));
             }
           }
         }
@@ -583,9 +603,9 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
   // The warps' O, maxima and sums, merged in shared memory (the rings are done): [warp][row](D values, m, l)
   cp_async_wait<0>();
   __syncthreads();
-  constexpr int PITCH = D + 4;
+  constexpr int PITCH = MERGE_PITCH<D>;
   float* mem = reinterpret_cast<float*>(smem);
-  const float v_down = __uint_as_float(((v_top >> 10) + 106u) << 23);  // 2^-(21 - exponent field)
+  const float v_down = __uint_as_float(((v_top >> 10) + (TERMS == 1 ? 112u : 106u)) << 23);  // 2^-(15 - e), 2^-(21 - e)
 #pragma unroll
   for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
@@ -623,118 +643,7 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
       else store_out<WE_BF16>(p.out, at + e, v[e]);
     }
   };
-  struct Sum {  // of parts of a row: 4 values and the sum of weights, relative to the row's maximum over the parts
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-    __device__ __forceinline__ void add(float4 x, float m, float sum, float top) {
-      const float f = m == -INFINITY ? 0.f : ex2_ftz(m - top);  // -inf: the part saw no key of the row
-      v.x = fmaf(x.x, f, v.x);
-      v.y = fmaf(x.y, f, v.y);
-      v.z = fmaf(x.z, f, v.z);
-      v.w = fmaf(x.w, f, v.w);
-      l = fmaf(sum, f, l);
-    }
-  };
-  // the CTA's warps, into a place of its own
-  float* cta = mem + WARPS * QROWS * PITCH;
-  for (int x = threadIdx.x; x < QROWS * (D / 4); x += THREADS) {
-    const int r = x / (D / 4), d = x % (D / 4) * 4;
-    const float* from = mem + r * PITCH;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WARPS; w++) top = fmaxf(top, from[w * QROWS * PITCH + D]);
-    Sum sum;
-#pragma unroll
-    for (int w = 0; w < WARPS; w++, from += QROWS * PITCH) sum.add(*reinterpret_cast<const float4*>(from + d), from[D], from[D + 1], top);
-    *reinterpret_cast<float4*>(cta + r * PITCH + d) = sum.v;
-    if (d == 0) {
-      cta[r * PITCH + D] = top;
-      cta[r * PITCH + D + 1] = sum.l;
-    }
-  }
-  __syncwarp();
-  tc::cluster_sync_all();
-  // the cluster's CTAs: a CTA takes an eighth of the values
-  constexpr int ITEMS = QROWS * (D / 4) / CLUSTER;
-  const uint32_t cta_addr = (uint32_t)__cvta_generic_to_shared(cta);
-  auto remote = [](uint32_t addr, int cta_rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(tc::map_rank(addr, cta_rank)) : "memory");
-    return v;
-  };
-  float* part = runs > 1 ? p.part + (int64_t)unit * (gridDim.x / CLUSTER) * (QROWS * PITCH) : nullptr;
-  for (int x = threadIdx.x; x < ITEMS; x += THREADS) {
-    const int r = (rank * ITEMS + x) / (D / 4), d = (rank * ITEMS + x) % (D / 4) * 4;
-    const uint32_t at = cta_addr + 4 * (r * PITCH);
-    float ms[CLUSTER], ls[CLUSTER], top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < CLUSTER; w++) {
-      ms[w] = remote(at + 4 * D, w);
-      ls[w] = remote(at + 4 * (D + 1), w);
-      top = fmaxf(top, ms[w]);
-    }
-    Sum sum;
-#pragma unroll
-    for (int w = 0; w < CLUSTER; w++) {
-      float4 v;
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                   : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                   : "r"(tc::map_rank(at + 4 * d, w))
-                   : "memory");
-      sum.add(v, ms[w], ls[w], top);
-    }
-    if (runs == 1) {
-      finish(r, d, sum.v, sum.l);
-    } else {
-      float* to = part + ((int64_t)run * QROWS + r) * PITCH;
-      *reinterpret_cast<float4*>(to + d) = sum.v;
-      if (d == 0) {
-        to[D] = top;
-        to[D + 1] = sum.l;
-      }
-    }
-  }
-  if (runs > 1) __threadfence();
-  __syncwarp();
-  tc::cluster_sync_all();  // no CTA leaves while another reads its place; the cluster's part is written
-  if (runs == 1) return;
-  // the last cluster of the unit to get here merges all of its parts, in the order of the keys, a CTA an eighth of the values
-  if (rank == 0 && threadIdx.x == 0) {
-    const int is_last = atomicAdd(p.done + unit, 1u) == (uint32_t)runs - 1u;
-    if (is_last) p.done[unit] = 0u;
-    __threadfence();
-    const uint32_t flag = (uint32_t)__cvta_generic_to_shared(&last);
-    for (int w = 0; w < CLUSTER; w++)
-      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::map_rank(flag, w)), "r"(is_last) : "memory");
-  }
-  __syncwarp();
-  tc::cluster_sync_all();
-  if (!last) return;
-  __threadfence();
-  // 4 threads share the runs of one item
-  for (int x = threadIdx.x / 4; x < ITEMS; x += THREADS / 4) {
-    const int r = (rank * ITEMS + x) / (D / 4), d = (rank * ITEMS + x) % (D / 4) * 4, sub = threadIdx.x & 3;
-    const float* from = part + (int64_t)r * PITCH;
-    float top = -INFINITY;
-    for (int z = 0; z < runs; z++) top = fmaxf(top, from[(int64_t)z * (QROWS * PITCH) + D]);
-    Sum sum;
-    const int z1 = runs * (sub + 1) / 4;
-#pragma unroll 4
-    for (int z = runs * sub / 4; z < z1; z++) {
-      const float* row = from + (int64_t)z * (QROWS * PITCH);
-      sum.add(*reinterpret_cast<const float4*>(row + d), row[D], row[D + 1], top);
-    }
-#pragma unroll
-    for (int w = 1; w < 4; w *= 2) {
-      const uint32_t quad = 0xfu << (lane & ~3);
-      sum.v.x += __shfl_xor_sync(quad, sum.v.x, w);
-      sum.v.y += __shfl_xor_sync(quad, sum.v.y, w);
-      sum.v.z += __shfl_xor_sync(quad, sum.v.z, w);
-      sum.v.w += __shfl_xor_sync(quad, sum.v.w, w);
-      sum.l += __shfl_xor_sync(quad, sum.l, w);
-    }
-    if (sub == 0) finish(r, d, sum.v, sum.l);
-  }
+  merge_parts<D, QROWS, WARPS, CLUSTER>(mem, p.part, p.done, &last, unit, (int)gridDim.x / CLUSTER, runs, run, rank, finish);
 }
 
 static unsigned grid_of(int64_t work, int per_cta, int sms, int ctas_per_sm) {
@@ -776,12 +685,13 @@ Kv4Plan kv4_plan(const Kv4AttnArgs& a, int sms) {
   q.nq = rows <= 8 ? 1 : 2;
   q.row_tiles = (int)((rows + 8 * q.nq - 1) / (8 * q.nq));
   q.units = a.c.batch * a.c.kv_heads * q.row_tiles;
-  // Four CTAs an SM. A sequence's length is known on the device only, so runs are cut for the longest possible one, into
+  // Four CTAs an SM, less what no cluster of 8 fits into (71 of 74 do). A sequence's length is known on the device only, so runs are cut for the longest possible one, into
   // about one wave of CTAs; more and shorter ones cost more in their first and last steps than ragged lengths gain (68 us
-  // against 81 with four waves for 16 sequences of 3001 to 16384 keys, 68 against 78 for one of 131000).
+  // against 81 with four waves for 16 sequences of 3001 to 16384 keys, 60 against 78 for one of 131000).
   const int64_t cap = std::max<int64_t>(1, a.c.max_pages * a.c.page);
-  const int64_t chunk = (cap * q.units + sms * 4 - 1) / (sms * 4);
-  q.chunk = (int)std::min<int64_t>((std::max<int64_t>(chunk, 128) + 31) / 32 * 32, 0x4000000);
+  const int64_t runs = std::max<int64_t>(1, (int64_t)(sms * 4 - 24) / (q.units * kv::CLUSTER));
+  const int64_t chunk = std::max<int64_t>(128, (cap + runs * kv::CLUSTER - 1) / (runs * kv::CLUSTER));
+  q.chunk = (int)((std::min<int64_t>(chunk, 0x4000000) + 31) / 32 * 32);
   q.runs = (int)((cap + (int64_t)q.chunk * kv::CLUSTER - 1) / ((int64_t)q.chunk * kv::CLUSTER));
   q.part_floats = q.runs > 1 ? q.units * q.runs * 8 * q.nq * (a.c.dim + 4) : 0;
   return q;
