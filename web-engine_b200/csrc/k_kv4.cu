@@ -107,8 +107,8 @@ __global__ void kv4_advance_kernel(int32_t* lengths, int64_t batch, int32_t toke
 //   times the key's scale of v, times a power of two that keeps it in f16's range (2^15 at most), is the other operand,
 //   turned by movmatrix from S^T's layout. The offset 8 is taken out at the end with the sum of those weights, which one
 //   more tile of ones accumulates.
-// - f32 q or out (TERMS = 2): q and the weights are two f16 terms each (22 bits), and codes of v become exact signed f16
-//   by one more operation, because weights are all positive and the offset's sum would cost 3 to 5 bits.
+// - f32 q or out (TERMS = 2): q and the weights are two f16 terms each (22 bits), and codes become signed f16 by one more
+//   operation, because the offset's sums would cost 2 bits of a score and, weights being positive, up to 5 of an output.
 // - A warp takes 16 or 32 keys at a time through a ring of its own (cp.async), with its own running maximum; the O and
 //   sums are only rescaled when the maximum grows by more than 2^8 or v's scales outgrow their power of two.
 // - A cluster of 8 CTAs shares the keys of a sequence evenly and merges over distributed shared memory; a longer sequence
@@ -342,13 +342,13 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
       sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
       sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
     }
-    const float back = p.scale_log2 * 512.f * __uint_as_float(ex << 23);  // 2^24 2^-15 2^E
+    const float back = p.scale_log2 * (TERMS == 1 ? 512.f : 3.0517578125e-5f) * __uint_as_float(ex << 23);  // (2^24) 2^-15 2^E
 #pragma unroll
     for (int k = 0; k < 2; k++) {
       const int from = (c * 2 + k) * 4;
       q_back[nq][k] = __shfl_sync(0xffffffffu, back, from);
 #pragma unroll
-      for (int g = 0; g < G; g++) q_start[nq][g][k] = q_start[nq][g][2 + k] = __shfl_sync(0xffffffffu, sum[g], from) * -4.76837158203125e-07f;  // -8 2^-24
+      for (int g = 0; g < G; g++) q_start[nq][g][k] = q_start[nq][g][2 + k] = TERMS == 1 ? __shfl_sync(0xffffffffu, sum[g], from) * -4.76837158203125e-07f : 0.f;  // -8 2^-24
     }
   }
 
@@ -365,6 +365,7 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
   uint32_t v_top = 1u << 10;  // the largest scale of v so far, as f16 bits (at least the smallest normal one)
   uint32_t low = 0x000f000fu, high = 0x00f000f0u;  // in registers: a pair of codes is one operation with its other constant
   asm volatile("" : "+r"(low), "+r"(high));
+  const __half2 sub1 = __float2half2_rn(-1032.f), sub16 = __float2half2_rn(-1152.f);
   const int full = have + (rtile * QROWS) / p.group + 1;  // keys below are seen by every row of the tile
 
   // offsets of this lane's pieces of a tile: for k words 2 c, 2 c + 1 of a group of its key and (+ 8 rows) the other; for v
@@ -402,8 +403,16 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
 #pragma unroll
         for (int x = 0; x < 4; x++) {  // word x / 2, half x % 2
           const uint32_t wa = (x < 2 ? a2.x : a2.y) >> ((x & 1) * 8), wb = (x < 2 ? b2.x : b2.y) >> ((x & 1) * 8);
-          const uint32_t av[4] = {and_xor(wa, low, 0x00080008u), and_xor(wb, low, 0x00080008u),
-                                  and_xor(wa, high, 0x00800080u), and_xor(wb, high, 0x00800080u)};
+          uint32_t av[4];
+          if constexpr (TERMS == 1) {
+            av[0] = and_xor(wa, low, 0x00080008u), av[1] = and_xor(wb, low, 0x00080008u);
+            av[2] = and_xor(wa, high, 0x00800080u), av[3] = and_xor(wb, high, 0x00800080u);
+          } else {  // 1024 + u - 1032 = q, 1024 + 16 u - 1152 = 16 q
+            av[0] = as_u32(__hadd2(as_half2(and_xor(wa, low, 0x64086408u)), sub1));
+            av[1] = as_u32(__hadd2(as_half2(and_xor(wb, low, 0x64086408u)), sub1));
+            av[2] = as_u32(__hadd2(as_half2(and_xor(wa, high, 0x64806480u)), sub16));
+            av[3] = as_u32(__hadd2(as_half2(and_xor(wb, high, 0x64806480u)), sub16));
+          }
 #pragma unroll
           for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
@@ -575,19 +584,17 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
         for (int h = 0; h < 2; h++) {  // dims 8 u + 4 h ..
           const uint32_t x = __byte_perm(v0, v1, h ? 0x7632 : 0x5410), y = __byte_perm(v2, v3, h ? 0x7632 : 0x5410);
 #pragma unroll
-          for (int j = 0; j < 2; j++) {  // rows u and u + 8 of the tile: dims 8 u + 4 h + 2 j and the next (for TERMS 1 times 16)
+          for (int j = 0; j < 2; j++) {  // rows u and u + 8 of the tile: dims 8 u + 4 h + 2 j and the next (times 16)
             const uint32_t xs = x >> (8 * j), ys = y >> (8 * j);
             uint32_t av[4];
             if constexpr (TERMS == 1) {
               av[0] = and_xor(xs, low, 0x00080008u), av[1] = and_xor(xs, high, 0x00800080u);
               av[2] = and_xor(ys, low, 0x00080008u), av[3] = and_xor(ys, high, 0x00800080u);
             } else {
-              // 1024 + u - 1032, and (1024 + 16 u) / 16 - 72: q exactly
-              const __half2 sub = __float2half2_rn(-1032.f), sixteenth = __float2half2_rn(0.0625f), sub2 = __float2half2_rn(-72.f);
-              av[0] = as_u32(__hadd2(as_half2(and_xor(xs, low, 0x64086408u)), sub));
-              av[1] = as_u32(__hfma2(as_half2(and_xor(xs, high, 0x64806480u)), sixteenth, sub2));
-              av[2] = as_u32(__hadd2(as_half2(and_xor(ys, low, 0x64086408u)), sub));
-              av[3] = as_u32(__hfma2(as_half2(and_xor(ys, high, 0x64806480u)), sixteenth, sub2));
+              av[0] = as_u32(__hadd2(as_half2(and_xor(xs, low, 0x64086408u)), sub1));
+              av[1] = as_u32(__hadd2(as_half2(and_xor(xs, high, 0x64806480u)), sub16));
+              av[2] = as_u32(__hadd2(as_half2(and_xor(ys, low, 0x64086408u)), sub1));
+              av[3] = as_u32(__hadd2(as_half2(and_xor(ys, high, 0x64806480u)), sub16));
             }
 #pragma unroll
             for (int nq = 0; nq < NQ; nq++)
@@ -622,6 +629,8 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
           const float off = 8.f * w_sum[nq][t / 4][k];
           x0 = fmaf(x0, 16777216.f, -off);
           x1 = fmaf(x1, 1048576.f, -off);
+        } else {
+          x1 *= 0.0625f;
         }
         *reinterpret_cast<float2*>(to + (t / 4) * 64 + u * 8 + (t % 4) * 2) = make_float2(x0 * v_down, x1 * v_down);
       }

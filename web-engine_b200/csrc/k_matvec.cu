@@ -12,8 +12,9 @@
 //   starting each group's sum at -8 sum(x): sum u x - 8 sum x = sum q x.
 // - x is laid out once per CTA as f16 in the order of the tiles, each group of 64 times a power of two that brings its
 //   maximum to 2^15. bf16 values keep all their bits down to 2^-24 of the maximum (below, an error of at most 2^-36 of
-//   it); an f32 value is two columns, 11 bits and the next 11 times 2^10, together within 2^-22. So a product is exact
-//   or within 2^-22, sums are f32, and a group's two scales are one f32 multiply-add per output.
+//   it); an f32 value is two columns, 11 bits and the next 11 times 2^10, together within 2^-22, and its codes take one
+//   more operation to be signed f16, because the offset's sums would cost 2 to 3 bits of f32. So a product is exact or
+//   within 2^-22, sums are f32, and a group's two scales are one f32 multiply-add per output.
 // - A lane reads 16 bytes of a channel at once, so the four lanes of a tile's row hold two groups of 64. A token
 //   therefore is two columns, one per group, each zero where the lane's values belong to the other group: one product
 //   gives both groups' sums side by side and each takes its own scale.
@@ -125,6 +126,15 @@ __device__ __forceinline__ uint32_t and_xor(uint32_t v, uint32_t mask, uint32_t 
 
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ float2 unpack_f16x2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+
+// A pair of codes in the low (odd = 0) or high nibbles of the halves of v, high ones times 16: as u 2^-24, u = q + 8, or
+// (PIECES = 2) as q: 1024 + u - 1032, 1024 + 16 u - 1152.
+template <int PIECES>
+__device__ __forceinline__ uint32_t code_pair(uint32_t v, uint32_t mask, int odd) {
+  if constexpr (PIECES == 1) return and_xor(v, mask, odd ? 0x00800080u : 0x00080008u);
+  const uint32_t b = and_xor(v, mask, odd ? 0x64806480u : 0x64086408u);
+  return as_u32(__hadd2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(odd ? -1152.f : -1032.f)));
+}
 
 // XT: type of x; NT: tiles of 8 columns; RT: row tiles of 16 channels of a warp; PER_SM: CTAs that fit an SM. Columns 2 t
 // and 2 t + 1 are the two groups of a chunk for piece t / m (f32: the leading bits, the following ones) of token t % m.
@@ -275,7 +285,7 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
         piece[4] = make_uint4(o[4], o[5], o[6], o[7]);
         if ((e & 3) == 0) {  // group (e / 4) % 2 of chunk e / 8; an infinity or NaN makes its row NaN
           float* at = reinterpret_cast<float*>(base + (e >> 3) * TOKS + i + c * m) + ((e >> 2) & 1);
-          at[0] = ex == 255u ? __uint_as_float(0x7fc00000u) : s * -4.76837158203125e-07f;  // -8 2^-24
+          at[0] = ex == 255u ? __uint_as_float(0x7fc00000u) : PIECES == 1 ? s * -4.76837158203125e-07f : 0.f;  // -8 2^-24
           at[2] = power * (c ? 9.765625e-4f : 1.f);
         }
       }
@@ -335,10 +345,10 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
             const uint4 &l4 = wq[st][2 * r], &h4 = wq[st][2 * r + 1];
             const uint32_t lo = q == 0 ? l4.x : q == 1 ? l4.y : q == 2 ? l4.z : l4.w, lo8 = lo >> 8;
             const uint32_t hi = q == 0 ? h4.x : q == 1 ? h4.y : q == 2 ? h4.z : h4.w, hi8 = hi >> 8;
-            const uint32_t a0[4] = {and_xor(lo, low, 0x00080008u), and_xor(hi, low, 0x00080008u),
-                                    and_xor(lo, high, 0x00800080u), and_xor(hi, high, 0x00800080u)};
-            const uint32_t a1[4] = {and_xor(lo8, low, 0x00080008u), and_xor(hi8, low, 0x00080008u),
-                                    and_xor(lo8, high, 0x00800080u), and_xor(hi8, high, 0x00800080u)};
+            const uint32_t a0[4] = {code_pair<PIECES>(lo, low, 0), code_pair<PIECES>(hi, low, 0),
+                                    code_pair<PIECES>(lo, high, 1), code_pair<PIECES>(hi, high, 1)};
+            const uint32_t a1[4] = {code_pair<PIECES>(lo8, low, 0), code_pair<PIECES>(hi8, low, 0),
+                                    code_pair<PIECES>(lo8, high, 1), code_pair<PIECES>(hi8, high, 1)};
 #pragma unroll
             for (int t = 0; t < NT; t++) {
               mma_f16(d[r][t], a0, b[t].x, b[t].y);
@@ -348,9 +358,10 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
         }
 #pragma unroll
         for (int r = 0; r < RT; r++) {
-          // with 2^24 2^-15; the powers come last, in the addition, so that sums of tiny values are rounded once
-          const float2 s0 = __fmul2_rn(unpack_f16x2(sc[st][2 * r]), make_float2(512.f, 512.f));
-          const float2 s1 = __fmul2_rn(unpack_f16x2(sc[st][2 * r + 1]), make_float2(512.f, 512.f));
+          // with (2^24) 2^-15; the powers come last, in the addition, so that sums of tiny values are rounded once
+          constexpr float F = PIECES == 1 ? 512.f : 3.0517578125e-5f;
+          const float2 s0 = __fmul2_rn(unpack_f16x2(sc[st][2 * r]), make_float2(F, F));
+          const float2 s1 = __fmul2_rn(unpack_f16x2(sc[st][2 * r + 1]), make_float2(F, F));
 #pragma unroll
           for (int t = 0; t < NT; t++) {
             float(&u)[4] = d[r][t];
