@@ -165,6 +165,8 @@ void kv4_attention_scratch(const Kv4AttnArgs& a, int sms, int64_t* part_bytes, i
 cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, void* part, uint32_t* done, uint32_t* err, int sms,
                                  cudaStream_t st);
 
-cudaError_t launch_cross_simt(const we_cross_desc& d, int sms, cudaStream_t st);
+// Strides and scale of `d` are resolved. Scratch and counters as kv4_attention_scratch; grid_y: CTAs along y (at most 65535).
+void cross_tile_scratch(const we_cross_desc& d, int sms, int64_t* part_bytes, int64_t* units, int64_t* grid_y);
+cudaError_t launch_cross_tile(const we_cross_desc& d, void* part, uint32_t* done, int sms, cudaStream_t st);
 
 }  // namespace we

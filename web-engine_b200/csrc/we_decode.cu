@@ -1,6 +1,7 @@
 // The C ABI of the decoder-side operators (include/we_b200.h): few-row products with 4-bit weights, the paged 4-bit
 // K/V cache and its attention, and cross attention. Argument checks and dispatch; the kernels are in k_matvec.cu,
 // k_kv4.cu and k_cross.cu.
+#include <algorithm>
 #include <string>
 
 #include "common.cuh"
@@ -210,7 +211,39 @@ int we_cross_attention(we_ctx* ctx, const we_cross_desc* desc) {
   if (!d.k_stride) d.k_stride = kw;
   if (!d.v_stride) d.v_stride = kw;
   if (d.scale == 0.f) d.scale = 1.f / sqrtf((float)d.dim);
-  DLK(we::launch_cross_simt(d, we_num_sms(ctx), we_ctx_stream(ctx)), "cross attention");
+  const int64_t group = d.heads / d.kv_heads;
+  if (d.tq > 0x7fffffff / group) return we_ctx_fail(ctx, WE_EINVAL, "cross attention: tq * heads / kv_heads must fit 31 bits");
+  // a call of many query rows goes in pieces whose tiles fit a grid
+  const int64_t most = std::max<int64_t>(1, 65535 / d.kv_heads * 8 / group);
+  const we_cross_desc whole = d;
+  for (int64_t b = 0; b < (whole.tq > most ? whole.batch : 1); b++)
+    for (int64_t t = 0; t < whole.tq; t += most) {
+      if (whole.tq > most) {  // then entry by entry: a piece's rows follow each other
+        d = whole;
+        d.batch = 1;
+        d.tq = std::min(most, whole.tq - t);
+        d.q = static_cast<const char*>(whole.q) + (b * whole.tq + t) * whole.q_stride * es;
+        d.out = static_cast<char*>(whole.out) + (b * whole.tq + t) * whole.out_stride * dsize(d.out_dtype);
+        d.k = static_cast<const char*>(whole.k) + b * whole.tk * whole.k_stride * es;
+        d.v = static_cast<const char*>(whole.v) + b * whole.tk * whole.v_stride * es;
+        if (whole.key_lengths) d.key_lengths = whole.key_lengths + b;
+        if (whole.key_mask) d.key_mask = whole.key_mask + b * whole.tk;
+      }
+      int64_t part_bytes, units, grid_y;
+      we::cross_tile_scratch(d, we_num_sms(ctx), &part_bytes, &units, &grid_y);
+      if (grid_y > 65535) return we_ctx_fail(ctx, WE_EINVAL, "cross attention: too many heads in one call");
+      void* part = nullptr;
+      uint32_t* done = nullptr;
+      if (units > 0) {
+        done = we_ctx_counters(ctx, units);
+        if (!done) return we_ctx_fail(ctx, WE_EINVAL, "cross attention: too many rows to split in one call");
+        int rc = we_ctx_scratch_take(ctx, (size_t)part_bytes, &part);
+        if (rc != WE_OK) return rc;
+      }
+      const cudaError_t e = we::launch_cross_tile(d, part, done, we_num_sms(ctx), we_ctx_stream(ctx));
+      if (part) we_ctx_scratch_put(ctx, part);
+      DLK(e, "cross attention");
+    }
   return WE_OK;
 }
 
