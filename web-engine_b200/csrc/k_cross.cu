@@ -17,7 +17,7 @@
 namespace we {
 
 namespace cross {
-constexpr int WARPS = 4, THREADS = WARPS * 32, CLUSTER = 8, TILE = 16;
+constexpr int WARPS = 4, THREADS = WARPS * 32, TILE = 16;
 
 struct Params {
   we_cross_desc d;  // strides and scale resolved
@@ -74,8 +74,9 @@ __device__ __forceinline__ int piece(int r, int ch, int is_v) {
 }
 }  // namespace cross
 
-// F32: type of q, k and v; D: dim rounded up; NQ: tiles of 8 query rows; DEPTH: steps of 16 keys in a warp's ring.
-template <bool F32, int D, int NQ, int DEPTH>
+// F32: type of q, k and v; D: dim rounded up; NQ: tiles of 8 query rows; DEPTH: steps of 16 keys in a warp's ring; CLUSTER:
+// CTAs that share a run of keys.
+template <bool F32, int D, int NQ, int DEPTH, int CLUSTER>
 __global__ void __launch_bounds__(cross::THREADS) cross_tile_kernel(const cross::Params p) {
   using namespace cross;
   constexpr int ES = F32 ? 4 : 2, ROW = D * ES, SIDE = TILE * ROW, STAGE = 2 * SIDE, QROWS = 8 * NQ, MTILES = D / 16;
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(cross::THREADS) cross_tile_kernel(const cross:
 // ---------------- host side ----------------
 namespace {
 struct CrossPlan {
-  int dim, nq, depth, row_tiles, runs, chunk;  // dim: rounded up to 64, 128 or 256
+  int dim, nq, row_tiles, cluster, runs, chunk;  // dim: rounded up to 64, 128 or 256
   int64_t units, part_floats;
 };
 CrossPlan cross_plan(const we_cross_desc& d, int sms) {
@@ -408,23 +409,24 @@ CrossPlan cross_plan(const we_cross_desc& d, int sms) {
   const bool f32 = d.dtype == WE_F32;
   q.dim = d.dim <= 64 ? 64 : d.dim <= 128 ? 128 : 256;
   q.nq = rows <= 8 ? 1 : 2;
-  q.depth = f32 && q.dim == 256 ? 1 : 2;
   q.row_tiles = (int)((rows + 8 * q.nq - 1) / (8 * q.nq));
   q.units = d.batch * d.kv_heads * q.row_tiles;
   // about one wave of runs (as the cached attention's plan), by the CTAs that fit an SM's shared memory
   const int per_sm = f32 ? (q.dim == 64 ? 3 : 1) : (q.dim == 64 ? 4 : q.dim == 128 ? 3 : 1);
   const int64_t slots = (int64_t)sms * per_sm - 8 * per_sm, tk = std::max<int64_t>(1, d.tk);
-  const int64_t runs = std::max<int64_t>(1, slots / (q.units * cross::CLUSTER));
-  const int64_t chunk = std::max<int64_t>(64, (tk + runs * cross::CLUSTER - 1) / (runs * cross::CLUSTER));
+  // where the row tiles alone fill the SMs, a CTA takes all keys of its rows
+  q.cluster = q.nq == 2 && q.units >= slots ? 1 : 8;
+  const int64_t runs = std::max<int64_t>(1, slots / (q.units * q.cluster));
+  const int64_t chunk = std::max<int64_t>(64, (tk + runs * q.cluster - 1) / (runs * q.cluster));
   q.chunk = (int)((std::min<int64_t>(chunk, 0x4000000) + 15) / 16 * 16);
-  q.runs = (int)((tk + (int64_t)q.chunk * cross::CLUSTER - 1) / ((int64_t)q.chunk * cross::CLUSTER));
+  q.runs = (int)((tk + (int64_t)q.chunk * q.cluster - 1) / ((int64_t)q.chunk * q.cluster));
   q.part_floats = q.runs > 1 ? q.units * q.runs * 8 * q.nq * (q.dim + 4) : 0;
   return q;
 }
 
-template <bool F32, int D, int NQ, int DEPTH>
+template <bool F32, int D, int NQ, int DEPTH, int CLUSTER>
 cudaError_t cross_tile(const cross::Params& p, dim3 grid, cudaStream_t st) {
-  auto kern = cross_tile_kernel<F32, D, NQ, DEPTH>;
+  auto kern = cross_tile_kernel<F32, D, NQ, DEPTH, CLUSTER>;
   constexpr int es = F32 ? 4 : 2;
   constexpr int ring = (F32 ? NQ * (D / 8) * 512 : 0) + cross::WARPS * DEPTH * 2 * cross::TILE * D * es;
   constexpr int merge = (cross::WARPS + 1) * 8 * NQ * MERGE_PITCH<D> * 4;
@@ -438,7 +440,7 @@ cudaError_t cross_tile(const cross::Params& p, dim3 grid, cudaStream_t st) {
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cross::CLUSTER;
+  attr[0].val.clusterDim.x = CLUSTER;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   pdl_attribute(attr[1]);
   cfg.attrs = attr;
@@ -471,9 +473,12 @@ cudaError_t launch_cross_tile(const we_cross_desc& d, void* part, uint32_t* done
   p.scale_log2 = d.scale * 1.4426950408889634f;
   p.part = static_cast<float*>(part);
   p.done = done;
-  const dim3 grid((unsigned)(q.runs * cross::CLUSTER), (unsigned)(d.kv_heads * q.row_tiles), (unsigned)d.batch);
+  const dim3 grid((unsigned)(q.runs * q.cluster), (unsigned)(d.kv_heads * q.row_tiles), (unsigned)d.batch);
   cudaError_t e;
-#define CROSS_CASE(F32, D, DEPTH) e = q.nq == 1 ? cross_tile<F32, D, 1, DEPTH>(p, grid, st) : cross_tile<F32, D, 2, DEPTH>(p, grid, st)
+#define CROSS_CASE(F32, D, DEPTH)                                          \
+  e = q.cluster == 1 ? cross_tile<F32, D, 2, DEPTH, 1>(p, grid, st)        \
+      : q.nq == 1    ? cross_tile<F32, D, 1, DEPTH, 8>(p, grid, st)        \
+                     : cross_tile<F32, D, 2, DEPTH, 8>(p, grid, st)
   if (f32) {
     if (q.dim == 64) CROSS_CASE(true, 64, 2);
     else if (q.dim == 128) CROSS_CASE(true, 128, 2);
