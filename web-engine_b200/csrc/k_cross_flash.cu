@@ -1,15 +1,17 @@
 // Cross attention with many queries on tcgen05: bf16, heads of 64 or 128.
 //
-// One CTA = 128 queries of one head over the head's keys in tiles of 128. Warp 0 brings Q and the K and V tiles by TMA, one
-// thread of warp 1 issues S = Q K^T and O += P V (kind::f16, accumulators in TMEM, P read from TMEM over the first half of
-// S's columns, V an MN-major operand as it is stored), warps 2 to 5 run the softmax, a thread a query row. Text states are a
-// few tiles, so a CTA lives for a few steps only and each step is a chain (S, softmax, P V): what keeps the tensor cores fed
-// is a second CTA on the SM (256 TMEM columns and about 100 KB of shared memory each), which also covers the other's first
-// loads and last stores. S is read from TMEM twice (64 columns at a time: for the maximum, then for the weights) so that a
-// thread stays below 168 registers.
+// A CTA takes items of 128 queries of one head, one after the other, over the head's keys in tiles of 128. Warp 0 brings Q and
+// the K and V tiles by TMA, one thread of warp 1 issues S = Q K^T and O += P V (kind::f16, accumulators in TMEM, P read from
+// TMEM over the first half of S's columns, V an MN-major operand as it is stored), warps 2 to 9 run the softmax, a thread one
+// query row and one half of the tile's keys (the two exchange their maxima through shared memory).
+// Text states are a few tiles, so an item is a few steps only and each step is a chain (S, softmax, P V): what keeps the
+// tensor cores fed is a second CTA on the SM (256 TMEM columns and about 100 KB of shared memory each), and that a CTA's next
+// item is under way while the last one is written: its Q, K and V are loaded and its first S computed by then.
 // Hidden keys (past a length, or masked) have scores of -inf, and the softmax warps write zeros over their rows of V in
 // shared memory before they hand P over, so that nothing of them reaches a product; tiles without any skip both.
 #include <cudaTypedefs.h>
+
+#include <algorithm>
 
 #include "attn_merge.cuh"
 #include "common.cuh"
@@ -21,13 +23,14 @@ namespace we {
 namespace cf {
 constexpr int B = 128;            // queries of a CTA, keys of a tile
 constexpr int ATOM = B * 128;     // 128 rows of 64 bf16 (one swizzle-128B box)
-constexpr int THREADS = 192;
+constexpr int SOFTMAX_WARPS = 8;   // 4 row quarters x 2 halves of the keys (and of O's columns)
+constexpr int THREADS = 64 + SOFTMAX_WARPS * 32;
 constexpr uint32_t TMEM_COLS = 256, O_COL = 128;
 constexpr float RESCALE_LOG2 = 8.f;
 
 struct Params {
-  int64_t tq, tk, out_stride;
-  int heads, group;  // group: heads per kv head
+  int64_t tq, tk, out_stride, items;
+  int heads, group, q_tiles;  // group: heads per kv head; items = batch * heads * q_tiles
   float scale_log2;
   void* out;
   int out_dtype;
@@ -40,8 +43,9 @@ template <int D>
 struct Layout {
   static constexpr int STAGES = D == 64 ? 2 : 1, TILE = D / 64 * ATOM;
   static constexpr int Q = 0, K = TILE, V = K + STAGES * TILE, BARS = V + STAGES * TILE;
-  static constexpr int NUM_BARS = 1 + 4 * STAGES + 4;
-  static constexpr int BYTES = BARS + NUM_BARS * 8 + 16 + 1024;
+  static constexpr int NUM_BARS = 4 * STAGES + 8;                    // (a multiple of 2)
+  static constexpr int RED = BARS + NUM_BARS * 8 + 16;               // row maxima of two tile parities and row sums, by halves
+  static constexpr int BYTES = RED + 3 * 2 * B * 4 + 1024;
   static constexpr uint32_t IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(B >> 3) << 17) | ((uint32_t)(B >> 4) << 24);
   static constexpr uint32_t IDESC_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(B >> 4) << 24);
 };
@@ -75,26 +79,28 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
   const uint32_t sbase = smem_u32(smem), bars = sbase + L::BARS;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::BARS + L::NUM_BARS * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  const uint32_t Q_FULL = bars, S_FULL = bars + 8 * (1 + 4 * NS), P_FULL = S_FULL + 8, O_DONE = S_FULL + 16, DRAIN = S_FULL + 24;
-  auto K_FULL = [&](int s) { return bars + 8u * (1 + s); };
-  auto K_EMPTY = [&](int s) { return bars + 8u * (1 + NS + s); };
-  auto V_FULL = [&](int s) { return bars + 8u * (1 + 2 * NS + s); };
-  auto V_EMPTY = [&](int s) { return bars + 8u * (1 + 3 * NS + s); };
+  const uint32_t MISC = bars + 8 * 4 * NS, Q_FULL = MISC, Q_EMPTY = MISC + 8, S_FULL = MISC + 16, P_FULL = MISC + 24,
+                 O_DONE = MISC + 32, O_FREE = MISC + 40, DRAIN = MISC + 48;
+  auto K_FULL = [&](int s) { return bars + 8u * s; };
+  auto K_EMPTY = [&](int s) { return bars + 8u * (NS + s); };
+  auto V_FULL = [&](int s) { return bars + 8u * (2 * NS + s); };
+  auto V_EMPTY = [&](int s) { return bars + 8u * (3 * NS + s); };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int q0 = blockIdx.x * B, h = blockIdx.y, b = blockIdx.z, g = h / p.group;
 
   if (threadIdx.x == 0) {
-    mbar_init(Q_FULL, 1);
     for (int i = 0; i < NS; i++) {
       mbar_init(K_FULL(i), 1);
       mbar_init(K_EMPTY(i), 1);
       mbar_init(V_FULL(i), 1);
       mbar_init(V_EMPTY(i), 1);
     }
+    mbar_init(Q_FULL, 1);
+    mbar_init(Q_EMPTY, 1);
     mbar_init(S_FULL, 1);
-    mbar_init(P_FULL, 4);
+    mbar_init(P_FULL, SOFTMAX_WARPS);
     mbar_init(O_DONE, 1);
+    mbar_init(O_FREE, SOFTMAX_WARPS);
     mbar_init(DRAIN, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -110,34 +116,55 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
   pdl_launch_dependents();
   const uint32_t tmem = *tmem_holder;
 
-  int keys = (int)p.tk;
-  if (p.key_lengths) keys = max(0, min(keys, p.key_lengths[b]));
-  const int nt = (keys + B - 1) / B;
+  // The items of this CTA, in every role alike: query tile fastest, then heads, then entries. An item without keys takes part
+  // in no barrier. `tiles` and `done` count the tiles and the items with keys so far: the parities of the barriers.
+  struct Item {
+    int q0, h, b, keys, nt;
+  };
+  auto item = [&](int64_t i) {
+    Item x;
+    x.q0 = (int)(i % p.q_tiles) * B;
+    const int bh = (int)(i / p.q_tiles);
+    x.h = bh % p.heads;
+    x.b = bh / p.heads;
+    x.keys = (int)p.tk;
+    if (p.key_lengths) x.keys = max(0, min(x.keys, p.key_lengths[x.b]));
+    x.nt = (x.keys + B - 1) / B;
+    return x;
+  };
 
   if (warp == 0) {
-    if (lane == 0 && nt > 0) {
-      auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar, int head, int row) {
-        mbar_expect_tx(bar, L::TILE);
-#pragma unroll
-        for (int x = 0; x < D / 64; x++) tma_load_3d(dst + x * ATOM, map, bar, head * D + x * 64, row, b);
-      };
+    if (lane == 0) {
       bool ok = true;
-      load(&tm_q, sbase + L::Q, Q_FULL, h, q0);
-      int k_issued = 0, v_issued = 0;
-      for (int j = 0; j < nt && ok; j++) {
-        const int s = j % NS;
-        const uint32_t free_parity = ((j / NS) & 1) ^ 1u;
-        ok = wait_fast(K_EMPTY(s), free_parity, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER, WAIT_LIMIT_NS, true);
+      int tiles = 0, done = 0, k_issued = 0, v_issued = 0;
+      for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+        const Item x = item(i);
+        if (x.nt == 0) continue;
+        const int g = x.h / p.group;
+        auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar, int head, int row) {
+          mbar_expect_tx(bar, L::TILE);
+#pragma unroll
+          for (int c = 0; c < D / 64; c++) tma_load_3d(dst + c * ATOM, map, bar, head * D + c * 64, row, x.b);
+        };
+        ok = wait_fast(Q_EMPTY, (done & 1) ^ 1u, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER, WAIT_LIMIT_NS, true);
         if (!ok) break;
-        load(&tm_k, sbase + L::K + s * L::TILE, K_FULL(s), g, j * B);
-        k_issued = j + 1;
-        ok = wait_fast(V_EMPTY(s), free_parity, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER, WAIT_LIMIT_NS, true);
-        if (!ok) break;
-        load(&tm_v, sbase + L::V + s * L::TILE, V_FULL(s), g, j * B);
-        v_issued = j + 1;
+        load(&tm_q, sbase + L::Q, Q_FULL, x.h, x.q0);
+        done++;
+        for (int j = 0; j < x.nt; j++, tiles++) {
+          const int s = tiles % NS;
+          const uint32_t free_parity = ((tiles / NS) & 1) ^ 1u;
+          ok = wait_fast(K_EMPTY(s), free_parity, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER, WAIT_LIMIT_NS, true);
+          if (!ok) break;
+          load(&tm_k, sbase + L::K + s * L::TILE, K_FULL(s), g, j * B);
+          k_issued = tiles + 1;
+          ok = wait_fast(V_EMPTY(s), free_parity, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER, WAIT_LIMIT_NS, true);
+          if (!ok) break;
+          load(&tm_v, sbase + L::V + s * L::TILE, V_FULL(s), g, j * B);
+          v_issued = tiles + 1;
+        }
       }
       if (!ok) {  // the copies already issued land before the CTA exits
-        wait_fast(Q_FULL, 0, abort_flag, p.err, DEV_ERR_TIMEOUT_DRAIN, DRAIN_LIMIT_NS, false);
+        if (done > 0) wait_fast(Q_FULL, (done - 1) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_DRAIN, DRAIN_LIMIT_NS, false);
         for (int t = max(0, k_issued - NS); t < k_issued; t++)
           wait_fast(K_FULL(t % NS), (t / NS) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_DRAIN, DRAIN_LIMIT_NS, false);
         for (int t = max(0, v_issued - NS); t < v_issued; t++)
@@ -146,11 +173,12 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && nt > 0) {
-      bool ok = wait_fast(Q_FULL, 0, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA, WAIT_LIMIT_NS, true);
-      auto s_mma = [&](int j) -> bool {  // S(j) = Q K_j^T
-        const int s = j % NS;
-        if (!wait_fast(K_FULL(s), (j / NS) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA, WAIT_LIMIT_NS, true)) return false;
+    if (lane == 0) {
+      bool ok = true;
+      int tiles = 0, done = 0;
+      auto s_mma = [&](int t) -> bool {  // S(t) = Q K_t^T
+        const int s = t % NS;
+        if (!wait_fast(K_FULL(s), (t / NS) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA, WAIT_LIMIT_NS, true)) return false;
         tc_fence_after();
         const uint64_t qdesc = sw128_desc(sbase + L::Q), kdesc = sw128_desc(sbase + L::K + s * L::TILE);
 #pragma unroll
@@ -162,20 +190,28 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
         umma_commit(K_EMPTY(s));
         return true;
       };
-      ok = ok && s_mma(0);
-      for (int j = 0; j < nt && ok; j++) {
-        const int s = j % NS;
-        ok = wait_fast(P_FULL, j & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA, WAIT_LIMIT_NS, true) &&
-             wait_fast(V_FULL(s), (j / NS) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA, WAIT_LIMIT_NS, true);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t vdesc = mn_sw128_desc(sbase + L::V + s * L::TILE, ATOM);
+      for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+        const Item x = item(i);
+        if (x.nt == 0) continue;
+        ok = wait_fast(Q_FULL, done & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA, WAIT_LIMIT_NS, true) && s_mma(tiles);
+        for (int j = 0; j < x.nt && ok; j++, tiles++) {
+          const int s = tiles % NS;
+          if (j + 1 == x.nt) umma_commit(Q_EMPTY);  // the item's last S is issued: Q is free once it is done
+          // the item before must be out of O before this one's first product overwrites it
+          ok = wait_spin(P_FULL, tiles & 1, 4096, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA, WAIT_LIMIT_NS, true) &&
+               wait_fast(V_FULL(s), (tiles / NS) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA, WAIT_LIMIT_NS, true) &&
+               (j > 0 || wait_fast(O_FREE, (done & 1) ^ 1u, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA, WAIT_LIMIT_NS, true));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t vdesc = mn_sw128_desc(sbase + L::V + s * L::TILE, ATOM);
 #pragma unroll
-        for (int kk = 0; kk < 8; kk++)  // 128 keys: 8 products of 16 (16 rows of 128 bytes of V, 8 columns of P)
-          umma_tmem_a(tmem + O_COL, tmem + (uint32_t)(kk * 8), vdesc + (uint64_t)(kk * (16 * 128 >> 4)), L::IDESC_O, (j | kk) != 0);
-        umma_commit(V_EMPTY(s));
-        if (j + 1 < nt) ok = s_mma(j + 1);
-        else umma_commit(O_DONE);
+          for (int kk = 0; kk < 8; kk++)  // 128 keys: 8 products of 16 (16 rows of 128 bytes of V, 8 columns of P)
+            umma_tmem_a(tmem + O_COL, tmem + (uint32_t)(kk * 8), vdesc + (uint64_t)(kk * (16 * 128 >> 4)), L::IDESC_O, (j | kk) != 0);
+          umma_commit(V_EMPTY(s));
+          if (j + 1 < x.nt) ok = s_mma(tiles + 1);
+          else umma_commit(O_DONE);
+        }
+        done++;
       }
       // every product this thread issued completes before TMEM is freed
       umma_commit(DRAIN);
@@ -183,76 +219,74 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, r = quarter * 32 + lane;
-    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint8_t* mask = p.key_mask ? p.key_mask + (int64_t)b * p.tk : nullptr;
-    float m = NONE, l = 0.f;
+    const int quarter = warp & 3, half = (warp - 2) >> 2, r = quarter * 32 + lane;
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16), o_addr = lane_addr + O_COL + half * (D / 2);
+    const uint32_t pair_bar = 1u + quarter;  // the two warps of a row quarter
+    float* red = reinterpret_cast<float*>(smem + L::RED);  // [2 parities][2 halves][128 rows], then [2 halves][128 rows] of sums
+    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
-    for (int j = 0; j < nt; j++) {
-      // which keys of the tile are seen
-      uint32_t bits[4];
-#pragma unroll
-      for (int w = 0; w < 4; w++) {
-        const int key = j * B + w * 32 + lane;
-        bits[w] = __ballot_sync(0xffffffffu, key < keys && (!mask || mask[key] != 0));
-      }
-      const bool whole = (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu;
-      ok = wait_fast(S_FULL, j & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE, WAIT_LIMIT_NS, true);
-      if (ok && !whole) ok = wait_fast(V_FULL(j % NS), (j / NS) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE, WAIT_LIMIT_NS, true);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      if (!whole && !((bits[quarter] >> lane) & 1)) {  // zeros over this thread's key of V
-#pragma unroll
-        for (int x = 0; x < D / 64; x++)
-#pragma unroll
-          for (int e = 0; e < 8; e++)
-            *reinterpret_cast<uint4*>(smem + L::V + (j % NS) * L::TILE + x * ATOM + r * 128 + e * 16) = make_uint4(0, 0, 0, 0);
-      }
-      if (!whole) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      uint32_t sc[64];
-      auto load_half = [&](int half) {
+    int tiles = 0, done = 0;
+    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+      const Item it = item(i);
+      const uint8_t* mask = p.key_mask ? p.key_mask + (int64_t)it.b * p.tk : nullptr;
+      float m = NONE, l = 0.f;
+      for (int j = 0; j < it.nt; j++, tiles++) {
+        // which of this half's keys are seen
+        const int key = j * B + half * 64 + lane, s = tiles % NS;
+        const uint32_t w0 = __ballot_sync(0xffffffffu, key < it.keys && (!mask || mask[key] != 0));
+        const uint32_t w1 = __ballot_sync(0xffffffffu, key + 32 < it.keys && (!mask || mask[key + 32] != 0));
+        const bool whole = (w0 & w1) == 0xffffffffu;
+        ok = wait_fast(S_FULL, tiles & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE, WAIT_LIMIT_NS, true);
+        if (ok && !whole) ok = wait_fast(V_FULL(s), (tiles / NS) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE, WAIT_LIMIT_NS, true);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+        uint32_t sc[64];
         tmem_ld32_async(lane_addr + half * 64, *reinterpret_cast<uint32_t(*)[32]>(sc));
         tmem_ld32_async(lane_addr + half * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(sc + 32));
+        if (!whole && ok) {  // zeros over the hidden keys' rows of V: a warp 16 of its half's rows
+          uint8_t* v = smem + L::V + s * L::TILE + (half * 64 + quarter * 16) * 128;
+          const uint32_t hidden = ~(quarter < 2 ? w0 : w1) >> ((quarter & 1) * 16);
+          for (int at = lane; at < 16 * 8; at += 32)
+            if ((hidden >> (at >> 3)) & 1)
+#pragma unroll
+              for (int c = 0; c < D / 64; c++) *reinterpret_cast<uint4*>(v + c * ATOM + at * 16) = make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
         tmem_wait_ld(*reinterpret_cast<uint32_t(*)[32]>(sc));
         reg_fence(*reinterpret_cast<uint32_t(*)[32]>(sc + 32));
         if (!whole) {
-          const uint32_t w0 = half ? bits[2] : bits[0], w1 = half ? bits[3] : bits[1];
 #pragma unroll
           for (int c = 0; c < 32; c++) {
             if (!((w0 >> c) & 1)) sc[c] = 0xff800000u;
             if (!((w1 >> c) & 1)) sc[32 + c] = 0xff800000u;
           }
         }
-      };
-      auto half_max = [&]() {
         float mx[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) mx[i] = fmaxf(__uint_as_float(sc[2 * i]), __uint_as_float(sc[2 * i + 1]));
+        for (int c = 0; c < 4; c++) mx[c] = fmaxf(__uint_as_float(sc[2 * c]), __uint_as_float(sc[2 * c + 1]));
 #pragma unroll
         for (int c = 8; c < 64; c += 8)
 #pragma unroll
-          for (int i = 0; i < 4; i++) mx[i] = max3(mx[i], __uint_as_float(sc[c + 2 * i]), __uint_as_float(sc[c + 2 * i + 1]));
-        return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      };
-      load_half(1);
-      const float top1 = half_max();
-      load_half(0);
-      const float top = fmaxf(half_max(), top1) * p.scale_log2;
-      float corr = 1.f;
-      const bool grow = top > m + RESCALE_LOG2;
-      if (grow) {
-        corr = ex2_ftz(m - top);
-        l *= corr;
-        m = top;
-      }
-      const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(-m, -m);
-      float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-      for (int half = 0; half < 2; half++) {
-        if (half) load_half(1);
+          for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], __uint_as_float(sc[c + 2 * e]), __uint_as_float(sc[c + 2 * e + 1]));
+        float* rm = red + (tiles & 1) * 2 * B;
+        rm[half * B + r] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        // the exchange also ANDs the two warps' wait results, so that a pair always leaves the loop together, and orders both
+        // halves' reads of S before the writes of P over its columns
+        if (!named_bar_and(pair_bar, 64, ok)) {
+          ok = false;
+          break;
+        }
+        const float top = fmaxf(rm[r], rm[B + r]) * p.scale_log2;
+        float corr = 1.f;
+        const bool grow = top > m + RESCALE_LOG2;
+        if (grow) {
+          corr = ex2_ftz(m - top);
+          l *= corr;
+          m = top;
+        }
+        const float2 nm2 = make_float2(-m, -m);
+        float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         uint32_t pk[32];
 #pragma unroll
         for (int e = 0; e < 32; e++) {
@@ -261,60 +295,71 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
           sum[e & 3] = __fadd2_rn(sum[e & 3], w);
           pk[e] = pack_bf16_up(w.x, w.y);
         }
-        tmem_st32(lane_addr + half * 32, pk);  // P over columns of S that have been read
-      }
-      l += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) + ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
-      // O is scaled for the old maximum (P V of the tile before is done: its commit came before S's)
-      if (__any_sync(0xffffffffu, grow && j > 0)) {
+        tmem_st32(lane_addr + half * 32, pk);
+        l += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) + ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
+        // O is scaled for the old maximum (P V of the tile before is done: its commit came before S's)
+        if (__any_sync(0xffffffffu, grow && j > 0)) {
 #pragma unroll
-        for (int c = 0; c < D / 32; c++) {
-          uint32_t u[32];
-          tmem_ld32(lane_addr + O_COL + c * 32, u);
+          for (int c = 0; c < D / 64; c++) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + c * 32, o);
 #pragma unroll
-          for (int e = 0; e < 32; e++) u[e] = __float_as_uint(__uint_as_float(u[e]) * corr);
-          tmem_st32(lane_addr + O_COL + c * 32, u);
+            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+            tmem_st32(o_addr + c * 32, o);
+          }
         }
+        tmem_st_wait();  // P (and O) are in TMEM before the products read them
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(P_FULL);
       }
-      tmem_st_wait();  // P (and O) are in TMEM before the products read them
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(P_FULL);
-    }
-    if (ok && nt > 0) {
-      ok = wait_fast(O_DONE, 0, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE, WAIT_LIMIT_NS, true);
-      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      // the row's sum over both halves; the second barrier keeps the next item's sums behind these reads
+      float* row_sum = red + 4 * B;
+      row_sum[half * B + r] = l;
+      if (it.nt > 0) ok = wait_fast(O_DONE, done & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE, WAIT_LIMIT_NS, true);
+      ok = named_bar_and(pair_bar, 64, __all_sync(0xffffffffu, ok));
+      if (!ok) break;
       tc_fence_after();
-    }
-    if (ok) {
-      const int qi = q0 + r;
+      l = row_sum[r] + row_sum[B + r];
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key seen: zeros; NaN stays
+      const int64_t at0 = ((int64_t)it.b * p.tq + it.q0 + r) * p.out_stride + (int64_t)it.h * D + half * (D / 2);
 #pragma unroll
-      for (int c = 0; c < D / 32; c++) {
-        uint32_t u[32];
-        if (nt > 0) {
-          tmem_ld32(lane_addr + O_COL + c * 32, u);
+      for (int c = 0; c < D / 64; c++) {
+        uint32_t o[32];
+        if (it.nt > 0) {
+          tmem_ld32(o_addr + c * 32, o);
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; e++) u[e] = 0;
+          for (int e = 0; e < 32; e++) o[e] = 0;
         }
-        if (qi >= p.tq) continue;
-        const int64_t at = ((int64_t)b * p.tq + qi) * p.out_stride + (int64_t)h * D + c * 32;
-        if (p.out_dtype == WE_BF16) {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            dst[e] = make_uint4(pack_bf16x2(__uint_as_float(u[8 * e]) * inv, __uint_as_float(u[8 * e + 1]) * inv),
-                                pack_bf16x2(__uint_as_float(u[8 * e + 2]) * inv, __uint_as_float(u[8 * e + 3]) * inv),
-                                pack_bf16x2(__uint_as_float(u[8 * e + 4]) * inv, __uint_as_float(u[8 * e + 5]) * inv),
-                                pack_bf16x2(__uint_as_float(u[8 * e + 6]) * inv, __uint_as_float(u[8 * e + 7]) * inv));
-        } else {
-          float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
-#pragma unroll
-          for (int e = 0; e < 8; e++)
-            dst[e] = make_float4(__uint_as_float(u[4 * e]) * inv, __uint_as_float(u[4 * e + 1]) * inv,
-                                 __uint_as_float(u[4 * e + 2]) * inv, __uint_as_float(u[4 * e + 3]) * inv);
+        if (c + 1 == D / 64 && it.nt > 0) {  // this warp has read its part of O
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(O_FREE);
         }
+        if (it.q0 + r < p.tq) {
+          const int64_t at = at0 + c * 32;
+          if (p.out_dtype == WE_BF16) {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              dst[e] = make_uint4(pack_bf16x2(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv),
+                                  pack_bf16x2(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv),
+                                  pack_bf16x2(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv),
+                                  pack_bf16x2(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv));
+          } else {
+            float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+              dst[e] = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
+                                   __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
+          }
+        }
+        __syncwarp();
       }
+      named_bar_sync(pair_bar, 64);
+      if (it.nt > 0) done++;
     }
   }
   tc_fence_before();
@@ -351,18 +396,19 @@ bool cross_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, i
 }
 
 template <int D>
-cudaError_t cross_flash(const we_cross_desc& d, uint32_t* err, cudaStream_t st) {
+cudaError_t cross_flash(const we_cross_desc& d, uint32_t* err, int sms, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
   if (!cross_map(&mq, d.q, d.heads * D, d.tq, d.batch, d.q_stride) ||
       !cross_map(&mk, d.k, d.kv_heads * D, d.tk, d.batch, d.k_stride) ||
       !cross_map(&mv, d.v, d.kv_heads * D, d.tk, d.batch, d.v_stride))
     return cudaErrorNotSupported;
-  cf::Params p{d.tq, d.tk, d.out_stride, (int)d.heads, (int)(d.heads / d.kv_heads), d.scale * 1.4426950408889634f,
-               d.out, d.out_dtype, d.key_lengths, d.key_mask, err};
+  const int64_t q_tiles = (d.tq + cf::B - 1) / cf::B, items = q_tiles * d.heads * d.batch;
+  cf::Params p{d.tq, d.tk, d.out_stride, items, (int)d.heads, (int)(d.heads / d.kv_heads), (int)q_tiles,
+               d.scale * 1.4426950408889634f, d.out, d.out_dtype, d.key_lengths, d.key_mask, err};
   constexpr int bytes = cf::Layout<D>::BYTES;
   cudaError_t e = cudaFuncSetAttribute(cross_flash_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)((d.tq + cf::B - 1) / cf::B), (unsigned)d.heads, (unsigned)d.batch);
+  const dim3 grid((unsigned)std::min<int64_t>(items, 2 * sms));
   e = launch_pdl(cross_flash_kernel<D>, grid, cf::THREADS, bytes, st, mq, mk, mv, p);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
@@ -379,8 +425,8 @@ bool cross_flash_supported(const we_cross_desc& d) {
   return (bits & 15) == 0 && d.tq * d.q_stride < most && d.tk * d.k_stride < most && d.tk * d.v_stride < most;
 }
 
-cudaError_t launch_cross_flash(const we_cross_desc& d, uint32_t* err, cudaStream_t st) {
-  return d.dim == 64 ? cross_flash<64>(d, err, st) : cross_flash<128>(d, err, st);
+cudaError_t launch_cross_flash(const we_cross_desc& d, uint32_t* err, int sms, cudaStream_t st) {
+  return d.dim == 64 ? cross_flash<64>(d, err, sms, st) : cross_flash<128>(d, err, sms, st);
 }
 
 }  // namespace we

@@ -169,7 +169,7 @@ cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, void* part, uint32_t* don
 void cross_tile_scratch(const we_cross_desc& d, int sms, int64_t* part_bytes, int64_t* units, int64_t* grid_y);
 // the tcgen05 kernel, for many queries
 bool cross_flash_supported(const we_cross_desc& d);
-cudaError_t launch_cross_flash(const we_cross_desc& d, uint32_t* err, cudaStream_t st);
+cudaError_t launch_cross_flash(const we_cross_desc& d, uint32_t* err, int sms, cudaStream_t st);
 cudaError_t launch_cross_tile(const we_cross_desc& d, void* part, uint32_t* done, int sms, cudaStream_t st);
 
 }  // namespace we

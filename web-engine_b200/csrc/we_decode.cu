@@ -216,7 +216,7 @@ int we_cross_attention(we_ctx* ctx, const we_cross_desc* desc) {
   int64_t from = 64;
   if (const char* env = getenv("WE_CROSS_FLASH")) from = atoi(env);  // test / tuning override: queries from which it is used
   if (d.tq >= from && we::cross_flash_supported(d)) {
-    const cudaError_t e = we::launch_cross_flash(d, we_ctx_dev_err(ctx), we_ctx_stream(ctx));
+    const cudaError_t e = we::launch_cross_flash(d, we_ctx_dev_err(ctx), we_num_sms(ctx), we_ctx_stream(ctx));
     if (e != cudaErrorNotSupported) {
       DLK(e, "cross attention");
       return WE_OK;
