@@ -64,6 +64,33 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 __device__ __forceinline__ uint32_t pack_bf16_up(float lo, float hi) {  // non-negative, to nearest (ties up)
   return __byte_perm(__float_as_uint(lo) + 0x8000u, __float_as_uint(hi) + 0x8000u, 0x7632);
 }
+// Lane t of four holds pieces 0..3 of row t; afterwards piece t of rows 0..3.
+__device__ __forceinline__ void transpose4(uint4 (&w)[4], int lane) {
+  auto swap = [&](uint4& lo, uint4& hi, int bit) {  // the lane with the bit gives its lo for the other's hi
+    const bool up = (lane & bit) != 0;
+    uint4 x = up ? lo : hi;
+    x.x = __shfl_xor_sync(0xffffffffu, x.x, bit);
+    x.y = __shfl_xor_sync(0xffffffffu, x.y, bit);
+    x.z = __shfl_xor_sync(0xffffffffu, x.z, bit);
+    x.w = __shfl_xor_sync(0xffffffffu, x.w, bit);
+    if (up) lo = x;
+    else hi = x;
+  };
+  swap(w[0], w[1], 1);
+  swap(w[2], w[3], 1);
+  swap(w[0], w[2], 2);
+  swap(w[1], w[3], 2);
+}
+// 64 bytes of each of the warp's 32 rows (lane = row, `stride` values apart, the first at `out`); only the first `rows` are stored.
+template <typename T>
+__device__ __forceinline__ void store_quads(uint4 (&w)[4], T* out, int64_t stride, int64_t rows, int lane) {
+  transpose4(w, lane);
+  const int row = lane & ~3;
+  T* at = out + row * stride + (lane & 3) * (16 / (int)sizeof(T));
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    if (row + e < rows) *reinterpret_cast<uint4*>(at + e * stride) = w[e];
+}
 }  // namespace cf
 
 template <int D>
@@ -323,7 +350,8 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
       tc_fence_after();
       l = row_sum[r] + row_sum[B + r];
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key seen: zeros; NaN stays
-      const int64_t at0 = ((int64_t)it.b * p.tq + it.q0 + r) * p.out_stride + (int64_t)it.h * D + half * (D / 2);
+      const int64_t at0 = ((int64_t)it.b * p.tq + it.q0 + quarter * 32) * p.out_stride + (int64_t)it.h * D + half * (D / 2);
+      const int64_t rows = p.tq - it.q0 - quarter * 32;  // of this warp's 32
 #pragma unroll
       for (int c = 0; c < D / 64; c++) {
         uint32_t o[32];
@@ -338,25 +366,30 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
           __syncwarp();
           if (lane == 0) mbar_arrive(O_FREE);
         }
-        if (it.q0 + r < p.tq) {
-          const int64_t at = at0 + c * 32;
-          if (p.out_dtype == WE_BF16) {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
+        // 16-byte pieces of the lanes' rows are exchanged among four lanes, so that a store writes 64 bytes of a row: with
+        // each lane storing its own row an item took 10400 cycles to write, of about 29000
+        if (p.out_dtype == WE_BF16) {
+          uint4 w[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-              dst[e] = make_uint4(pack_bf16x2(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv),
-                                  pack_bf16x2(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv),
-                                  pack_bf16x2(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv),
-                                  pack_bf16x2(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv));
-          } else {
-            float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+          for (int e = 0; e < 4; e++)
+            w[e] = make_uint4(pack_bf16x2(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv),
+                              pack_bf16x2(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv),
+                              pack_bf16x2(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv),
+                              pack_bf16x2(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv));
+          store_quads(w, static_cast<uint16_t*>(p.out) + at0 + c * 32, p.out_stride, rows, lane);
+        } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-              dst[e] = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
-                                   __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
+          for (int i2 = 0; i2 < 2; i2++) {
+            uint4 w[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const int at = i2 * 16 + 4 * e;
+              w[e] = make_uint4(__float_as_uint(__uint_as_float(o[at]) * inv), __float_as_uint(__uint_as_float(o[at + 1]) * inv),
+                                __float_as_uint(__uint_as_float(o[at + 2]) * inv), __float_as_uint(__uint_as_float(o[at + 3]) * inv));
+            }
+            store_quads(w, static_cast<float*>(p.out) + at0 + c * 32 + i2 * 16, p.out_stride, rows, lane);
           }
         }
-        __syncwarp();
       }
       named_bar_sync(pair_bar, 64);
       if (it.nt > 0) done++;
