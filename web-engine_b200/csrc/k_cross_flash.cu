@@ -251,9 +251,9 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
     const uint32_t pair_bar = 1u + quarter;  // the two warps of a row quarter
     float* red = reinterpret_cast<float*>(smem + L::RED);  // [2 parities][2 halves][128 rows], then [2 halves][128 rows] of sums
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
-    bool ok = true;
+    bool ok = true, stop = false;  // ok: of this warp; the two warps of a pair only leave together, by a barrier's answer
     int tiles = 0, done = 0;
-    for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+    for (int64_t i = blockIdx.x; i < p.items; i += gridDim.x) {
       const Item it = item(i);
       const uint8_t* mask = p.key_mask ? p.key_mask + (int64_t)it.b * p.tk : nullptr;
       float m = NONE, l = 0.f;
@@ -263,23 +263,12 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
         const uint32_t w0 = __ballot_sync(0xffffffffu, key < it.keys && (!mask || mask[key] != 0));
         const uint32_t w1 = __ballot_sync(0xffffffffu, key + 32 < it.keys && (!mask || mask[key + 32] != 0));
         const bool whole = (w0 & w1) == 0xffffffffu;
-        ok = wait_fast(S_FULL, tiles & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE, WAIT_LIMIT_NS, true);
-        if (ok && !whole) ok = wait_fast(V_FULL(s), (tiles / NS) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE, WAIT_LIMIT_NS, true);
+        ok = ok && wait_fast(S_FULL, tiles & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE, WAIT_LIMIT_NS, true);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
         uint32_t sc[64];
         tmem_ld32_async(lane_addr + half * 64, *reinterpret_cast<uint32_t(*)[32]>(sc));
         tmem_ld32_async(lane_addr + half * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(sc + 32));
-        if (!whole && ok) {  // zeros over the hidden keys' rows of V: a warp 16 of its half's rows
-          uint8_t* v = smem + L::V + s * L::TILE + (half * 64 + quarter * 16) * 128;
-          const uint32_t hidden = ~(quarter < 2 ? w0 : w1) >> ((quarter & 1) * 16);
-          for (int at = lane; at < 16 * 8; at += 32)
-            if ((hidden >> (at >> 3)) & 1)
-#pragma unroll
-              for (int c = 0; c < D / 64; c++) *reinterpret_cast<uint4*>(v + c * ATOM + at * 16) = make_uint4(0, 0, 0, 0);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
         tmem_wait_ld(*reinterpret_cast<uint32_t(*)[32]>(sc));
         reg_fence(*reinterpret_cast<uint32_t(*)[32]>(sc + 32));
         if (!whole) {
@@ -301,7 +290,7 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
         // the exchange also ANDs the two warps' wait results, so that a pair always leaves the loop together, and orders both
         // halves' reads of S before the writes of P over its columns
         if (!named_bar_and(pair_bar, 64, ok)) {
-          ok = false;
+          stop = true;
           break;
         }
         const float top = fmaxf(rm[r], rm[B + r]) * p.scale_log2;
@@ -335,18 +324,32 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
             tmem_st32(o_addr + c * 32, o);
           }
         }
+        if (!whole) {  // zeros over the hidden keys' rows of V (here by now): a warp 16 of its half's rows
+          ok = ok && wait_fast(V_FULL(s), (tiles / NS) & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE, WAIT_LIMIT_NS, true);
+          ok = __all_sync(0xffffffffu, ok);
+          uint8_t* v = smem + L::V + s * L::TILE + (half * 64 + quarter * 16) * 128;
+          const uint32_t hidden = ~(quarter < 2 ? w0 : w1) >> ((quarter & 1) * 16);
+          if (ok) {
+#pragma unroll
+            for (int at = lane; at < 16 * 8; at += 32)
+              if ((hidden >> (at >> 3)) & 1)
+#pragma unroll
+                for (int c = 0; c < D / 64; c++) *reinterpret_cast<uint4*>(v + c * ATOM + at * 16) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
         tmem_st_wait();  // P (and O) are in TMEM before the products read them
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(P_FULL);
       }
-      if (!ok) break;
+      if (stop) break;
       // the row's sum over both halves; the second barrier keeps the next item's sums behind these reads
       float* row_sum = red + 4 * B;
       row_sum[half * B + r] = l;
-      if (it.nt > 0) ok = wait_fast(O_DONE, done & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE, WAIT_LIMIT_NS, true);
-      ok = named_bar_and(pair_bar, 64, __all_sync(0xffffffffu, ok));
-      if (!ok) break;
+      if (it.nt > 0) ok = ok && wait_fast(O_DONE, done & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_EPILOGUE, WAIT_LIMIT_NS, true);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!named_bar_and(pair_bar, 64, ok)) break;
       tc_fence_after();
       l = row_sum[r] + row_sum[B + r];
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key seen: zeros; NaN stays
