@@ -183,3 +183,15 @@ def test_refusals(we, graph):
     refused("shorter", k_stride=32)
     refused("f32 or bf16", dtype="fp8")
     refused("65535", batch=70000)
+
+
+@pytest.mark.parametrize("dim,out_dtype", [(64, "bf16"), (128, "bf16"), (128, "f32"), (64, "f32")])
+@pytest.mark.parametrize("tk", [100, 300, 1111])
+def test_more_query_tiles_than_resident_blocks(we, graph, dim, out_dtype, tk):
+    """Blocks that take several query tiles each: entries without keys, with hidden tiles and with whole ones in turn,
+    and rows that end inside a tile."""
+    lengths = [tk, 0, tk // 2, tk - 1, 1]
+    mask = (np.random.default_rng(21).random((5, tk)) < 0.9).astype(np.uint8)
+    mask[3] = 1
+    run(we, graph, 5, 300, tk, 24, 8, dim, "bf16", lengths, mask, out_dtype=out_dtype, seed=22, poison=True)
+    run(we, graph, 5, 300, tk, 24, 24, dim, "bf16", lengths, None, out_dtype=out_dtype, seed=23, poison=True)

@@ -59,11 +59,7 @@ __device__ __forceinline__ void merge_parts(float* mem, float* part_base, uint32
   tc::cluster_sync_all();
   // the cluster's CTAs
   const uint32_t cta_addr = (uint32_t)__cvta_generic_to_shared(cta);
-  auto remote = [](uint32_t addr, int cta_rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(tc::map_rank(addr, cta_rank)) : "memory");
-    return v;
-  };
+  auto remote = [](uint32_t addr, int cta_rank) { return tc::ld_cluster_f32(tc::map_rank(addr, cta_rank)); };
   float* part = runs > 1 ? part_base + (int64_t)unit * all_runs * (QROWS * PITCH) : nullptr;
   for (int x = threadIdx.x; x < ITEMS; x += THREADS) {
     const int r = (rank * ITEMS + x) / (D / 4), d = (rank * ITEMS + x) % (D / 4) * 4;
@@ -78,12 +74,7 @@ __device__ __forceinline__ void merge_parts(float* mem, float* part_base, uint32
     PartSum sum;
 #pragma unroll
     for (int w = 0; w < CLUSTER; w++) {
-      float4 v;
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                   : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                   : "r"(tc::map_rank(at + 4 * d, w))
-                   : "memory");
-      sum.add(v, ms[w], ls[w], top);
+      sum.add(tc::ld_cluster_f32x4(tc::map_rank(at + 4 * d, w)), ms[w], ls[w], top);
     }
     if (runs == 1) {
       finish(r, d, sum.v, sum.l);

@@ -30,7 +30,7 @@ constexpr float RESCALE_LOG2 = 8.f;
 
 struct Params {
   int64_t tq, tk, out_stride, items;
-  int heads, group, q_tiles;  // group: heads per kv head; items = batch * heads * q_tiles
+  int heads, group, q_tiles, splits;  // group: heads per kv head; items = batch * heads * q_tiles; splits: CTAs per item
   float scale_log2;
   void* out;
   int out_dtype;
@@ -93,7 +93,7 @@ __device__ __forceinline__ void store_quads(uint4 (&w)[4], T* out, int64_t strid
 }
 }  // namespace cf
 
-template <int D>
+template <int D, bool SPLIT>
 __global__ void __launch_bounds__(cf::THREADS, 2)
     cross_flash_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const cf::Params p) {
@@ -145,9 +145,11 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
 
   // The items of this CTA, in every role alike: query tile fastest, then heads, then entries. An item without keys takes part
   // in no barrier. `tiles` and `done` count the tiles and the items with keys so far: the parities of the barriers.
+  // SPLIT: a cluster of p.splits CTAs has one item, each CTA its share of the tiles (from tile t0).
   struct Item {
-    int q0, h, b, keys, nt;
+    int q0, h, b, keys, t0, nt;
   };
+  const int64_t first = SPLIT ? blockIdx.x / p.splits : blockIdx.x, step = SPLIT ? p.items : gridDim.x;
   auto item = [&](int64_t i) {
     Item x;
     x.q0 = (int)(i % p.q_tiles) * B;
@@ -156,7 +158,13 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
     x.b = bh / p.heads;
     x.keys = (int)p.tk;
     if (p.key_lengths) x.keys = max(0, min(x.keys, p.key_lengths[x.b]));
+    x.t0 = 0;
     x.nt = (x.keys + B - 1) / B;
+    if constexpr (SPLIT) {
+      const int rank = (int)cluster_rank(), all = x.nt;
+      x.t0 = (int)((int64_t)all * rank / p.splits);
+      x.nt = (int)((int64_t)all * (rank + 1) / p.splits) - x.t0;
+    }
     return x;
   };
 
@@ -164,7 +172,7 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
     if (lane == 0) {
       bool ok = true;
       int tiles = 0, done = 0, k_issued = 0, v_issued = 0;
-      for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+      for (int64_t i = first; i < p.items && ok; i += step) {
         const Item x = item(i);
         if (x.nt == 0) continue;
         const int g = x.h / p.group;
@@ -182,11 +190,11 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
           const uint32_t free_parity = ((tiles / NS) & 1) ^ 1u;
           ok = wait_fast(K_EMPTY(s), free_parity, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER, WAIT_LIMIT_NS, true);
           if (!ok) break;
-          load(&tm_k, sbase + L::K + s * L::TILE, K_FULL(s), g, j * B);
+          load(&tm_k, sbase + L::K + s * L::TILE, K_FULL(s), g, (x.t0 + j) * B);
           k_issued = tiles + 1;
           ok = wait_fast(V_EMPTY(s), free_parity, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER, WAIT_LIMIT_NS, true);
           if (!ok) break;
-          load(&tm_v, sbase + L::V + s * L::TILE, V_FULL(s), g, j * B);
+          load(&tm_v, sbase + L::V + s * L::TILE, V_FULL(s), g, (x.t0 + j) * B);
           v_issued = tiles + 1;
         }
       }
@@ -217,7 +225,7 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
         umma_commit(K_EMPTY(s));
         return true;
       };
-      for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+      for (int64_t i = first; i < p.items && ok; i += step) {
         const Item x = item(i);
         if (x.nt == 0) continue;
         ok = wait_fast(Q_FULL, done & 1, abort_flag, p.err, DEV_ERR_TIMEOUT_MMA, WAIT_LIMIT_NS, true) && s_mma(tiles);
@@ -253,13 +261,13 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true, stop = false;  // ok: of this warp; the two warps of a pair only leave together, by a barrier's answer
     int tiles = 0, done = 0;
-    for (int64_t i = blockIdx.x; i < p.items; i += gridDim.x) {
+    for (int64_t i = first; i < p.items; i += step) {
       const Item it = item(i);
       const uint8_t* mask = p.key_mask ? p.key_mask + (int64_t)it.b * p.tk : nullptr;
       float m = NONE, l = 0.f;
       for (int j = 0; j < it.nt; j++, tiles++) {
         // which of this half's keys are seen
-        const int key = j * B + half * 64 + lane, s = tiles % NS;
+        const int key = (it.t0 + j) * B + half * 64 + lane, s = tiles % NS;
         const uint32_t w0 = __ballot_sync(0xffffffffu, key < it.keys && (!mask || mask[key] != 0));
         const uint32_t w1 = __ballot_sync(0xffffffffu, key + 32 < it.keys && (!mask || mask[key + 32] != 0));
         const bool whole = (w0 & w1) == 0xffffffffu;
@@ -352,6 +360,29 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
       if (!named_bar_and(pair_bar, 64, ok)) break;
       tc_fence_after();
       l = row_sum[r] + row_sum[B + r];
+      if constexpr (SPLIT) {  // this CTA's part of the rows, for the cluster's merge (K and V are read by now)
+        if (half == 0) {
+          red[r] = m;
+          red[B + r] = l;
+        }
+#pragma unroll
+        for (int c = 0; c < D / 64; c++) {
+          uint32_t o[32];
+          if (it.nt > 0) {
+            tmem_ld32(o_addr + c * 32, o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] = 0;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const int piece = (half * (D / 8) + c * 8 + e) ^ (r & 7);
+            *reinterpret_cast<uint4*>(smem + L::K + r * (D * 4) + piece * 16) =
+                make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
+        break;
+      }
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key seen: zeros; NaN stays
       const int64_t at0 = ((int64_t)it.b * p.tq + it.q0 + quarter * 32) * p.out_stride + (int64_t)it.h * D + half * (D / 2);
       const int64_t rows = p.tq - it.q0 - quarter * 32;  // of this warp's 32
@@ -404,6 +435,33 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
   }
+  if constexpr (SPLIT) {  // each CTA joins the parts of its share of the rows, always in the same order
+    __syncwarp();
+    cluster_sync_all();
+    const Item x = item(first);
+    const int rows = B / p.splits;
+    for (int at = threadIdx.x; at < rows * (D / 4); at += THREADS) {
+      const int row = (int)cluster_rank() * rows + at / (D / 4), piece = at % (D / 4);
+      if (x.q0 + row >= p.tq) break;
+      float top = NONE;
+      for (int c = 0; c < p.splits; c++) top = fmaxf(top, ld_cluster_f32(map_rank(sbase + L::RED + row * 4, c)));
+      PartSum sum;
+      for (int c = 0; c < p.splits; c++)
+        sum.add(ld_cluster_f32x4(map_rank(sbase + L::K + row * (D * 4) + (piece ^ (row & 7)) * 16, c)),
+                ld_cluster_f32(map_rank(sbase + L::RED + row * 4, c)),
+                ld_cluster_f32(map_rank(sbase + L::RED + (B + row) * 4, c)), top);
+      const float l = sum.l, inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      const int64_t o = ((int64_t)x.b * p.tq + x.q0 + row) * p.out_stride + (int64_t)x.h * D + piece * 4;
+      if (p.out_dtype == WE_BF16)
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + o) =
+            make_uint2(pack_bf16x2(sum.v.x * inv, sum.v.y * inv), pack_bf16x2(sum.v.z * inv, sum.v.w * inv));
+      else
+        *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) =
+            make_float4(sum.v.x * inv, sum.v.y * inv, sum.v.z * inv, sum.v.w * inv);
+    }
+    __syncwarp();
+    cluster_sync_all();  // no CTA leaves while another reads from it
+  }
 }
 
 // ---------------- host side ----------------
@@ -439,13 +497,30 @@ cudaError_t cross_flash(const we_cross_desc& d, uint32_t* err, int sms, cudaStre
       !cross_map(&mv, d.v, d.kv_heads * D, d.tk, d.batch, d.v_stride))
     return cudaErrorNotSupported;
   const int64_t q_tiles = (d.tq + cf::B - 1) / cf::B, items = q_tiles * d.heads * d.batch;
-  cf::Params p{d.tq, d.tk, d.out_stride, items, (int)d.heads, (int)(d.heads / d.kv_heads), (int)q_tiles,
+  // CTAs that would be idle take a share of the keys (powers of two up to 8 a cluster, a tile of keys each at the least; 24
+  // CTAs fewer than two an SM, because clusters of 8 leave some places of a GPC empty)
+  const int64_t tiles = (d.tk + cf::B - 1) / cf::B;
+  int splits = 1;
+  while (splits < 8 && items * splits * 2 <= 2 * sms - 24 && splits * 2 <= tiles) splits *= 2;
+  cf::Params p{d.tq, d.tk, d.out_stride, items, (int)d.heads, (int)(d.heads / d.kv_heads), (int)q_tiles, splits,
                d.scale * 1.4426950408889634f, d.out, d.out_dtype, d.key_lengths, d.key_mask, err};
   constexpr int bytes = cf::Layout<D>::BYTES;
-  cudaError_t e = cudaFuncSetAttribute(cross_flash_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  const auto kernel = splits > 1 ? cross_flash_kernel<D, true> : cross_flash_kernel<D, false>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)std::min<int64_t>(items, 2 * sms));
-  e = launch_pdl(cross_flash_kernel<D>, grid, cf::THREADS, bytes, st, mq, mk, mv, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(splits > 1 ? items * splits : std::min<int64_t>(items, 2 * sms)));
+  cfg.blockDim = dim3(cf::THREADS);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  pdl_attribute(attr[0]);
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = splits;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  e = cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, p);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
 }  // namespace
