@@ -195,3 +195,10 @@ def test_more_query_tiles_than_resident_blocks(we, graph, dim, out_dtype, tk):
     mask[3] = 1
     run(we, graph, 5, 300, tk, 24, 8, dim, "bf16", lengths, mask, out_dtype=out_dtype, seed=22, poison=True)
     run(we, graph, 5, 300, tk, 24, 24, dim, "bf16", lengths, None, out_dtype=out_dtype, seed=23, poison=True)
+
+
+@pytest.mark.parametrize("tq", [1, 3, 44, 131])
+@pytest.mark.parametrize("heads,kv_heads", [(3, 1), (12, 2), (40, 1), (128, 1), (260, 2)])
+def test_groups_of_heads_that_share_keys(we, graph, heads, kv_heads, tq):
+    """Groups that do not divide a tile of rows, that fill it, and one larger than it."""
+    run(we, graph, 2, tq, 333, heads, kv_heads, 64, "bf16", lengths=[333, 130], seed=31, poison=True)

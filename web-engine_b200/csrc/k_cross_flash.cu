@@ -1,6 +1,7 @@
 // Cross attention with many queries on tcgen05: bf16, heads of 64 or 128.
 //
-// A CTA takes items of 128 queries of one head, one after the other, over the head's keys in tiles of 128. Warp 0 brings Q and
+// A CTA takes items of 128 rows, one after the other, over a kv head's keys in tiles of 128: rows are tokens x the kv head's
+// group of heads, so that a group reads its keys once however few its tokens. Warp 0 brings Q and
 // the K and V tiles by TMA, one thread of warp 1 issues S = Q K^T and O += P V (kind::f16, accumulators in TMEM, P read from
 // TMEM over the first half of S's columns, V an MN-major operand as it is stored), warps 2 to 9 run the softmax, a thread one
 // query row and one half of the tile's keys (the two exchange their maxima through shared memory).
@@ -30,7 +31,8 @@ constexpr float RESCALE_LOG2 = 8.f;
 
 struct Params {
   int64_t tq, tk, out_stride, items;
-  int heads, group, q_tiles, splits;  // group: heads per kv head; items = batch * heads * q_tiles; splits: CTAs per item
+  int kv_heads, group, span, q_tiles, splits;  // group: heads per kv head; span: tokens of an item (span * group rows);
+                                               // items = batch * kv_heads * q_tiles; splits: CTAs per item
   float scale_log2;
   void* out;
   int out_dtype;
@@ -54,6 +56,13 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t c0, int32_t c1, int32_t c2,
+                                            int32_t c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -81,15 +90,13 @@ __device__ __forceinline__ void transpose4(uint4 (&w)[4], int lane) {
   swap(w[0], w[2], 2);
   swap(w[1], w[3], 2);
 }
-// 64 bytes of each of the warp's 32 rows (lane = row, `stride` values apart, the first at `out`); only the first `rows` are stored.
+// 64 bytes of each of the warp's 32 rows (lane = row); to: where rows 4 (lane / 4) + 0..3 go, values from `out`, or -1.
 template <typename T>
-__device__ __forceinline__ void store_quads(uint4 (&w)[4], T* out, int64_t stride, int64_t rows, int lane) {
+__device__ __forceinline__ void store_quads(uint4 (&w)[4], T* out, const int64_t (&to)[4], int lane) {
   transpose4(w, lane);
-  const int row = lane & ~3;
-  T* at = out + row * stride + (lane & 3) * (16 / (int)sizeof(T));
 #pragma unroll
   for (int e = 0; e < 4; e++)
-    if (row + e < rows) *reinterpret_cast<uint4*>(at + e * stride) = w[e];
+    if (to[e] >= 0) *reinterpret_cast<uint4*>(out + to[e] + (lane & 3) * (16 / (int)sizeof(T))) = w[e];
 }
 }  // namespace cf
 
@@ -147,15 +154,15 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
   // in no barrier. `tiles` and `done` count the tiles and the items with keys so far: the parities of the barriers.
   // SPLIT: a cluster of p.splits CTAs has one item, each CTA its share of the tiles (from tile t0).
   struct Item {
-    int q0, h, b, keys, t0, nt;
+    int q0, h, b, keys, t0, nt;  // first token, kv head
   };
   const int64_t first = SPLIT ? blockIdx.x / p.splits : blockIdx.x, step = SPLIT ? p.items : gridDim.x;
   auto item = [&](int64_t i) {
     Item x;
-    x.q0 = (int)(i % p.q_tiles) * B;
+    x.q0 = (int)(i % p.q_tiles) * p.span;
     const int bh = (int)(i / p.q_tiles);
-    x.h = bh % p.heads;
-    x.b = bh / p.heads;
+    x.h = bh % p.kv_heads;
+    x.b = bh / p.kv_heads;
     x.keys = (int)p.tk;
     if (p.key_lengths) x.keys = max(0, min(x.keys, p.key_lengths[x.b]));
     x.t0 = 0;
@@ -168,6 +175,14 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
     return x;
   };
 
+  // Row r of an item: head r % group of the kv head's, token q0 + r / group. Its first value's place in out, -1: no row.
+  const uint32_t recip = (65536u + p.group - 1) / p.group;  // r / group = r recip >> 16, exact for r < 128, group <= 128
+  auto out_at = [&](const Item& x, int r) -> int64_t {
+    const int t = (int)((r * recip) >> 16);
+    if (t >= p.span || x.q0 + t >= p.tq) return -1;
+    return ((int64_t)x.b * p.tq + x.q0 + t) * p.out_stride + ((int64_t)x.h * p.group + r - t * p.group) * D;
+  };
+
   if (warp == 0) {
     if (lane == 0) {
       bool ok = true;
@@ -175,7 +190,6 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
       for (int64_t i = first; i < p.items && ok; i += step) {
         const Item x = item(i);
         if (x.nt == 0) continue;
-        const int g = x.h / p.group;
         auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar, int head, int row) {
           mbar_expect_tx(bar, L::TILE);
 #pragma unroll
@@ -183,18 +197,20 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
         };
         ok = wait_fast(Q_EMPTY, (done & 1) ^ 1u, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER, WAIT_LIMIT_NS, true);
         if (!ok) break;
-        load(&tm_q, sbase + L::Q, Q_FULL, x.h, x.q0);
+        mbar_expect_tx(Q_FULL, (uint32_t)(p.span * p.group) * (D * 2));
+#pragma unroll
+        for (int c = 0; c < D / 64; c++) tma_load_4d(sbase + L::Q + c * ATOM, &tm_q, Q_FULL, c * 64, x.h * p.group, x.q0, x.b);
         done++;
         for (int j = 0; j < x.nt; j++, tiles++) {
           const int s = tiles % NS;
           const uint32_t free_parity = ((tiles / NS) & 1) ^ 1u;
           ok = wait_fast(K_EMPTY(s), free_parity, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER, WAIT_LIMIT_NS, true);
           if (!ok) break;
-          load(&tm_k, sbase + L::K + s * L::TILE, K_FULL(s), g, (x.t0 + j) * B);
+          load(&tm_k, sbase + L::K + s * L::TILE, K_FULL(s), x.h, (x.t0 + j) * B);
           k_issued = tiles + 1;
           ok = wait_fast(V_EMPTY(s), free_parity, abort_flag, p.err, DEV_ERR_TIMEOUT_PRODUCER, WAIT_LIMIT_NS, true);
           if (!ok) break;
-          load(&tm_v, sbase + L::V + s * L::TILE, V_FULL(s), g, (x.t0 + j) * B);
+          load(&tm_v, sbase + L::V + s * L::TILE, V_FULL(s), x.h, (x.t0 + j) * B);
           v_issued = tiles + 1;
         }
       }
@@ -384,8 +400,12 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
         break;
       }
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key seen: zeros; NaN stays
-      const int64_t at0 = ((int64_t)it.b * p.tq + it.q0 + quarter * 32) * p.out_stride + (int64_t)it.h * D + half * (D / 2);
-      const int64_t rows = p.tq - it.q0 - quarter * 32;  // of this warp's 32
+      int64_t to[4];  // where the four rows go that this lane stores pieces of, or -1
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        to[e] = out_at(it, quarter * 32 + (lane & ~3) + e);
+        if (to[e] >= 0) to[e] += half * (D / 2);
+      }
 #pragma unroll
       for (int c = 0; c < D / 64; c++) {
         uint32_t o[32];
@@ -410,7 +430,7 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
                               pack_bf16x2(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv),
                               pack_bf16x2(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv),
                               pack_bf16x2(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv));
-          store_quads(w, static_cast<uint16_t*>(p.out) + at0 + c * 32, p.out_stride, rows, lane);
+          store_quads(w, static_cast<uint16_t*>(p.out) + c * 32, to, lane);
         } else {
 #pragma unroll
           for (int i2 = 0; i2 < 2; i2++) {
@@ -421,7 +441,7 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
               w[e] = make_uint4(__float_as_uint(__uint_as_float(o[at]) * inv), __float_as_uint(__uint_as_float(o[at + 1]) * inv),
                                 __float_as_uint(__uint_as_float(o[at + 2]) * inv), __float_as_uint(__uint_as_float(o[at + 3]) * inv));
             }
-            store_quads(w, static_cast<float*>(p.out) + at0 + c * 32 + i2 * 16, p.out_stride, rows, lane);
+            store_quads(w, static_cast<float*>(p.out) + c * 32 + i2 * 16, to, lane);
           }
         }
       }
@@ -442,7 +462,8 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
     const int rows = B / p.splits;
     for (int at = threadIdx.x; at < rows * (D / 4); at += THREADS) {
       const int row = (int)cluster_rank() * rows + at / (D / 4), piece = at % (D / 4);
-      if (x.q0 + row >= p.tq) break;
+      const int64_t to = out_at(x, row);
+      if (to < 0) break;
       float top = NONE;
       for (int c = 0; c < p.splits; c++) top = fmaxf(top, ld_cluster_f32(map_rank(sbase + L::RED + row * 4, c)));
       PartSum sum;
@@ -451,7 +472,7 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
                 ld_cluster_f32(map_rank(sbase + L::RED + row * 4, c)),
                 ld_cluster_f32(map_rank(sbase + L::RED + (B + row) * 4, c)), top);
       const float l = sum.l, inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-      const int64_t o = ((int64_t)x.b * p.tq + x.q0 + row) * p.out_stride + (int64_t)x.h * D + piece * 4;
+      const int64_t o = to + piece * 4;
       if (p.out_dtype == WE_BF16)
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + o) =
             make_uint2(pack_bf16x2(sum.v.x * inv, sum.v.y * inv), pack_bf16x2(sum.v.z * inv, sum.v.w * inv));
@@ -477,6 +498,17 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn_cross() {
   }
   return fn;
 }
+// [batch, tq, heads, D] of bf16, tokens `stride` values apart, in boxes of 64 values of `group` heads of `span` tokens
+bool cross_q_map(CUtensorMap* map, const we_cross_desc& d, int group, int span) {
+  auto fn = encode_fn_cross();
+  if (!fn) return false;
+  cuuint64_t dims[4] = {(cuuint64_t)d.dim, (cuuint64_t)d.heads, (cuuint64_t)d.tq, (cuuint64_t)d.batch};
+  cuuint64_t strides[3] = {(cuuint64_t)(d.dim * 2), (cuuint64_t)(d.q_stride * 2), (cuuint64_t)(d.tq * d.q_stride * 2)};
+  cuuint32_t box[4] = {64, (cuuint32_t)group, (cuuint32_t)span, 1}, estr[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(d.q), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 // [batch, rows, cols] of bf16, rows `stride` values apart, in boxes of 64 columns x 128 rows with 128-byte swizzle
 bool cross_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t batch, int64_t stride) {
   auto fn = encode_fn_cross();
@@ -492,17 +524,18 @@ bool cross_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, i
 template <int D>
 cudaError_t cross_flash(const we_cross_desc& d, uint32_t* err, int sms, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
-  if (!cross_map(&mq, d.q, d.heads * D, d.tq, d.batch, d.q_stride) ||
+  const int group = (int)(d.heads / d.kv_heads), span = cf::B / group;
+  if (!cross_q_map(&mq, d, group, span) ||
       !cross_map(&mk, d.k, d.kv_heads * D, d.tk, d.batch, d.k_stride) ||
       !cross_map(&mv, d.v, d.kv_heads * D, d.tk, d.batch, d.v_stride))
     return cudaErrorNotSupported;
-  const int64_t q_tiles = (d.tq + cf::B - 1) / cf::B, items = q_tiles * d.heads * d.batch;
+  const int64_t q_tiles = (d.tq + span - 1) / span, items = q_tiles * d.kv_heads * d.batch;
   // CTAs that would be idle take a share of the keys (powers of two up to 8 a cluster, a tile of keys each at the least; 24
   // CTAs fewer than two an SM, because clusters of 8 leave some places of a GPC empty)
   const int64_t tiles = (d.tk + cf::B - 1) / cf::B;
   int splits = 1;
   while (splits < 8 && items * splits * 2 <= 2 * sms - 24 && splits * 2 <= tiles) splits *= 2;
-  cf::Params p{d.tq, d.tk, d.out_stride, items, (int)d.heads, (int)(d.heads / d.kv_heads), (int)q_tiles, splits,
+  cf::Params p{d.tq, d.tk, d.out_stride, items, (int)d.kv_heads, group, span, (int)q_tiles, splits,
                d.scale * 1.4426950408889634f, d.out, d.out_dtype, d.key_lengths, d.key_mask, err};
   constexpr int bytes = cf::Layout<D>::BYTES;
   const auto kernel = splits > 1 ? cross_flash_kernel<D, true> : cross_flash_kernel<D, false>;
@@ -527,7 +560,7 @@ cudaError_t cross_flash(const we_cross_desc& d, uint32_t* err, int sms, cudaStre
 
 // Whether launch_cross_flash takes the call: types, head size, 16-byte rows, sizes of a tensor map.
 bool cross_flash_supported(const we_cross_desc& d) {
-  if (d.dtype != WE_BF16 || (d.dim != 64 && d.dim != 128) || d.tk < 1) return false;
+  if (d.dtype != WE_BF16 || (d.dim != 64 && d.dim != 128) || d.tk < 1 || d.heads / d.kv_heads > cf::B) return false;
   const int64_t os = d.out_dtype == WE_F32 ? 4 : 2;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(d.q) | reinterpret_cast<uintptr_t>(d.k) | reinterpret_cast<uintptr_t>(d.v) |
                          reinterpret_cast<uintptr_t>(d.out) | (uintptr_t)(d.q_stride * 2) | (uintptr_t)(d.k_stride * 2) |

@@ -213,9 +213,9 @@ int we_cross_attention(we_ctx* ctx, const we_cross_desc* desc) {
   if (d.scale == 0.f) d.scale = 1.f / sqrtf((float)d.dim);
   const int64_t group = d.heads / d.kv_heads;
   if (d.tq > 0x7fffffff / group) return we_ctx_fail(ctx, WE_EINVAL, "cross attention: tq * heads / kv_heads must fit 31 bits");
-  int64_t from = 64;
-  if (const char* env = getenv("WE_CROSS_FLASH")) from = atoi(env);  // test / tuning override: queries from which it is used
-  if (d.tq >= from && we::cross_flash_supported(d)) {
+  int64_t from = 9;
+  if (const char* env = getenv("WE_CROSS_FLASH")) from = atoi(env);  // test / tuning override: query rows from which it is used
+  if (d.tq * group >= from && we::cross_flash_supported(d)) {
     const cudaError_t e = we::launch_cross_flash(d, we_ctx_dev_err(ctx), we_num_sms(ctx), we_ctx_stream(ctx));
     if (e != cudaErrorNotSupported) {
       DLK(e, "cross attention");
