@@ -8,10 +8,10 @@
 
 namespace we {
 
-// Row index (in rows of `dim` values) of token t of sequence b and kv head h, or -1 when the page table does not hold
-// it (recorded in the device error word).
-__device__ __forceinline__ int64_t kv4_row(const we_kv4_cache& c, int64_t b, int64_t h, int64_t t, uint32_t* err) {
-  const int64_t slot = t / c.page;
+// Row index (in rows of `dim` values) of token t of sequence b at kv head 0, or -1 when the page table does not hold it
+// (recorded in the device error word). Head h's row is h * page further.
+__device__ __forceinline__ int64_t kv4_row(const we_kv4_cache& c, int64_t b, int64_t t, uint32_t* err) {
+  const uint32_t page = (uint32_t)c.page, slot = (uint32_t)t / page;  // (a page of the table and t are below 2^32)
   if (slot >= c.max_pages) {
     atomicCAS(err, 0u, (uint32_t)DEV_ERR_KV_FULL);
     return -1;
@@ -21,69 +21,198 @@ __device__ __forceinline__ int64_t kv4_row(const we_kv4_cache& c, int64_t b, int
     atomicCAS(err, 0u, (uint32_t)DEV_ERR_KV_PAGE);
     return -1;
   }
-  return (id * c.kv_heads + h) * c.page + t % c.page;
+  return id * c.kv_heads * c.page + ((uint32_t)t - slot * page);
 }
 
-// One warp per (sequence, token, kv head, k or v) group of 64 values: a lane holds two.
-template <int DT>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const we_kv4_cache c, const void* __restrict__ k,
-                                                         const void* __restrict__ v, int64_t tokens, int64_t stride,
-                                                         uint32_t* err) {
+// Rows in and out of the cache. A thread moves 8 values of k or of v a step: 16 bytes (bf16) or 32 on the wide side, a 4-byte
+// word on the packed one, 8 neighbouring lanes a group. It keeps its place within a token (side, head, values) and steps
+// over the tokens of its CTA, whose rows are looked up once, so that a step has little to compute but the values.
+constexpr int ROW_THREADS = 256, ROW_SPAN = 32;
+struct RowShape {
+  int units;       // of 8 values in a token: k's, then v's
+  int head_shift;  // log2 of a head's
+  int lanes;       // threads on one token (at most ROW_THREADS), a multiple of 8
+  int along;       // tokens side by side in a CTA
+  int span;        // tokens of a CTA, at most ROW_SPAN
+};
+
+// The rows of `here` tokens from t0 of all sequences' (from start[b], or the sequence's length, on), as the index of their
+// first word of codes at kv head 0, -1 where there is none.
+__device__ __forceinline__ void find_rows(const we_kv4_cache& c, int64_t* rows, int64_t t0, uint32_t here, int64_t tokens,
+                                          const int32_t* start, int head_shift, uint32_t* err) {
+  if (threadIdx.x >= here) return;
+  const int64_t i = t0 + threadIdx.x, b = i >> 32 ? i / tokens : (uint32_t)i / (uint32_t)tokens;
+  const int64_t have = c.lengths[b], from = start ? (int64_t)start[b] : have;
+  const int64_t row = have < 0 || from < 0 ? -1 : kv4_row(c, b, from + (i - b * tokens), err);
+  rows[threadIdx.x] = row < 0 ? row : row << head_shift;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float rcp_approx(float x) {  // to 1 ulp
+  float d;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // keeps a NaN
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// The codes of 8 values, 8 lanes to a group of 64, and the group's scale: s = f16(max|x| / 7), q = rint(x / s) in -8..7.
+// The first division is by a constant: q + (a - 7 q) / 7 with q = a / 7 to a rounding is the rounded quotient (Markstein).
+// For the second, x (1 / s) added to 1.5 2^23 is rounded to an integer q, the quotient's own rounding unless |x - q s| is
+// within 2e-6 s of s / 2 (1 / s is to 2^-23, the quotient to 2^-24). Halves are common where few-bit values meet (one in 650
+// bf16 values): where x - q s is exactly s / 2, q goes to the even side. What is left takes the division (f32 values close
+// to a half), as do values that need the clamp: NaN, infinities, and groups whose s is not a normal f16 (in all others
+// |x / s| <= 7.01). The q + 8 of four values add up to 16 bits in f32.
+__device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], uint16_t* scale) {
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) top = max3(top, fabsf(x[j]), fabsf(x[j + 1]));
+#pragma unroll
+  for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  constexpr float SEVENTH = 1.f / 7.f, MAGIC = 12582912.f;
+  const float near = top * SEVENTH, want = fmaf(fmaf(-7.f, near, top), SEVENTH, near);
+  const __half s16 = __float2half_rn(fminf(want, 65504.f));
+  const float s = __half2float(s16), inv = rcp_approx(s);
+  *scale = __half_as_ushort(s16);
+  const float2 inv2 = make_float2(inv, inv), magic2 = make_float2(MAGIC, MAGIC), back2 = make_float2(-MAGIC, -MAGIC),
+               less2 = make_float2(-s, -s);
+  float far = 0.f;
+  float2 sum[2];  // of values 0..3 and 4..7, the even and the odd ones apart
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const float2 v = make_float2(x[2 * j], x[2 * j + 1]);
+    const float2 q = __fadd2_rn(__ffma2_rn(v, inv2, magic2), back2);
+    const float2 e = __ffma2_rn(q, less2, v);
+    far = max3_nan(far, fabsf(e.x), fabsf(e.y));
+    const float w = j & 1 ? 256.f : 1.f;  // 8 (1 + 16 + 256 + 4096) = 34952
+    sum[j / 2] = __ffma2_rn(q, make_float2(w, 16.f * w), j & 1 ? sum[j / 2] : make_float2(34952.f + 8388608.f, 0.f));
+  }
+  uint32_t word = __byte_perm(__float_as_uint(sum[0].x + sum[0].y), __float_as_uint(sum[1].x + sum[1].y), 0x5410);
+  if (!(far <= 0.499998f * s && s >= 6.104e-5f && want <= 65504.f)) {
+    if (s == 0.f) return 0;
+    bool rest = !(far <= s && s >= 6.104e-5f && want <= 65504.f);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float r = fmaf(x[j], inv, MAGIC), e = fmaf(__fadd_rn(r, -MAGIC), -s, x[j]), twice = 2.f * fabsf(e);
+      const uint32_t odd = (__float_as_uint(r) & 1u) << (4 * j);
+      if (twice == s) word += e < 0.f ? 0u - odd : odd;
+      else rest |= twice >= 0.999996f * s;
+    }
+    if (rest) {
+      word = 0x88888888u;
+#pragma unroll 1
+      for (int j = 0; j < 8; j++) {
+        float one = x[0];
+#pragma unroll
+        for (int e = 1; e < 8; e++) one = j == e ? x[e] : one;
+        word += (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(one, s)), -8.f), 7.f) << (4 * j);
+      }
+    }
+  }
+  return word ^ 0x88888888u;
+}
+
+template <int DT, bool WIDE>
+__global__ void __launch_bounds__(ROW_THREADS) kv4_append_kernel(const we_kv4_cache c, const void* __restrict__ k,
+                                                                 const void* __restrict__ v, int64_t tokens, int64_t stride,
+                                                                 const RowShape z, uint32_t* err) {
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int64_t groups = c.dim / 64, per_token = c.kv_heads * groups * 2, all = c.batch * tokens * per_token;
-  for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < all; u += (int64_t)gridDim.x * 8) {
-    const int64_t bt = u / per_token, b = bt / tokens, t = bt % tokens;
-    int64_t r = u % per_token;
-    const bool is_v = r >= c.kv_heads * groups;
-    if (is_v) r -= c.kv_heads * groups;
-    const int64_t h = r / groups, g = r % groups;
-    const int64_t have = c.lengths[b];
-    if (have < 0) continue;
-    const int64_t row = kv4_row(c, b, h, have + t, err);
-    if (row < 0) continue;
-    const int64_t at = bt * stride + h * c.dim + g * 64 + 2 * lane;
-    const void* src = is_v ? v : k;
-    const float x0 = load_act<DT>(src, at), x1 = load_act<DT>(src, at + 1);
-    const float top = warp_max(fmaxf(fabsf(x0), fabsf(x1)));
-    const __half s16 = __float2half_rn(fminf(__fdiv_rn(top, 7.f), 65504.f));
-    const float s = __half2float(s16);
-    int q0 = 0, q1 = 0;
-    if (s != 0.f) {
-      q0 = (int)fminf(fmaxf(rintf(__fdiv_rn(x0, s)), -8.f), 7.f);
-      q1 = (int)fminf(fmaxf(rintf(__fdiv_rn(x1, s)), -8.f), 7.f);
+  __shared__ int64_t rows[ROW_SPAN];
+  const int64_t all = c.batch * tokens;
+  const uint32_t slot = threadIdx.x / z.lanes, unit = threadIdx.x - slot * z.lanes;
+  for (int64_t t0 = (int64_t)blockIdx.x * z.span; t0 < all; t0 += (int64_t)gridDim.x * z.span) {
+    const uint32_t here = (uint32_t)(all - t0 < z.span ? all - t0 : z.span);
+    bool found = false;
+    for (uint32_t a = blockIdx.y * z.lanes + unit; a - unit < (uint32_t)z.units; a += gridDim.y * z.lanes) {
+      const bool mine = a < (uint32_t)z.units && slot < (uint32_t)z.along, is_v = a >= (uint32_t)z.units / 2;
+      const uint32_t at = is_v ? a - z.units / 2 : a, h = at >> z.head_shift, e = at - (h << z.head_shift);
+      const void* src = is_v ? v : k;
+      const int64_t head = ((int64_t)h * c.page << z.head_shift) + e;
+      uint32_t* codes = reinterpret_cast<uint32_t*>(is_v ? c.v : c.k) + head;
+      uint16_t* scales = (is_v ? c.v_scale : c.k_scale) + head / 8;
+      float x[8] = {};
+      auto load = [&](uint32_t t) {
+        if (!mine || t >= here) return;
+        const int64_t from = (t0 + t) * stride + (int64_t)at * 8;
+        if constexpr (WIDE) {
+          load8<DT>(src, from, x);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; j++) x[j] = load_act<DT>(src, from + j);
+        }
+      };
+      load(slot);  // (on its way during the look-up)
+      if (!found) {
+        __syncthreads();  // (rows of the tokens before are read)
+        find_rows(c, rows, t0, here, tokens, nullptr, z.head_shift, err);
+        __syncthreads();
+        found = true;
+      }
+      for (uint32_t t = slot; t - slot < here; t += z.along) {  // (all lanes together: the groups' maxima are shuffled)
+        uint16_t scale;
+        const uint32_t word = kv4_codes(x, &scale);
+        load(t + z.along);
+        const int64_t row = mine && t < here ? rows[t] : -1;
+        if (row >= 0) {
+          codes[row] = word;
+          if (e % 8 == 0) scales[(uint64_t)row / 8] = scale;
+        }
+      }
     }
-    (is_v ? c.v : c.k)[row * (c.dim / 2) + g * 32 + lane] = (uint8_t)((q0 & 15) | ((q1 & 15) << 4));
-    if (lane == 0) (is_v ? c.v_scale : c.k_scale)[row * groups + g] = __half_as_ushort(s16);
   }
 }
 
 template <int DT>
-__global__ void __launch_bounds__(256) kv4_unpack_kernel(const we_kv4_cache c, void* __restrict__ k, void* __restrict__ v,
-                                                         int64_t tokens, const int32_t* __restrict__ start,
-                                                         uint32_t* err) {
+__global__ void __launch_bounds__(ROW_THREADS) kv4_unpack_kernel(const we_kv4_cache c, void* __restrict__ k,
+                                                                 void* __restrict__ v, int64_t tokens,
+                                                                 const int32_t* __restrict__ start, const RowShape z,
+                                                                 uint32_t* err) {
   pdl_wait();
   pdl_launch_dependents();
-  // a thread: 8 values of one row, of k and of v
-  const int64_t per_row = c.dim / 8, all = c.batch * tokens * c.kv_heads * per_row;
-  for (int64_t u = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; u < all; u += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t bt = u / (c.kv_heads * per_row), b = bt / tokens, t = bt % tokens;
-    const int64_t h = u / per_row % c.kv_heads, e = u % per_row;
-    const int64_t have = c.lengths[b], from = start ? (int64_t)start[b] : have;
-    const int64_t row = have < 0 || from < 0 ? -1 : kv4_row(c, b, h, from + t, err);
+  __shared__ int64_t rows[ROW_SPAN];
+  const int64_t all = c.batch * tokens;
+  const uint32_t slot = threadIdx.x / z.lanes, unit = threadIdx.x - slot * z.lanes;
+  for (int64_t t0 = (int64_t)blockIdx.x * z.span; t0 < all; t0 += (int64_t)gridDim.x * z.span) {
+    const uint32_t here = (uint32_t)(all - t0 < z.span ? all - t0 : z.span);
+    __syncthreads();
+    find_rows(c, rows, t0, here, tokens, start, z.head_shift, err);
+    __syncthreads();
+    for (uint32_t a = blockIdx.y * z.lanes + unit; a < (uint32_t)z.units; a += gridDim.y * z.lanes) {
+      const bool is_v = a >= (uint32_t)z.units / 2;
+      const uint32_t at = is_v ? a - z.units / 2 : a, h = at >> z.head_shift, e = at - (h << z.head_shift);
+      void* out = is_v ? v : k;
+      if (!out || slot >= (uint32_t)z.along) continue;
+      const int64_t head = ((int64_t)h * c.page << z.head_shift) + e, to = t0 * z.units / 2 + at;
+      const uint32_t* codes = reinterpret_cast<const uint32_t*>(is_v ? c.v : c.k) + head;
+      const uint16_t* scales = (is_v ? c.v_scale : c.k_scale) + head / 8;
+#pragma unroll 4
+      for (uint32_t t = slot; t < here; t += z.along) {
+        const int64_t row = rows[t];
+        uint32_t word = 0x88888888u;
+        float s = 0.f;
+        if (row >= 0) {
+          word = codes[row] ^ 0x88888888u;
+          s = __half2float(__ushort_as_half(scales[(uint64_t)row / 8]));
+        }
+        float x[8];
 #pragma unroll
-    for (int side = 0; side < 2; side++) {
-      void* out = side ? v : k;
-      if (!out) continue;
-      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (row >= 0) {
-        const uint32_t word = *reinterpret_cast<const uint32_t*>((side ? c.v : c.k) + row * (c.dim / 2) + e * 4);
-        const float s = __half2float(__ushort_as_half((side ? c.v_scale : c.k_scale)[row * (c.dim / 64) + e / 8]));
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = (float)(int(((word >> (4 * j)) & 15u) ^ 8u) - 8) * s;
+        for (int j = 0; j < 8; j += 2) {  // q + 8 as the low bits of 2^23
+          const float2 u = make_float2(__uint_as_float(0x4b000000u | ((word >> (4 * j)) & 15u)),
+                                       __uint_as_float(0x4b000000u | ((word >> (4 * j + 4)) & 15u)));
+          const float2 y = __fmul2_rn(__fadd2_rn(u, make_float2(-8388616.f, -8388616.f)), make_float2(s, s));
+          x[j] = y.x;
+          x[j + 1] = y.y;
+        }
+        store8<DT>(out, (to + (int64_t)t * (z.units / 2)) * 8, x);
       }
-      store8<DT>(out, (bt * c.kv_heads + h) * c.dim + e * 8, x);
     }
   }
 }
@@ -655,24 +784,43 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
   merge_parts<D, QROWS, WARPS, CLUSTER>(mem, p.part, p.done, &last, unit, (int)gridDim.x / CLUSTER, runs, run, rank, finish);
 }
 
-static unsigned grid_of(int64_t work, int per_cta, int sms, int ctas_per_sm) {
-  const int64_t g = (work + per_cta - 1) / per_cta, cap = (int64_t)sms * ctas_per_sm;
-  return (unsigned)(g < cap ? g : cap);
+// How rows are cut: a token over as many threads as it has units, evenly over several rounds of at most ROW_THREADS (over
+// CTAs where there are few tokens); 8 tokens a thread where that leaves two CTAs an SM.
+struct RowPlan {
+  RowShape shape;
+  dim3 grid;
+  int threads;
+};
+static RowPlan kv4_rows(const we_kv4_cache& c, int64_t tokens, int sms) {
+  RowPlan p;
+  const int64_t units = 2 * c.kv_heads * (c.dim / 8), all = c.batch * tokens, rounds = (units + ROW_THREADS - 1) / ROW_THREADS;
+  p.shape.units = (int)units;
+  p.shape.head_shift = c.dim == 64 ? 3 : c.dim == 128 ? 4 : 5;
+  p.shape.lanes = (int)(((units + rounds - 1) / rounds + 7) / 8 * 8);
+  p.shape.along = (int)std::min<int64_t>({ROW_THREADS / p.shape.lanes, ROW_SPAN, std::max<int64_t>(1, all / (2 * sms))});
+  p.shape.span = (int)std::min<int64_t>(ROW_SPAN, p.shape.along * std::max<int64_t>(1, std::min<int64_t>(8, all / (2 * sms * p.shape.along))));
+  p.threads = (p.shape.lanes * p.shape.along + 31) / 32 * 32;
+  const int64_t x = std::min<int64_t>((all + p.shape.span - 1) / p.shape.span, 0x7fffffff);
+  p.grid = dim3((unsigned)x, (unsigned)rounds);
+  return p;
 }
 
 cudaError_t launch_kv4_append(const we_kv4_cache& c, const void* k, const void* v, int dt, int64_t tokens,
                               int64_t stride, uint32_t* err, int sms, cudaStream_t st) {
-  const unsigned grid = grid_of(c.batch * tokens * c.kv_heads * (c.dim / 64) * 2, 8, sms, 16);
-  const cudaError_t e = dt == WE_F32 ? launch_pdl(kv4_append_kernel<WE_F32>, dim3(grid), 256, 0, st, c, k, v, tokens, stride, err)
-                                     : launch_pdl(kv4_append_kernel<WE_BF16>, dim3(grid), 256, 0, st, c, k, v, tokens, stride, err);
+  const RowPlan p = kv4_rows(c, tokens, sms);
+  const int64_t es = dt == WE_F32 ? 4 : 2;
+  const bool wide = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | (uintptr_t)(stride * es)) & 15) == 0;
+  const auto kernel = dt == WE_F32 ? (wide ? kv4_append_kernel<WE_F32, true> : kv4_append_kernel<WE_F32, false>)
+                                   : (wide ? kv4_append_kernel<WE_BF16, true> : kv4_append_kernel<WE_BF16, false>);
+  const cudaError_t e = launch_pdl(kernel, p.grid, p.threads, 0, st, c, k, v, tokens, stride, p.shape, err);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
 cudaError_t launch_kv4_unpack(const we_kv4_cache& c, void* k, void* v, int dt, int64_t tokens, const int32_t* start,
                               uint32_t* err, int sms, cudaStream_t st) {
-  const unsigned grid = grid_of(c.batch * tokens * c.kv_heads * (c.dim / 8), 256, sms, 8);
-  const cudaError_t e = dt == WE_F32 ? launch_pdl(kv4_unpack_kernel<WE_F32>, dim3(grid), 256, 0, st, c, k, v, tokens, start, err)
-                                     : launch_pdl(kv4_unpack_kernel<WE_BF16>, dim3(grid), 256, 0, st, c, k, v, tokens, start, err);
+  const RowPlan p = kv4_rows(c, tokens, sms);
+  const auto kernel = dt == WE_F32 ? kv4_unpack_kernel<WE_F32> : kv4_unpack_kernel<WE_BF16>;
+  const cudaError_t e = launch_pdl(kernel, p.grid, p.threads, 0, st, c, k, v, tokens, start, p.shape, err);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
