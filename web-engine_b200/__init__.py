@@ -10,13 +10,14 @@ from .ops import (Linear, Mod, Rope, attention, cross_attention, k_split_for, li
 from . import kernels, kv4, parallel
 from .stream import Streamer
 from . import block as blocks
+from . import decoder
 from . import transformer
 from . import weights
 from . import sequence
 from . import comm
 
 __all__ = ["Graph", "Buffer", "Binding", "Linear", "Mod", "Rope", "linear", "linear_host", "norm", "no_mod", "rotate",
-           "qk_norm_rotate", "k_split_for", "matvec", "cross_attention", "kernels", "kv4", "blocks", "transformer", "parallel", "Streamer", "weights", "sequence", "comm", "build"]
+           "qk_norm_rotate", "k_split_for", "matvec", "cross_attention", "kernels", "kv4", "blocks", "decoder", "transformer", "parallel", "Streamer", "weights", "sequence", "comm", "build"]
 
 
 def build(verbose: bool = False) -> str:
