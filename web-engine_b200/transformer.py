@@ -310,6 +310,8 @@ def transformer(graph: Graph, w: TransformerWeights, cfg: StepConfig, inp, dtype
         raise ValueError("sequence parallelism runs one image on the bf16 path")
     if tp is not None and (B != 1 or dtype != "bf16" or sp is not None or captured is not None or streamed is not None):
         raise ValueError("tensor parallelism runs one image on the bf16 path, eagerly")
+    if captured is not None and (captured.key != (b0.height, b0.width, Lt, B, dtype) or captured.sp is not sp):
+        raise ValueError("the captured step is for another geometry, batch, dtype or sequence-parallel group")
     group = sp if sp is not None else tp
     r0, n = group.shard(T) if group is not None else (0, R)  # this rank's rows
     outs = velocity if isinstance(velocity, (list, tuple)) else [velocity] * B if velocity is not None else [None] * B
@@ -339,8 +341,6 @@ def transformer(graph: Graph, w: TransformerWeights, cfg: StepConfig, inp, dtype
         rope = ops.Rope(graph.buffer(np.tile(cos, B)), graph.buffer(np.tile(sin, B)), pairs, R)
 
     if captured is not None:
-        if captured.key != (b0.height, b0.width, Lt, B, dtype) or captured.sp is not sp:
-            raise ValueError("the captured step is for another geometry, batch, dtype or sequence-parallel group")
         x = captured.run(graph, x, tvec)  # graph-owned; the last layer reads it
     else:
         if streamed is not None and captured is not None:
