@@ -232,6 +232,9 @@ __global__ void __launch_bounds__(cross::THREADS) cross_tile_kernel(const cross:
 #pragma unroll
       for (int nq = 0; nq < NQ; nq++) s[nq][0] = s[nq][1] = s[nq][2] = s[nq][3] = 0.f;
       if constexpr (F32) {
+        // The tensor cores cut each sum's last bits off: a chain for the large products of even dims, one for the odd
+        // ones and one for the small products, added at the end.
+        float part[NQ][3][4] = {};
 #pragma unroll
         for (int x = 0; x < D / 16; x++) {
           const float4 k0 = *reinterpret_cast<const float4*>(kt + u * ROW + piece<true>(u, x * 4 + c, 0) * 16);
@@ -246,11 +249,16 @@ __global__ void __launch_bounds__(cross::THREADS) cross_tile_kernel(const cross:
 #pragma unroll
             for (int nq = 0; nq < NQ; nq++) {
               const uint4 t = q_terms[(nq * (D / 8) + x * 2 + h) * 32 + lane];
-              const uint32_t bt[4] = {t.x, t.y, t.z, t.w};
-              mma_3tf32(s[nq], ah, al, bt);
+              mma_tf32(part[nq][2], al, t.x, t.y);
+              mma_tf32(part[nq][2], ah, t.z, t.w);
+              mma_tf32(part[nq][h], ah, t.x, t.y);
             }
           }
         }
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[nq][e] = part[nq][2][e] + (part[nq][0][e] + part[nq][1][e]);
       } else {
         const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
@@ -305,32 +313,43 @@ __global__ void __launch_bounds__(cross::THREADS) cross_tile_kernel(const cross:
           l[nq][e & 1] += w[nq][e];
         }
       if constexpr (F32) {
+        uint32_t bt[2][NQ][4];  // keys 8 h ..: a lane's are 8 h + 2 c and the next
 #pragma unroll
-        for (int h = 0; h < 2; h++) {  // keys 8 h ..: a lane's are 8 h + 2 c and the next
-          uint32_t bt[NQ][4];
+        for (int h = 0; h < 2; h++)
 #pragma unroll
           for (int nq = 0; nq < NQ; nq++) {
             // the 8 x 8 weights turned, 16 bits at a time
             const uint32_t w0 = __float_as_uint(w[nq][2 * h]), w1 = __float_as_uint(w[nq][2 * h + 1]);
             const uint32_t lo = transposed(__byte_perm(w0, w1, 0x5410)), hi = transposed(__byte_perm(w0, w1, 0x7632));
-            split_tf32(__uint_as_float(__byte_perm(lo, hi, 0x5410)), bt[nq][0], bt[nq][2]);
-            split_tf32(__uint_as_float(__byte_perm(lo, hi, 0x7632)), bt[nq][1], bt[nq][3]);
+            split_tf32(__uint_as_float(__byte_perm(lo, hi, 0x5410)), bt[h][nq][0], bt[h][nq][2]);
+            split_tf32(__uint_as_float(__byte_perm(lo, hi, 0x7632)), bt[h][nq][1], bt[h][nq][3]);
           }
-          const int r0 = h * 8 + c * 2;
 #pragma unroll
-          for (int x = 0; x < D / 32; x++) {  // dims 32 x + 4 u .. + 3: rows u, u + 8 of two tiles
-            const float4 v0 = *reinterpret_cast<const float4*>(vt + r0 * ROW + piece<true>(r0, x * 8 + u, 1) * 16);
-            const float4 v1 = *reinterpret_cast<const float4*>(vt + (r0 + 1) * ROW + piece<true>(r0 + 1, x * 8 + u, 1) * 16);
+        for (int x = 0; x < D / 32; x++) {  // dims 32 x + 4 u .. + 3: rows u, u + 8 of two tiles
+          float4 v0[2], v1[2];
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
+          for (int h = 0; h < 2; h++) {
+            const int r0 = h * 8 + c * 2;
+            v0[h] = *reinterpret_cast<const float4*>(vt + r0 * ROW + piece<true>(r0, x * 8 + u, 1) * 16);
+            v1[h] = *reinterpret_cast<const float4*>(vt + (r0 + 1) * ROW + piece<true>(r0 + 1, x * 8 + u, 1) * 16);
+          }
+#pragma unroll
+          for (int t = 0; t < 2; t++) {
+            float part[NQ][4] = {};  // of the tile's keys, added in f32's own rounding
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
               uint32_t ah[4], al[4];
-              split_tf32(t ? v0.z : v0.x, ah[0], al[0]);
-              split_tf32(t ? v0.w : v0.y, ah[1], al[1]);
-              split_tf32(t ? v1.z : v1.x, ah[2], al[2]);
-              split_tf32(t ? v1.w : v1.y, ah[3], al[3]);
+              split_tf32(t ? v0[h].z : v0[h].x, ah[0], al[0]);
+              split_tf32(t ? v0[h].w : v0[h].y, ah[1], al[1]);
+              split_tf32(t ? v1[h].z : v1[h].x, ah[2], al[2]);
+              split_tf32(t ? v1[h].w : v1[h].y, ah[3], al[3]);
 #pragma unroll
-              for (int nq = 0; nq < NQ; nq++) mma_3tf32(o[nq][x * 2 + t], ah, al, bt[nq]);
+              for (int nq = 0; nq < NQ; nq++) mma_3tf32(part[nq], ah, al, bt[h][nq]);
             }
+#pragma unroll
+            for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) o[nq][x * 2 + t][e] += part[nq][e];
           }
         }
       } else {
