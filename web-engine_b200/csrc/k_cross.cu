@@ -103,41 +103,43 @@ __global__ void __launch_bounds__(cross::THREADS) cross_tile_kernel(const cross:
   uint8_t* ring = smem + QBYTES + warp * (DEPTH * STAGE);
   const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
   const uint8_t* mask = a.key_mask ? a.key_mask + (int64_t)b * a.tk : nullptr;
+  // f32: a side's place is filled again as soon as it is read, so that one stage a warp (three CTAs an SM; two stages leave
+  // one) keeps copies on their way: one token to 4096 keys of 8 x 12 heads of 128 158 -> 72 us. bf16 has room for two
+  // stages, the next one's copies queued before this one is waited for (3% faster there).
+  constexpr bool EARLY = F32;
+  static_assert(EARLY || DEPTH > 1, "");
   uint32_t seen[DEPTH];  // which of a stage's 16 keys are seen
-  auto copy = [&](int i, int st) {
-    uint32_t bits = 0;
+  auto copy = [&](int i, int st, int side) {  // k first: that also finds which keys are seen
     if (i < mine) {
       const int first = key0 + (warp + WARPS * i) * TILE;
-      const int key = first + lane;
-      bits = __ballot_sync(0xffffffffu, lane < TILE && key < key1 && (!mask || mask[key] != 0));
+      if (side == 0) {
+        const int key = first + lane;
+        seen[st] = __ballot_sync(0xffffffffu, lane < TILE && key < key1 && (!mask || mask[key] != 0));
+      }
       const int there = min(TILE, key1 - first);  // rows that exist
-      if (bits) {
+      if (seen[st]) {
+        const int64_t stride = side ? a.v_stride : a.k_stride;
+        const uint8_t* from = static_cast<const uint8_t*>(side ? a.v : a.k) + (((int64_t)b * a.tk + first) * stride + (int64_t)head * dim) * ES;
+        uint8_t* to = ring + st * STAGE + side * SIDE;
+        const uint32_t to_addr = ring_addr + st * STAGE + side * SIDE;
+        if (p.wide_kv) {
 #pragma unroll
-        for (int side = 0; side < 2; side++) {
-          const int64_t stride = side ? a.v_stride : a.k_stride;
-          const uint8_t* from = static_cast<const uint8_t*>(side ? a.v : a.k) + (((int64_t)b * a.tk + first) * stride + (int64_t)head * dim) * ES;
-          uint8_t* to = ring + st * STAGE + side * SIDE;
-          const uint32_t to_addr = ring_addr + st * STAGE + side * SIDE;
-          if (p.wide_kv) {
-#pragma unroll
-            for (int j = 0; j < SIDE / 512; j++) {
-              const int at = j * 32 + lane, r = at / (ROW / 16), ch = at % (ROW / 16);
-              if (r < there && ch * 16 < dim * ES)
-                cp_async16(to_addr + r * ROW + piece<F32>(r, ch, side) * 16, from + r * stride * ES + ch * 16);
-            }
-          } else {  // value by value
-            for (int at = lane; at < TILE * dim; at += 32) {
-              const int r = at / dim, e = at - r * dim;
-              if (r >= there) break;
-              uint8_t* dst = to + r * ROW + piece<F32>(r, e * ES / 16, side) * 16 + (e * ES) % 16;
-              if constexpr (F32) *reinterpret_cast<uint32_t*>(dst) = reinterpret_cast<const uint32_t*>(from)[r * stride + e];
-              else *reinterpret_cast<uint16_t*>(dst) = reinterpret_cast<const uint16_t*>(from)[r * stride + e];
-            }
+          for (int j = 0; j < SIDE / 512; j++) {
+            const int at = j * 32 + lane, r = at / (ROW / 16), ch = at % (ROW / 16);
+            if (r < there && ch * 16 < dim * ES)
+              cp_async16(to_addr + r * ROW + piece<F32>(r, ch, side) * 16, from + r * stride * ES + ch * 16);
+          }
+        } else {  // value by value
+          for (int at = lane; at < TILE * dim; at += 32) {
+            const int r = at / dim, e = at - r * dim;
+            if (r >= there) break;
+            uint8_t* dst = to + r * ROW + piece<F32>(r, e * ES / 16, side) * 16 + (e * ES) % 16;
+            if constexpr (F32) *reinterpret_cast<uint32_t*>(dst) = reinterpret_cast<const uint32_t*>(from)[r * stride + e];
+            else *reinterpret_cast<uint16_t*>(dst) = reinterpret_cast<const uint16_t*>(from)[r * stride + e];
           }
         }
       }
     }
-    seen[st] = bits;
     cp_async_commit();
   };
   if (dim < D) {  // the places past dim stay zero
@@ -146,7 +148,10 @@ __global__ void __launch_bounds__(cross::THREADS) cross_tile_kernel(const cross:
     __syncthreads();
   }
 #pragma unroll
-  for (int d = 0; d < DEPTH - 1; d++) copy(d, d);
+  for (int d = 0; d < (EARLY ? DEPTH : DEPTH - 1); d++) {
+    copy(d, d, 0);
+    copy(d, d, 1);
+  }
 
   // q as the B operand: column lane / 4 of tile nq is row nq * 8 + lane / 4
   auto q_row = [&](int nq) -> int64_t {
@@ -211,22 +216,22 @@ __global__ void __launch_bounds__(cross::THREADS) cross_tile_kernel(const cross:
     for (int st = 0; st < DEPTH; st++) {
       const int i = i0 + st;
       if (i >= mine) break;
-      if (DEPTH > 1) copy(i + DEPTH - 1, (st + DEPTH - 1) % DEPTH);
-      else copy(i, 0);
-      cp_async_wait<DEPTH - 1>();
+      if constexpr (!EARLY) {
+        copy(i + DEPTH - 1, (st + DEPTH - 1) % DEPTH, 0);
+        copy(i + DEPTH - 1, (st + DEPTH - 1) % DEPTH, 1);
+      }
+      cp_async_wait<EARLY ? 2 * DEPTH - 1 : 2 * DEPTH - 2>();
       __syncwarp();
       const uint32_t bits = seen[st];
-      if (bits == 0) continue;  // (uniform) no key of the tile is seen
+      if (bits == 0) {  // (uniform) no key of the tile is seen
+        if constexpr (EARLY) {
+          copy(i + DEPTH, st, 0);
+          copy(i + DEPTH, st, 1);
+        }
+        continue;
+      }
       const uint8_t *kt = ring + st * STAGE, *vt = kt + SIDE;
       const uint32_t k_addr = ring_addr + st * STAGE, v_addr = k_addr + SIDE;
-      if (bits != 0xffffu) {  // hidden rows of v become zeros
-#pragma unroll
-        for (int j = 0; j < SIDE / 512; j++) {
-          const int at = j * 32 + lane;
-          if (!((bits >> (at / (ROW / 16))) & 1)) reinterpret_cast<uint4*>(ring + st * STAGE + SIDE)[at] = make_uint4(0, 0, 0, 0);
-        }
-        __syncwarp();
-      }
       // S^T: row u of the tile is key u, and key u + 8
       float s[NQ][4];
 #pragma unroll
@@ -276,6 +281,10 @@ __global__ void __launch_bounds__(cross::THREADS) cross_tile_kernel(const cross:
           for (int e = 0; e < 4; e++)
             if (!((bits >> (u + (e >> 1) * 8)) & 1)) s[nq][e] = -INFINITY;
       }
+      if constexpr (EARLY) {
+        __syncwarp();
+        copy(i + DEPTH, st, 0);
+      }
       bool grow = false;
 #pragma unroll
       for (int nq = 0; nq < NQ; nq++)
@@ -312,6 +321,18 @@ __global__ void __launch_bounds__(cross::THREADS) cross_tile_kernel(const cross:
           w[nq][e] = ex2_ftz(fmaf(s[nq][e], p.scale_log2, -m[nq][e & 1]));
           l[nq][e & 1] += w[nq][e];
         }
+      if constexpr (EARLY) {
+        cp_async_wait<2 * DEPTH - 1>();
+        __syncwarp();
+      }
+      if (bits != 0xffffu) {  // hidden rows of v become zeros
+#pragma unroll
+        for (int j = 0; j < SIDE / 512; j++) {
+          const int at = j * 32 + lane;
+          if (!((bits >> (at / (ROW / 16))) & 1)) reinterpret_cast<uint4*>(ring + st * STAGE + SIDE)[at] = make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+      }
       if constexpr (F32) {
         uint32_t bt[2][NQ][4];  // keys 8 h ..: a lane's are 8 h + 2 c and the next
 #pragma unroll
@@ -368,6 +389,7 @@ __global__ void __launch_bounds__(cross::THREADS) cross_tile_kernel(const cross:
         }
       }
       __syncwarp();  // every lane has read the stage that is copied into next
+      if constexpr (EARLY) copy(i + DEPTH, st, 1);
     }
   }
 
@@ -431,7 +453,7 @@ CrossPlan cross_plan(const we_cross_desc& d, int sms) {
   q.row_tiles = (int)((rows + 8 * q.nq - 1) / (8 * q.nq));
   q.units = d.batch * d.kv_heads * q.row_tiles;
   // about one wave of runs (as the cached attention's plan), by the CTAs that fit an SM's shared memory
-  const int per_sm = f32 ? (q.dim == 64 ? 3 : 1) : (q.dim == 64 ? 4 : q.dim == 128 ? 3 : 1);
+  const int per_sm = f32 ? (q.dim == 64 ? 4 : q.dim == 128 ? 3 : 1) : (q.dim == 64 ? 4 : q.dim == 128 ? 3 : 1);
   const int64_t slots = (int64_t)sms * per_sm - 8 * per_sm, tk = std::max<int64_t>(1, d.tk);
   // where the row tiles alone fill the SMs, a CTA takes all keys of its rows
   q.cluster = q.nq == 2 && q.units >= slots ? 1 : 8;
@@ -499,8 +521,8 @@ cudaError_t launch_cross_tile(const we_cross_desc& d, void* part, uint32_t* done
       : q.nq == 1    ? cross_tile<F32, D, 1, DEPTH, 8>(p, grid, st)        \
                      : cross_tile<F32, D, 2, DEPTH, 8>(p, grid, st)
   if (f32) {
-    if (q.dim == 64) CROSS_CASE(true, 64, 2);
-    else if (q.dim == 128) CROSS_CASE(true, 128, 2);
+    if (q.dim == 64) CROSS_CASE(true, 64, 1);
+    else if (q.dim == 128) CROSS_CASE(true, 128, 1);
     else CROSS_CASE(true, 256, 1);
   } else {
     if (q.dim == 64) CROSS_CASE(false, 64, 2);
