@@ -192,6 +192,35 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
       }
     }
   };
+  // x: units of 16 values (half of a lane's share of a chunk), four neighbouring lanes a group: scaled, and as f16 pairs
+  // (v, v + 4) in the order of the codes, with the sum of each group. A thread's first unit is asked for before the weights
+  // (behind them it arrives some 2 us later), the next ones while one is worked on.
+  const int units_row = chunks * CHUNK / 16, units = m * units_row;
+  const char* src = static_cast<const char*>(x) + (int64_t)g0 * 64 * XB;
+  const bool wide = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)(a.x_stride * XB)) & 15) == 0;
+  uint32_t ahead[4 * XB];  // the values as they are
+  auto load_x = [&](int u) {
+#pragma unroll
+    for (int j = 0; j < 4 * XB; j++) ahead[j] = 0;
+    const int i = u / units_row, e = u - i * units_row;
+    if (u >= units || e * 16 >= my_groups * 64) return;
+    const char* from = src + ((int64_t)i * a.x_stride + e * 16) * XB;
+    if (wide) {
+#pragma unroll
+      for (int j = 0; j < XB; j++) {
+        const uint4 q = reinterpret_cast<const uint4*>(from)[j];
+        ahead[4 * j] = q.x, ahead[4 * j + 1] = q.y, ahead[4 * j + 2] = q.z, ahead[4 * j + 3] = q.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4 * XB; j++) {
+        if constexpr (XB == 4) ahead[j] = reinterpret_cast<const uint32_t*>(from)[j];
+        else ahead[j] = reinterpret_cast<const uint16_t*>(from)[2 * j] |
+                        (uint32_t)reinterpret_cast<const uint16_t*>(from)[2 * j + 1] << 16;
+      }
+    }
+  };
+  if (units > 0) load_x(threadIdx.x);
 #pragma unroll
   for (int d = 0; d < DEPTH; d++) {
 #pragma unroll
@@ -200,34 +229,13 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
   }
   for (int u = threadIdx.x; u < NOTHING / 16; u += THREADS) reinterpret_cast<uint4*>(smem)[u] = make_uint4(0, 0, 0, 0);
 
-  // x: units of 16 values (half of a lane's share of a chunk), four neighbouring lanes a group: scaled, and as f16 pairs
-  // (v, v + 4) in the order of the codes, with the sum of each group.
-  const int units_row = chunks * CHUNK / 16, units = m * units_row;
-  const char* src = static_cast<const char*>(x) + (int64_t)g0 * 64 * XB;
-  const bool wide = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)(a.x_stride * XB)) & 15) == 0;
   for (int u0 = 0; u0 < units; u0 += THREADS) {
     const int u = u0 + threadIdx.x;
     const int i = min(u / units_row, m - 1), e = u - i * units_row;
-    uint32_t t[4 * XB];  // the values as they are
+    uint32_t t[4 * XB];
 #pragma unroll
-    for (int j = 0; j < 4 * XB; j++) t[j] = 0;
-    if (u < units && e * 16 < my_groups * 64) {
-      const char* from = src + ((int64_t)i * a.x_stride + e * 16) * XB;
-      if (wide) {
-#pragma unroll
-        for (int j = 0; j < XB; j++) {
-          const uint4 q = reinterpret_cast<const uint4*>(from)[j];
-          t[4 * j] = q.x, t[4 * j + 1] = q.y, t[4 * j + 2] = q.z, t[4 * j + 3] = q.w;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4 * XB; j++) {
-          if constexpr (XB == 4) t[j] = reinterpret_cast<const uint32_t*>(from)[j];
-          else t[j] = reinterpret_cast<const uint16_t*>(from)[2 * j] |
-                      (uint32_t)reinterpret_cast<const uint16_t*>(from)[2 * j + 1] << 16;
-        }
-      }
-    }
+    for (int j = 0; j < 4 * XB; j++) t[j] = ahead[j];
+    if (u0 + THREADS < units) load_x(u + THREADS);
     uint32_t top = 0;  // the largest magnitude's bits (bf16: of the halves, then as f32)
 #pragma unroll
     for (int j = 0; j < 4 * XB; j++) top = XB == 4 ? max(top, t[j] & 0x7fffffffu) : __vmaxu2(top, t[j] & 0x7fff7fffu);
@@ -389,13 +397,16 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
     }
   __syncthreads();
   const int outs = cta_rows * m;
+  const int row_shift = 31 - __clz(cta_rows);
   for (int u = threadIdx.x; u < outs; u += THREADS) {
-    const int i = u / cta_rows, row = u - i * cta_rows;
+    const int i = u >> row_shift, row = u - (i << row_shift);
     const float* from = red + (row / ROWS * p.wk * ROWS + row % ROWS) * TOKS + i;
     float v = 0.f;
 #pragma unroll
     for (int c = PIECES - 1; c >= 0; c--)
-      for (int k = 0; k < p.wk; k++) v += from[k * (ROWS * TOKS) + c * m];
+#pragma unroll
+      for (int k = 0; k < WARPS; k++)
+        if (k < p.wk) v += from[k * (ROWS * TOKS) + c * m];
     if (p.cluster > 1) part[u] = v;
     else if (first + row < n) matvec_store(v, a, i, first + row, y);
   }
@@ -403,14 +414,13 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
     tc::cluster_sync_all();
     const uint32_t part_addr = tc::smem_u32(part);
     for (int u = rank * THREADS + threadIdx.x; u < outs; u += p.cluster * THREADS) {
-      const int i = u / cta_rows, channel = first + u - i * cta_rows;
+      const int i = u >> row_shift, channel = first + u - (i << row_shift);
       if (channel >= n) continue;
-      float v = 0.f;
-      for (int s = 0; s < p.cluster; s++) {
-        float o;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(tc::map_rank(part_addr + 4u * u, s)));
-        v += o;
-      }
+      float o[MAX_CLUSTER], v = 0.f;
+#pragma unroll
+      for (int s = 0; s < MAX_CLUSTER; s++) o[s] = s < p.cluster ? tc::ld_cluster_f32(tc::map_rank(part_addr + 4u * u, s)) : 0.f;
+#pragma unroll
+      for (int s = 0; s < MAX_CLUSTER; s++) v += o[s];
       matvec_store(v, a, i, channel, y);
     }
     tc::cluster_sync_all();  // no CTA leaves while another reads its part
