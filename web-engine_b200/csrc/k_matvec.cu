@@ -458,22 +458,25 @@ cudaError_t launch_matvec(const void* x, const void* wv, void* y, const MatmulAr
   const int64_t chunks = (a.k + CHUNK - 1) / CHUNK, tiles = (a.n + rt * 16 - 1) / (rt * 16);
   // How k is split over clusters and warps: the shortest chain of instructions of an SM's warp slot (its share of x's
   // layout, its steps, its sums and the cluster's, for as many waves of CTAs as it takes).
+  // ROOM: CTAs that 148 SMs hold at a time, 1 or 2 an SM, in clusters of 1 to 8 (cudaOccupancyMaxActiveClusters; a cluster
+  // stays within a GPC). Of the splits of nine shapes, all of them timed, this picks the fastest or one within 5% of it: 8
+  // tokens of 16384 values to 6144 channels take 26.8 us with clusters of 5 and 28.9 with the best power of two.
+  static constexpr int ROOM[2][MAX_CLUSTER] = {{148, 148, 135, 132, 130, 132, 105, 120}, {296, 296, 279, 284, 280, 270, 259, 264}};
   Plan p{};
   int64_t best = -1;
-  for (int cluster = 1; cluster <= MAX_CLUSTER; cluster *= 2)
+  for (int cluster = 1; cluster <= MAX_CLUSTER; cluster++)
     for (int wk = 1; wk <= WARPS; wk *= 2) {
       const int64_t per_cta = (chunks + cluster - 1) / cluster;
-      const int64_t depth = IN_FLIGHT / rt, blocks = (per_cta + depth - 1) / depth;
-      if (wk > 1 && wk > blocks) break;
+      if (wk > 1 && wk > per_cta) break;
       const int64_t rows = WARPS / wk * rt * 16, ctas = (tiles * wk + WARPS - 1) / WARPS * cluster;
-      const int64_t waves = (ctas + sms * per_sm - 1) / (sms * per_sm);
+      const int64_t slots = std::max<int64_t>(1, (int64_t)sms * ROOM[per_sm - 1][cluster - 1] / 148), waves = (ctas + slots - 1) / slots;
       const int64_t bytes = NOTHING + toks * per_cta * CHUNK * 2 +
                             (per_cta * nt * 16 + WARPS * rt * 16 * nt * 4 + (cluster > 1 ? rows * a.m : 0)) * 4;
       if (bytes > 226 * 1024 / per_sm) continue;
       const int64_t units = (a.m * per_cta * 8 + THREADS - 1) / THREADS, outs = (rows * a.m + THREADS - 1) / THREADS;
-      const int64_t cost = waves * (300 + units * (f32 ? 250 : 110) + (blocks + wk - 1) / wk * depth * rt * (70 + 20 * nt) +
+      const int64_t cost = waves * (300 + units * (f32 ? 250 : 110) + (per_cta + wk - 1) / wk * rt * (70 + 20 * nt) +
                                     outs * (30 + 4 * wk) + (cluster > 1 ? 300 : 0));
-      if (best >= 0 && cost >= best) continue;
+      if (best >= 0 && cost > best) continue;
       best = cost;
       p = Plan{wk, cluster, (int)per_cta, (int)per_cta * CHUNK * 2, (int)bytes};
     }
