@@ -218,3 +218,33 @@ def test_matvec_refusals(we, graph):
         we.matvec(graph, b, we.Linear(b, "fp8", 1.0, 8, 64), 1)
     K.matvec(graph, b, b, b, 1, 0, 64, group_scale=b)  # no channels: nothing to do
     assert graph.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("m,n,k", [(16, 37, 28736), (16, 21, 40000), (16, 19, 60032), (3, 9, 300032)])
+def test_matvec_long_rows(we, graph, m, n, k, dtype):
+    """x that leaves room for one block an SM, for a whole SM's shared memory, and (the last two, but for three bf16 rows) that does not fit 8 SMs':
+    there a lane sums k / 32 products in turn, each rounded, and 32 lanes join in 5 more additions."""
+    packed, s, w = weights(n, k, n + k)
+    x = randn(m * k, m).reshape(m, k)
+    if dtype == "bf16":
+        x = bf16_round(x).reshape(m, k)
+    x = x.astype(np.float64)
+    want = x @ w.T
+    got = product(we, graph, x.astype(np.float32), packed, s, m, n, k, dtype, dtype)
+    slack = (k / 32 + 84) * 2.0**-24 * (np.abs(x) @ np.abs(w).T) + (2.0**-8 * np.abs(want) if dtype == "bf16" else 0)
+    assert np.all(np.abs(got - want) <= slack)
+
+
+def test_matvec_non_finite_rows(we, graph):
+    """A row of x that holds a NaN or an infinity is NaN; the rows beside it are what they are without it."""
+    m, n, k = 4, 40, 320
+    packed, s, w = weights(n, k, 9)
+    for dtype in ("bf16", "f32"):
+        x = bf16_round(randn(m * k, 10)).reshape(m, k)
+        clean = product(we, graph, x, packed, s, m, n, k, dtype, "f32")
+        bad = x.copy()
+        bad[1, 77], bad[3, 319] = np.nan, np.inf
+        got = product(we, graph, bad, packed, s, m, n, k, dtype, "f32")
+        assert np.all(np.isnan(got[[1, 3]]))
+        assert np.array_equal(got[[0, 2]], clean[[0, 2]])

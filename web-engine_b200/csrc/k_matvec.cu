@@ -53,7 +53,7 @@ __device__ __forceinline__ void matvec_store(float v, const MatmulArgs& a, int64
 }
 
 // ---------------- any k: one warp per output channel on the CUDA cores ----------------
-// For x that does not fit the shared memory of 8 CTAs (about 1.1 MB). A lane takes 8 values (4 packed bytes) of every 256.
+// For x that does not fit the shared memory of 8 CTAs (about 1.8 MB as f16: 53000 values of 16 tokens). A lane takes 8 values (4 packed bytes) of every 256.
 template <int XT>
 __global__ void __launch_bounds__(256) matvec_long_kernel(const void* __restrict__ x, const uint8_t* __restrict__ w,
                                                           void* y, const MatmulArgs a) {
@@ -464,22 +464,24 @@ cudaError_t launch_matvec(const void* x, const void* wv, void* y, const MatmulAr
   static constexpr int ROOM[2][MAX_CLUSTER] = {{148, 148, 135, 132, 130, 132, 105, 120}, {296, 296, 279, 284, 280, 270, 259, 264}};
   Plan p{};
   int64_t best = -1;
-  for (int cluster = 1; cluster <= MAX_CLUSTER; cluster++)
-    for (int wk = 1; wk <= WARPS; wk *= 2) {
-      const int64_t per_cta = (chunks + cluster - 1) / cluster;
-      if (wk > 1 && wk > per_cta) break;
-      const int64_t rows = WARPS / wk * rt * 16, ctas = (tiles * wk + WARPS - 1) / WARPS * cluster;
-      const int64_t slots = std::max<int64_t>(1, (int64_t)sms * ROOM[per_sm - 1][cluster - 1] / 148), waves = (ctas + slots - 1) / slots;
-      const int64_t bytes = NOTHING + toks * per_cta * CHUNK * 2 +
-                            (per_cta * nt * 16 + WARPS * rt * 16 * nt * 4 + (cluster > 1 ? rows * a.m : 0)) * 4;
-      if (bytes > 226 * 1024 / per_sm) continue;
-      const int64_t units = (a.m * per_cta * 8 + THREADS - 1) / THREADS, outs = (rows * a.m + THREADS - 1) / THREADS;
-      const int64_t cost = waves * (300 + units * (f32 ? 250 : 110) + (per_cta + wk - 1) / wk * rt * (70 + 20 * nt) +
-                                    outs * (30 + 4 * wk) + (cluster > 1 ? 300 : 0));
-      if (best >= 0 && cost > best) continue;
-      best = cost;
-      p = Plan{wk, cluster, (int)per_cta, (int)per_cta * CHUNK * 2, (int)bytes};
-    }
+  // (x that does not leave room for two CTAs an SM has one)
+  for (int fit = per_sm; fit >= 1 && best < 0; fit--)
+    for (int cluster = 1; cluster <= MAX_CLUSTER; cluster++)
+      for (int wk = 1; wk <= WARPS; wk *= 2) {
+        const int64_t per_cta = (chunks + cluster - 1) / cluster;
+        if (wk > 1 && wk > per_cta) break;
+        const int64_t rows = WARPS / wk * rt * 16, ctas = (tiles * wk + WARPS - 1) / WARPS * cluster;
+        const int64_t slots = std::max<int64_t>(1, (int64_t)sms * ROOM[fit - 1][cluster - 1] / 148), waves = (ctas + slots - 1) / slots;
+        const int64_t bytes = NOTHING + toks * per_cta * CHUNK * 2 +
+                              (per_cta * nt * 16 + WARPS * rt * 16 * nt * 4 + (cluster > 1 ? rows * a.m : 0)) * 4;
+        if (bytes > 226 * 1024 / fit) continue;
+        const int64_t units = (a.m * per_cta * 8 + THREADS - 1) / THREADS, outs = (rows * a.m + THREADS - 1) / THREADS;
+        const int64_t cost = waves * (300 + units * (f32 ? 250 : 110) + (per_cta + wk - 1) / wk * rt * (70 + 20 * nt) +
+                                      outs * (30 + 4 * wk) + (cluster > 1 ? 300 : 0));
+        if (best >= 0 && cost > best) continue;
+        best = cost;
+        p = Plan{wk, cluster, (int)per_cta, (int)per_cta * CHUNK * 2, (int)bytes};
+      }
   const bool ok = best >= 0;
   const int64_t cta_rows = ok ? WARPS / p.wk * rt * 16 : 1, gy = (a.n + cta_rows - 1) / cta_rows;
   if (!ok || gy > 65535) {
