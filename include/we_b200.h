@@ -374,10 +374,11 @@ int we_attend(we_ctx* ctx, const void* q, const void* k, const void* v, int32_t 
 /* ---------------- single tokens: products with 4-bit weights (no reference counterpart) ----------------
    we_matmul for few rows: the same descriptor with w_dtype = WE_INT4G64 and 1 <= m <= WE_MATVEC_MAX_ROWS (a decoder's
    tokens of one step). y[i, n] = sum over groups g of s[n, g] sum over j in g of q[n, j] x[i, j], every product exact
-   and every sum in f32 (we_matmul rounds q s to bf16 first), then bias and the fused epilogue as we_matmul applies
-   them. x and y f32 or bf16 with row strides and offsets in values; w contiguous [n, k / 2] and 16-byte aligned, f16
-   group scales [n, k / 64], k a multiple of 64; scale, chan_scale and k_split do not apply (scale is ignored, the
-   others are refused). flags: WE_MM_ACCUMULATE. */
+   (f32 x: to 2^-22; we_matmul rounds q s to bf16 first) and every sum in f32, then bias and the fused epilogue as
+   we_matmul applies them. x and y f32 or bf16 with row strides and offsets in values; w contiguous [n, k / 2] and
+   16-byte aligned, f16 group scales [n, k / 64], k a multiple of 64; scale, chan_scale and k_split do not apply (scale is
+   ignored, the others are refused). flags: WE_MM_ACCUMULATE. Within a group of 64 values of a row, bits below 2^-36 of
+   the largest are lost; a row that holds a NaN or an infinity gives NaN. */
 #define WE_MATVEC_MAX_ROWS 16
 int we_matvec(we_ctx* ctx, const we_matmul_desc* desc, const void* x, const void* w, void* y);
 
