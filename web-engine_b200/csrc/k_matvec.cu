@@ -90,8 +90,9 @@ namespace mv {
 constexpr int WARPS = 8, THREADS = WARPS * 32;
 constexpr int CHUNK = 128;       // values of k of a step: 64 packed bytes of each channel
 constexpr int MAX_CLUSTER = 8;
-constexpr int IN_FLIGHT = 4;  // row tiles x steps that a warp loads ahead (1 KB each)
-constexpr int NOTHING = IN_FLIGHT * 256; // bytes of zeros that lanes without a token read
+constexpr int STEP = 2;          // chunks of a step: 128 bytes of each channel
+constexpr int AHEAD = 2;         // steps that a warp loads ahead
+constexpr int NOTHING = AHEAD * STEP * 256 + 128;  // bytes of zeros that lanes without a token read, on the banks that the others do not
 
 struct Plan {
   int wk;           // warps of a CTA that split k (a power of two); the others take further channels
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
                                                                  void* y, const MatmulArgs a, const mv::Plan p) {
   using namespace mv;
   constexpr int XB = XT == WE_F32 ? 4 : 2, PIECES = XT == WE_F32 ? 2 : 1;
-  constexpr int TOKS = NT * 4, ROWS = RT * 16, DEPTH = IN_FLIGHT / RT, CHAINS = NT * RT <= 2 ? 2 : 1;
+  constexpr int TOKS = NT * 4, ROWS = RT * 16, CHAINS = NT * RT <= 2 ? 2 : 1;
   extern __shared__ __align__(16) uint8_t smem[];
   const int m = (int)a.m, n = (int)a.n, toks = m * PIECES;
   const int groups = (int)(a.k / 64);
@@ -164,32 +165,50 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
   pdl_launch_dependents();
   pdl_wait();
 
-  // A step's weights and scales: of channels lane / 4 and + 8 of each row tile, the values 32 (lane % 4) and on of the
-  // chunk. Past the last channel the last one is read again (not stored); a lane whose group of the last chunk does not
-  // exist reads nothing there (its x is zero).
-  uint4 wq[DEPTH][2 * RT];
-  uint32_t sc[DEPTH][2 * RT];
-  const uint8_t* wp[2 * RT];
-  const uint16_t* sp[2 * RT];
+  // A step's weights: a lane loads 16 bytes of channels lane / 8 + 0, 4, 8 and 12 of each row tile, eight lanes 128 bytes
+  // of one (a load touches four lines; with 64 bytes of eight channels the load path took 14.4 us for 50 MB). Lanes 4 apart
+  // then exchange half of it, and hold 64 bytes of both chunks of channels `channel` and + 8 between four of them.
+  // Scales: lane c of the four loads the two of every fourth chunk. Past the last channel the last one is read again (not
+  // stored); a lane whose group of the last chunk does not exist reads nothing there (its x is zero).
+  const int channel = (lane >> 3) | (lane & 4), top_row = first + warp / p.wk * ROWS;
+  uint4 raw[AHEAD][RT][4];
+  uint32_t sc[RT][2], sc_next[RT][2];  // of channels `channel` and + 8
+  const uint8_t* wp[RT];
+  const uint16_t* sp[RT];
+  int w_off[RT][4], s_off[RT];
 #pragma unroll
-  for (int j = 0; j < 2 * RT; j++) {
-    const int64_t at = (int64_t)min(first + warp / p.wk * ROWS + j * 8 + (lane >> 2), n - 1) * groups + g0 + 2 * ch0;
-    wp[j] = w + at * 32 + (lane & 3) * 16;
-    sp[j] = a.group_scale + at;
+  for (int r = 0; r < RT; r++) {
+    const int at = min(top_row + r * 16 + (lane >> 3), n - 1), of = min(top_row + r * 16 + channel, n - 1);
+    wp[r] = w + ((int64_t)at * groups + g0 + 2 * ch0) * 32 + (lane & 7) * 16;
+    sp[r] = a.group_scale + (int64_t)of * groups + g0 + 2 * ch0 + (lane & 3) * 2;
+#pragma unroll
+    for (int i = 0; i < 4; i++) w_off[r][i] = (min(top_row + r * 16 + (lane >> 3) + 4 * i, n - 1) - at) * groups * 32;
+    s_off[r] = (min(top_row + r * 16 + channel + 8, n - 1) - of) * groups;
   }
   const bool pairs = (groups & 1) == 0 && (reinterpret_cast<uintptr_t>(a.group_scale) & 3) == 0;  // scales two at a time
-  // up to which chunk there are this lane's group, and two groups
-  const int lane_end = min(end, (my_groups - ((lane >> 1) & 1) + 1) / 2), two_end = min(end, my_groups / 2);
-  auto fetch = [&](int st, int c) {  // chunk c + st, where the pointers stand at chunk c
+  // up to which chunk there are this lane's group (of its half of a step), and two groups
+  const int lane_end = min(end, (my_groups - ((lane >> 1) & 1) + 1) / 2) - ((lane >> 2) & 1), two_end = min(end, my_groups / 2);
+  auto fetch = [&](int d, int r, int c) {  // the step from chunk c on, where the pointers stand
+    if (c < lane_end)
 #pragma unroll
-    for (int j = 0; j < 2 * RT; j++) {
-      if (c + st < lane_end) wq[st][j] = load_once16(wp[j] + st * 64);
-      if (pairs) {
-        if (c + st < end) sc[st][j] = __ldg(reinterpret_cast<const uint32_t*>(sp[j] + 2 * st));
-      } else {
-        if (c + st < end) sc[st][j] = __ldg(sp[j] + 2 * st);
-        if (c + st < two_end) sc[st][j] |= (uint32_t)__ldg(sp[j] + 2 * st + 1) << 16;
+      for (int i = 0; i < 4; i++) raw[d][r][i] = load_once16(wp[r] + w_off[r][i]);
+    wp[r] += STEP * 64;
+  };
+  auto fetch_scales = [&](int c) {  // of chunks c .. c + 3
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+      const int mine = c + (lane & 3);
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const uint16_t* from = sp[r] + (h ? s_off[r] : 0);
+        if (pairs) {
+          if (mine < end) sc_next[r][h] = __ldg(reinterpret_cast<const uint32_t*>(from));
+        } else {
+          if (mine < end) sc_next[r][h] = __ldg(from);
+          if (mine < two_end) sc_next[r][h] |= (uint32_t)__ldg(from + 1) << 16;
+        }
       }
+      sp[r] += 8;
     }
   };
   // x: units of 16 values (half of a lane's share of a chunk), four neighbouring lanes a group: scaled, and as f16 pairs
@@ -222,10 +241,16 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
   };
   if (units > 0) load_x(threadIdx.x);
 #pragma unroll
-  for (int d = 0; d < DEPTH; d++) {
+  for (int r = 0; r < RT; r++) sc[r][0] = sc[r][1] = sc_next[r][0] = sc_next[r][1] = 0;
 #pragma unroll
-    for (int j = 0; j < 2 * RT; j++) wq[d][j] = make_uint4(0, 0, 0, 0), sc[d][j] = 0;
-    fetch(d, ch0);
+  for (int d = 0; d < AHEAD; d++) {
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) raw[d][r][i] = make_uint4(0, 0, 0, 0);
+      fetch(d, r, ch0 + d * STEP);
+    }
+    if (d == 0) fetch_scales(ch0);
   }
   for (int u = threadIdx.x; u < NOTHING / 16; u += THREADS) reinterpret_cast<uint4*>(smem)[u] = make_uint4(0, 0, 0, 0);
 
@@ -316,25 +341,48 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
   for (int t = 0; t < NT; t++) {
     const int tok = t * 4 + (lane >> 3);
     const bool some = ((lane >> 2) & 1) == ((lane >> 1) & 1) && tok < toks;
-    bp[t] = some ? xs + tok * p.x_pitch + ch0 * 256 + (lane & 3) * 16 : smem;
-    b_step[t] = some ? DEPTH * 256 : 0;
+    bp[t] = some ? xs + tok * p.x_pitch + ch0 * 256 + (lane & 3) * 16 : smem + 64;
+    b_step[t] = some ? AHEAD * STEP * 256 : 0;
   }
   const float4* sp4 = base + ch0 * TOKS + (lane & 3);
   // the masks in registers, so that a code pair is one operation with its other constant
   uint32_t low = 0x000f000fu, high = 0x00f000f0u;
   asm volatile("" : "+r"(low), "+r"(high));
 
-  for (int c0 = ch0; c0 < end; c0 += DEPTH) {
+  const bool far = (lane & 4) != 0;
+  static_assert(AHEAD * STEP == 4, "a lane's scales are of every fourth chunk");
+  for (int c0 = ch0; c0 < end; c0 += AHEAD * STEP) {
 #pragma unroll
-    for (int j = 0; j < 2 * RT; j++) wp[j] += DEPTH * 64, sp[j] += DEPTH * 2;  // DEPTH chunks on, fetched behind these
+    for (int r = 0; r < RT; r++) sc[r][0] = sc_next[r][0], sc[r][1] = sc_next[r][1];
+    fetch_scales(c0 + AHEAD * STEP);
 #pragma unroll
-    for (int st = 0; st < DEPTH; st++) {
-      if (c0 + st < end) {
+    for (int ah = 0; ah < AHEAD; ah++) {
+      if (c0 + ah * STEP >= end) break;
+      uint4 wq[STEP][2 * RT];
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {  // lane l has a channel's first chunk, lane l + 4 its second, and of the channel 4 on too
+          const uint4 &one = raw[ah][r][2 * h], &two = raw[ah][r][2 * h + 1];
+          uint4 x = far ? one : two;
+          x.x = __shfl_xor_sync(0xffffffffu, x.x, 4);
+          x.y = __shfl_xor_sync(0xffffffffu, x.y, 4);
+          x.z = __shfl_xor_sync(0xffffffffu, x.z, 4);
+          x.w = __shfl_xor_sync(0xffffffffu, x.w, 4);
+          wq[0][2 * r + h] = far ? x : one;
+          wq[1][2 * r + h] = far ? two : x;
+        }
+        fetch(ah, r, c0 + (ah + AHEAD) * STEP);
+      }
+#pragma unroll
+      for (int st = 0; st < STEP; st++) {
+        const int ch = ah * STEP + st;
+        if (c0 + ch >= end) break;
         float d[RT][NT][4], e[RT][CHAINS == 2 ? NT : 1][4];  // one or two chains of products
         float2 power[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-          const float4 s = sp4[st * TOKS + t * 4];
+          const float4 s = sp4[ch * TOKS + t * 4];
           power[t] = make_float2(s.z, s.w);
 #pragma unroll
           for (int r = 0; r < RT; r++) {
@@ -347,7 +395,7 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
         for (int q = 0; q < 4; q++) {
           uint4 b[NT];
 #pragma unroll
-          for (int t = 0; t < NT; t++) b[t] = *reinterpret_cast<const uint4*>(bp[t] + st * 256 + q * 64);
+          for (int t = 0; t < NT; t++) b[t] = *reinterpret_cast<const uint4*>(bp[t] + ch * 256 + q * 64);
 #pragma unroll
           for (int r = 0; r < RT; r++) {
             const uint4 &l4 = wq[st][2 * r], &h4 = wq[st][2 * r + 1];
@@ -368,8 +416,9 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
         for (int r = 0; r < RT; r++) {
           // with (2^24) 2^-15; the powers come last, in the addition, so that sums of tiny values are rounded once
           constexpr float F = PIECES == 1 ? 512.f : 3.0517578125e-5f;
-          const float2 s0 = __fmul2_rn(unpack_f16x2(sc[st][2 * r]), make_float2(F, F));
-          const float2 s1 = __fmul2_rn(unpack_f16x2(sc[st][2 * r + 1]), make_float2(F, F));
+          const int holder = (lane & ~3) | ch;
+          const float2 s0 = __fmul2_rn(unpack_f16x2(__shfl_sync(0xffffffffu, sc[r][0], holder)), make_float2(F, F));
+          const float2 s1 = __fmul2_rn(unpack_f16x2(__shfl_sync(0xffffffffu, sc[r][1], holder)), make_float2(F, F));
 #pragma unroll
           for (int t = 0; t < NT; t++) {
             float(&u)[4] = d[r][t];
@@ -378,12 +427,11 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
             acc[r][t][1] = fmaf(u[3] * s1.y, power[t].y, fmaf(u[2] * s1.x, power[t].x, acc[r][t][1]));
           }
         }
-        fetch(st, c0 + DEPTH);
       }
     }
 #pragma unroll
     for (int t = 0; t < NT; t++) bp[t] += b_step[t];
-    sp4 += DEPTH * TOKS;
+    sp4 += AHEAD * STEP * TOKS;
   }
 
   // The sums over this CTA's part of k: the warps' parts in turn, a token's pieces.
@@ -391,7 +439,7 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
   for (int r = 0; r < RT; r++)
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const int at = (warp * ROWS + r * 16 + (lane >> 2)) * TOKS + t * 4 + (lane & 3);
+      const int at = (warp * ROWS + r * 16 + channel) * TOKS + t * 4 + (lane & 3);
       red[at] = acc[r][t][0];
       red[at + 8 * TOKS] = acc[r][t][1];
     }
@@ -454,7 +502,7 @@ cudaError_t launch_matvec(const void* x, const void* wv, void* y, const MatmulAr
   const bool f32 = a.x_dtype == WE_F32;
   const int toks = (int)a.m * (f32 ? 2 : 1);
   const int nt = toks <= 4 ? 1 : (toks <= 8 ? 2 : (toks <= 16 ? 4 : 8));
-  const int per_sm = nt == 8 ? 1 : 2, rt = nt <= 2 ? 2 : 1;  // the instances below
+  const int per_sm = nt == 8 ? 1 : 2, rt = 1;  // the instances below
   const int64_t chunks = (a.k + CHUNK - 1) / CHUNK, tiles = (a.n + rt * 16 - 1) / (rt * 16);
   // How k is split over clusters and warps: the shortest chain of instructions of an SM's warp slot (its share of x's
   // layout, its steps, its sums and the cluster's, for as many waves of CTAs as it takes).
@@ -493,13 +541,13 @@ cudaError_t launch_matvec(const void* x, const void* wv, void* y, const MatmulAr
   const int ny = (int)gy;
   cudaError_t e;
   if (f32) {
-    e = nt == 1   ? matvec_mma<WE_F32, 1, 2, 2>(x, w, y, a, p, ny, st)
-        : nt == 2 ? matvec_mma<WE_F32, 2, 2, 2>(x, w, y, a, p, ny, st)
+    e = nt == 1   ? matvec_mma<WE_F32, 1, 1, 2>(x, w, y, a, p, ny, st)
+        : nt == 2 ? matvec_mma<WE_F32, 2, 1, 2>(x, w, y, a, p, ny, st)
         : nt == 4 ? matvec_mma<WE_F32, 4, 1, 2>(x, w, y, a, p, ny, st)
                   : matvec_mma<WE_F32, 8, 1, 1>(x, w, y, a, p, ny, st);
   } else {
-    e = nt == 1   ? matvec_mma<WE_BF16, 1, 2, 2>(x, w, y, a, p, ny, st)
-        : nt == 2 ? matvec_mma<WE_BF16, 2, 2, 2>(x, w, y, a, p, ny, st)
+    e = nt == 1   ? matvec_mma<WE_BF16, 1, 1, 2>(x, w, y, a, p, ny, st)
+        : nt == 2 ? matvec_mma<WE_BF16, 2, 1, 2>(x, w, y, a, p, ny, st)
                   : matvec_mma<WE_BF16, 4, 1, 2>(x, w, y, a, p, ny, st);
   }
   return e == cudaSuccess ? cudaGetLastError() : e;
