@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
   // [chunks of the slice][TOKS]: the two groups' starts (-8 sum of x) and powers of two
   float4* base = reinterpret_cast<float4*>(xs + toks * p.x_pitch);
   float* red = reinterpret_cast<float*>(base + p.per_cta * TOKS);  // [WARPS][ROWS][TOKS]
-  float* part = red + WARPS * ROWS * TOKS;                         // [m][channels of the CTA]
+  float* part = red + WARPS * ROWS * TOKS;                         // [cluster][blocks of outputs][THREADS]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)tc::cluster_rank();
   const int kpart = warp & (p.wk - 1);                             // this warp's part of k
@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
   const int my_groups = max(0, min(p.per_cta * 2, groups - g0));
   const int chunks = (my_groups + 1) / 2;                          // of this CTA, the last one perhaps half
   const int ch0 = chunks * kpart / p.wk, end = chunks * (kpart + 1) / p.wk;  // this warp's chunks
+  if (p.cluster > 1) tc::cluster_arrive();
   pdl_launch_dependents();
   pdl_wait();
 
@@ -218,12 +219,13 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
   const char* src = static_cast<const char*>(x) + (int64_t)g0 * 64 * XB;
   const bool wide = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)(a.x_stride * XB)) & 15) == 0;
   uint32_t ahead[4 * XB];  // the values as they are
+  int i_ahead = 0, e_ahead = 0;  // their row, and unit of the row
   auto load_x = [&](int u) {
 #pragma unroll
     for (int j = 0; j < 4 * XB; j++) ahead[j] = 0;
-    const int i = u / units_row, e = u - i * units_row;
-    if (u >= units || e * 16 >= my_groups * 64) return;
-    const char* from = src + ((int64_t)i * a.x_stride + e * 16) * XB;
+    i_ahead = u / units_row, e_ahead = u - i_ahead * units_row;
+    if (u >= units || e_ahead * 16 >= my_groups * 64) return;
+    const char* from = src + ((int64_t)i_ahead * a.x_stride + e_ahead * 16) * XB;
     if (wide) {
 #pragma unroll
       for (int j = 0; j < XB; j++) {
@@ -255,64 +257,60 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
   for (int u = threadIdx.x; u < NOTHING / 16; u += THREADS) reinterpret_cast<uint4*>(smem)[u] = make_uint4(0, 0, 0, 0);
 
   for (int u0 = 0; u0 < units; u0 += THREADS) {
-    const int u = u0 + threadIdx.x;
-    const int i = min(u / units_row, m - 1), e = u - i * units_row;
-    uint32_t t[4 * XB];
-#pragma unroll
-    for (int j = 0; j < 4 * XB; j++) t[j] = ahead[j];
-    if (u0 + THREADS < units) load_x(u + THREADS);
+    const bool mine = u0 + threadIdx.x < units;
+    const int i = i_ahead, e = e_ahead;
     uint32_t top = 0;  // the largest magnitude's bits (bf16: of the halves, then as f32)
 #pragma unroll
-    for (int j = 0; j < 4 * XB; j++) top = XB == 4 ? max(top, t[j] & 0x7fffffffu) : __vmaxu2(top, t[j] & 0x7fff7fffu);
+    for (int j = 0; j < 4 * XB; j++) top = XB == 4 ? max(top, ahead[j] & 0x7fffffffu) : __vmaxu2(top, ahead[j] & 0x7fff7fffu);
     if (XB == 2) top = max(top & 0xffff0000u, top << 16);
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    float v[16], sum[PIECES];
+    float2 v[8];  // the pairs of the tiles: values 8 (j / 4) + j % 4 and 4 on
 #pragma unroll
-    for (int j = 0; j < 4 * XB; j++) {
-      if constexpr (XB == 4) {
-        v[j] = __uint_as_float(t[j]);
-      } else {
-        v[2 * j] = __uint_as_float(t[j] << 16);
-        v[2 * j + 1] = __uint_as_float(t[j] & 0xffff0000u);
-      }
+    for (int j = 0; j < 8; j++) {
+      const int l = (j >> 2) * 8 + (j & 3);
+      if constexpr (XB == 4) v[j] = make_float2(__uint_as_float(ahead[l]), __uint_as_float(ahead[l + 4]));
+      else if (j & 1) v[j] = make_float2(__uint_as_float(ahead[l >> 1] & 0xffff0000u), __uint_as_float(ahead[(l >> 1) + 2] & 0xffff0000u));
+      else v[j] = make_float2(__uint_as_float(ahead[l >> 1] << 16), __uint_as_float(ahead[(l >> 1) + 2] << 16));
     }
+    if (u0 + THREADS < units) load_x(u0 + THREADS + threadIdx.x);
     // 2^E of the maximum in [2^E, 2^(E + 1)); below 2^-111 the values are first brought up by 2^64
     uint32_t ex = top >> 23;
     float power = __uint_as_float(min(ex, 254u) << 23);
     if (ex < 16u) {
 #pragma unroll
-      for (int j = 0; j < 16; j++) v[j] *= 18446744073709551616.f;
+      for (int j = 0; j < 8; j++) v[j] = __fmul2_rn(v[j], make_float2(18446744073709551616.f, 18446744073709551616.f));
       ex = max(__float_as_uint(__uint_as_float(top) * 18446744073709551616.f) >> 23, 16u);
       power = __uint_as_float(ex << 23) * 5.421010862427522e-20f;
     }
     const float up = __uint_as_float((269u - min(ex, 254u)) << 23);  // 2^(15 - E)
+    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < 16; j++) v[j] *= up;
+    for (int j = 0; j < 8; j++) {
+      v[j] = __fmul2_rn(v[j], make_float2(up, up));
+      if constexpr (PIECES == 1) sum = __fadd2_rn(sum, v[j]);
+      if (j & 1) v[j] = __fmul2_rn(v[j], make_float2(0.0625f, 0.0625f));  // (the codes of these places are 16 times theirs)
+    }
+    float s = sum.x + sum.y;
+    if constexpr (PIECES == 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+    }
     uint8_t* to = xs + i * p.x_pitch + (e >> 3) * 256 + (e & 1) * 128 + ((e >> 1) & 3) * 16;
 #pragma unroll
     for (int c = 0; c < PIECES; c++) {
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < 16; j++) s += v[j];
       uint32_t o[8];
 #pragma unroll
-      for (int j = 0; j < 8; j++) {  // pair (8 (j / 4) + j % 4, + 4); odd j: x / 16
-        float *l = v + (j >> 2) * 8 + (j & 3), *h = l + 4;
-        const float down = (j & 1) ? 0.0625f : 1.f, back = (j & 1) ? 16.f : 1.f;
+      for (int j = 0; j < 8; j++) {
         if (c + 1 < PIECES) {  // the leading bits toward zero (2^16 is never reached), and what is left (below 2^5) times 2^10
-          o[j] = as_u32(__halves2half2(__float2half_rz(*l * down), __float2half_rz(*h * down)));
+          asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(o[j]) : "f"(v[j].y), "f"(v[j].x));
           const float2 f = unpack_f16x2(o[j]);
-          *l -= f.x * back, *h -= f.y * back;
-          s -= *l + *h;
-          *l *= 1024.f, *h *= 1024.f;
+          v[j] = __fmul2_rn(__fadd2_rn(v[j], make_float2(-f.x, -f.y)), make_float2(1024.f, 1024.f));
         } else {
-          o[j] = as_u32(__floats2half2_rn(*l * down, *h * down));
+          o[j] = as_u32(__floats2half2_rn(v[j].x, v[j].y));
         }
       }
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      if (u < units) {
+      if (mine) {
         uint4* piece = reinterpret_cast<uint4*>(to + c * m * p.x_pitch);
         piece[0] = make_uint4(o[0], o[1], o[2], o[3]);
         piece[4] = make_uint4(o[4], o[5], o[6], o[7]);
@@ -445,7 +443,8 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
     }
   __syncthreads();
   const int outs = cta_rows * m;
-  const int row_shift = 31 - __clz(cta_rows);
+  const int row_shift = 31 - __clz(cta_rows), blocks = ((outs + THREADS - 1) / THREADS + p.cluster - 1) / p.cluster;
+  if (p.cluster > 1) tc::cluster_wait();  // every CTA of the cluster has begun
   for (int u = threadIdx.x; u < outs; u += THREADS) {
     const int i = u >> row_shift, row = u - (i << row_shift);
     const float* from = red + (row / ROWS * p.wk * ROWS + row % ROWS) * TOKS + i;
@@ -455,23 +454,25 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
 #pragma unroll
       for (int k = 0; k < WARPS; k++)
         if (k < p.wk) v += from[k * (ROWS * TOKS) + c * m];
-    if (p.cluster > 1) part[u] = v;
-    else if (first + row < n) matvec_store(v, a, i, first + row, y);
-  }
-  if (p.cluster > 1) {  // the cluster's parts in rank order, each CTA a share of the outputs
-    tc::cluster_sync_all();
-    const uint32_t part_addr = tc::smem_u32(part);
-    for (int u = rank * THREADS + threadIdx.x; u < outs; u += p.cluster * THREADS) {
-      const int i = u >> row_shift, channel = first + u - (i << row_shift);
-      if (channel >= n) continue;
-      float o[MAX_CLUSTER], v = 0.f;
-#pragma unroll
-      for (int s = 0; s < MAX_CLUSTER; s++) o[s] = s < p.cluster ? tc::ld_cluster_f32(tc::map_rank(part_addr + 4u * u, s)) : 0.f;
-#pragma unroll
-      for (int s = 0; s < MAX_CLUSTER; s++) v += o[s];
-      matvec_store(v, a, i, channel, y);
+    if (p.cluster > 1) {  // to the CTA that adds the cluster's parts of these outputs
+      const int block = u / THREADS, owner = block % p.cluster;
+      tc::st_cluster_f32(tc::map_rank(tc::smem_u32(part + (rank * blocks + block / p.cluster) * THREADS + threadIdx.x), owner), v);
+    } else if (first + row < n) {
+      matvec_store(v, a, i, first + row, y);
     }
-    tc::cluster_sync_all();  // no CTA leaves while another reads its part
+  }
+  if (p.cluster > 1) {  // the cluster's parts in rank order
+    __syncwarp();
+    tc::cluster_sync_all();
+    for (int b = 0; b < blocks; b++) {
+      const int u = (b * p.cluster + rank) * THREADS + threadIdx.x, i = u >> row_shift, at = first + u - (i << row_shift);
+      if (u >= outs || at >= n) continue;
+      float v = 0.f;
+#pragma unroll
+      for (int s = 0; s < MAX_CLUSTER; s++)
+        if (s < p.cluster) v += part[(s * blocks + b) * THREADS + threadIdx.x];
+      matvec_store(v, a, i, at, y);
+    }
   }
 }
 
@@ -520,10 +521,11 @@ cudaError_t launch_matvec(const void* x, const void* wv, void* y, const MatmulAr
         if (wk > 1 && wk > per_cta) break;
         const int64_t rows = WARPS / wk * rt * 16, ctas = (tiles * wk + WARPS - 1) / WARPS * cluster;
         const int64_t slots = std::max<int64_t>(1, (int64_t)sms * ROOM[fit - 1][cluster - 1] / 148), waves = (ctas + slots - 1) / slots;
-        const int64_t bytes = NOTHING + toks * per_cta * CHUNK * 2 +
-                              (per_cta * nt * 16 + WARPS * rt * 16 * nt * 4 + (cluster > 1 ? rows * a.m : 0)) * 4;
-        if (bytes > 226 * 1024 / fit) continue;
         const int64_t units = (a.m * per_cta * 8 + THREADS - 1) / THREADS, outs = (rows * a.m + THREADS - 1) / THREADS;
+        const int64_t bytes = NOTHING + toks * per_cta * CHUNK * 2 +
+                              (per_cta * nt * 16 + WARPS * rt * 16 * nt * 4 +
+                               (cluster > 1 ? (outs + cluster - 1) / cluster * cluster * THREADS : 0)) * 4;
+        if (bytes > 226 * 1024 / fit) continue;
         const int64_t cost = waves * (300 + units * (f32 ? 250 : 110) + (per_cta + wk - 1) / wk * rt * (70 + 20 * nt) +
                                       outs * (30 + 4 * wk) + (cluster > 1 ? 300 : 0));
         if (best >= 0 && cost > best) continue;
