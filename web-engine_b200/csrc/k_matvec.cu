@@ -87,7 +87,6 @@ __global__ void __launch_bounds__(256) matvec_long_kernel(const void* __restrict
 
 // ---------------- tensor-core tiles ----------------
 namespace mv {
-constexpr int WARPS = 8, THREADS = WARPS * 32;
 constexpr int CHUNK = 128;       // values of k of a step: 64 packed bytes of each channel
 constexpr int MAX_CLUSTER = 8;
 constexpr int STEP = 2;          // chunks of a step: 128 bytes of each channel
@@ -139,12 +138,12 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t v, uint32_t mask, int odd
 
 // XT: type of x; NT: tiles of 8 columns; RT: row tiles of 16 channels of a warp; PER_SM: CTAs that fit an SM. Columns 2 t
 // and 2 t + 1 are the two groups of a chunk for piece t / m (f32: the leading bits, the following ones) of token t % m.
-template <int XT, int NT, int RT, int PER_SM>
-__global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const void* __restrict__ x, const uint8_t* __restrict__ w,
+template <int XT, int NT, int RT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 1) matvec_mma_kernel(const void* __restrict__ x, const uint8_t* __restrict__ w,
                                                                  void* y, const MatmulArgs a, const mv::Plan p) {
   using namespace mv;
   constexpr int XB = XT == WE_F32 ? 4 : 2, PIECES = XT == WE_F32 ? 2 : 1;
-  constexpr int TOKS = NT * 4, ROWS = RT * 16, CHAINS = NT * RT <= 2 ? 2 : 1;
+  constexpr int THREADS = WARPS * 32, TOKS = NT * 4, ROWS = RT * 16, CHAINS = NT * RT <= 2 ? 2 : 1;
   extern __shared__ __align__(16) uint8_t smem[];
   const int m = (int)a.m, n = (int)a.n, toks = m * PIECES;
   const int groups = (int)(a.k / 64);
@@ -445,6 +444,7 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
   const int outs = cta_rows * m;
   const int row_shift = 31 - __clz(cta_rows), blocks = ((outs + THREADS - 1) / THREADS + p.cluster - 1) / p.cluster;
   if (p.cluster > 1) tc::cluster_wait();  // every CTA of the cluster has begun
+  int owner = 0, slot = rank * blocks;  // the CTA that adds the cluster's parts of a block of outputs, and where it holds ours
   for (int u = threadIdx.x; u < outs; u += THREADS) {
     const int i = u >> row_shift, row = u - (i << row_shift);
     const float* from = red + (row / ROWS * p.wk * ROWS + row % ROWS) * TOKS + i;
@@ -454,9 +454,9 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
 #pragma unroll
       for (int k = 0; k < WARPS; k++)
         if (k < p.wk) v += from[k * (ROWS * TOKS) + c * m];
-    if (p.cluster > 1) {  // to the CTA that adds the cluster's parts of these outputs
-      const int block = u / THREADS, owner = block % p.cluster;
-      tc::st_cluster_f32(tc::map_rank(tc::smem_u32(part + (rank * blocks + block / p.cluster) * THREADS + threadIdx.x), owner), v);
+    if (p.cluster > 1) {
+      tc::st_cluster_f32(tc::map_rank(tc::smem_u32(part + slot * THREADS + threadIdx.x), owner), v);
+      if (++owner == p.cluster) owner = 0, slot++;
     } else if (first + row < n) {
       matvec_store(v, a, i, first + row, y);
     }
@@ -476,15 +476,15 @@ __global__ void __launch_bounds__(mv::THREADS, PER_SM) matvec_mma_kernel(const v
   }
 }
 
-template <int XT, int NT, int RT, int PER_SM>
+template <int XT, int NT, int RT, int WARPS>
 static cudaError_t matvec_mma(const void* x, const uint8_t* w, void* y, const MatmulArgs& a, const mv::Plan& p, int groups_y,
                               cudaStream_t st) {
-  auto kern = matvec_mma_kernel<XT, NT, RT, PER_SM>;
+  auto kern = matvec_mma_kernel<XT, NT, RT, WARPS>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p.cluster, (unsigned)groups_y);
-  cfg.blockDim = dim3(mv::THREADS);
+  cfg.blockDim = dim3(WARPS * 32);
   cfg.dynamicSmemBytes = (size_t)p.smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -503,29 +503,27 @@ cudaError_t launch_matvec(const void* x, const void* wv, void* y, const MatmulAr
   const bool f32 = a.x_dtype == WE_F32;
   const int toks = (int)a.m * (f32 ? 2 : 1);
   const int nt = toks <= 4 ? 1 : (toks <= 8 ? 2 : (toks <= 16 ? 4 : 8));
-  const int per_sm = nt == 8 ? 1 : 2, rt = 1;  // the instances below
+  const int WARPS = nt == 8 ? 8 : 16, THREADS = WARPS * 32, rt = 1;  // the instances below
   const int64_t chunks = (a.k + CHUNK - 1) / CHUNK, tiles = (a.n + rt * 16 - 1) / (rt * 16);
   // How k is split over clusters and warps: the shortest chain of instructions of an SM's warp slot (its share of x's
   // layout, its steps, its sums and the cluster's, for as many waves of CTAs as it takes).
   // ROOM: CTAs that 148 SMs hold at a time, 1 or 2 an SM, in clusters of 1 to 8 (cudaOccupancyMaxActiveClusters; a cluster
   // stays within a GPC). Of the splits of nine shapes, all of them timed, this picks the fastest or one within 5% of it: 8
   // tokens of 16384 values to 6144 channels take 26.8 us with clusters of 5 and 28.9 with the best power of two.
-  static constexpr int ROOM[2][MAX_CLUSTER] = {{148, 148, 135, 132, 130, 132, 105, 120}, {296, 296, 279, 284, 280, 270, 259, 264}};
+  static constexpr int ROOM[MAX_CLUSTER] = {148, 148, 135, 132, 130, 132, 105, 120};
   Plan p{};
   int64_t best = -1;
-  // (x that does not leave room for two CTAs an SM has one)
-  for (int fit = per_sm; fit >= 1 && best < 0; fit--)
     for (int cluster = 1; cluster <= MAX_CLUSTER; cluster++)
       for (int wk = 1; wk <= WARPS; wk *= 2) {
         const int64_t per_cta = (chunks + cluster - 1) / cluster;
         if (wk > 1 && wk > per_cta) break;
         const int64_t rows = WARPS / wk * rt * 16, ctas = (tiles * wk + WARPS - 1) / WARPS * cluster;
-        const int64_t slots = std::max<int64_t>(1, (int64_t)sms * ROOM[fit - 1][cluster - 1] / 148), waves = (ctas + slots - 1) / slots;
+        const int64_t slots = std::max<int64_t>(1, (int64_t)sms * ROOM[cluster - 1] / 148), waves = (ctas + slots - 1) / slots;
         const int64_t units = (a.m * per_cta * 8 + THREADS - 1) / THREADS, outs = (rows * a.m + THREADS - 1) / THREADS;
         const int64_t bytes = NOTHING + toks * per_cta * CHUNK * 2 +
                               (per_cta * nt * 16 + WARPS * rt * 16 * nt * 4 +
                                (cluster > 1 ? (outs + cluster - 1) / cluster * cluster * THREADS : 0)) * 4;
-        if (bytes > 226 * 1024 / fit) continue;
+        if (bytes > 226 * 1024) continue;
         const int64_t cost = waves * (300 + units * (f32 ? 250 : 110) + (per_cta + wk - 1) / wk * rt * (70 + 20 * nt) +
                                       outs * (30 + 4 * wk) + (cluster > 1 ? 300 : 0));
         if (best >= 0 && cost > best) continue;
@@ -543,14 +541,14 @@ cudaError_t launch_matvec(const void* x, const void* wv, void* y, const MatmulAr
   const int ny = (int)gy;
   cudaError_t e;
   if (f32) {
-    e = nt == 1   ? matvec_mma<WE_F32, 1, 1, 2>(x, w, y, a, p, ny, st)
-        : nt == 2 ? matvec_mma<WE_F32, 2, 1, 2>(x, w, y, a, p, ny, st)
-        : nt == 4 ? matvec_mma<WE_F32, 4, 1, 2>(x, w, y, a, p, ny, st)
-                  : matvec_mma<WE_F32, 8, 1, 1>(x, w, y, a, p, ny, st);
+    e = nt == 1   ? matvec_mma<WE_F32, 1, 1, 16>(x, w, y, a, p, ny, st)
+        : nt == 2 ? matvec_mma<WE_F32, 2, 1, 16>(x, w, y, a, p, ny, st)
+        : nt == 4 ? matvec_mma<WE_F32, 4, 1, 16>(x, w, y, a, p, ny, st)
+                  : matvec_mma<WE_F32, 8, 1, 8>(x, w, y, a, p, ny, st);
   } else {
-    e = nt == 1   ? matvec_mma<WE_BF16, 1, 1, 2>(x, w, y, a, p, ny, st)
-        : nt == 2 ? matvec_mma<WE_BF16, 2, 1, 2>(x, w, y, a, p, ny, st)
-                  : matvec_mma<WE_BF16, 4, 1, 2>(x, w, y, a, p, ny, st);
+    e = nt == 1   ? matvec_mma<WE_BF16, 1, 1, 16>(x, w, y, a, p, ny, st)
+        : nt == 2 ? matvec_mma<WE_BF16, 2, 1, 16>(x, w, y, a, p, ny, st)
+                  : matvec_mma<WE_BF16, 4, 1, 16>(x, w, y, a, p, ny, st);
   }
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
