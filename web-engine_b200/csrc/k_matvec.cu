@@ -18,9 +18,14 @@
 // - A lane reads 16 bytes of a channel at once, so the four lanes of a tile's row hold two groups of 64. A token
 //   therefore is two columns, one per group, each zero where the lane's values belong to the other group: one product
 //   gives both groups' sums side by side and each takes its own scale.
-// - Weights go from global memory to registers, 4 KB a warp ahead of their use. Warps split channels and k; clusters of up
-//   to 8 CTAs split k when there are few channels or x does not fit. Partial sums meet in shared memory in a fixed order,
-//   so a call always gives the same bits.
+// - Weights go from global memory to registers, 128 bytes of a channel a load and 4 KB a warp ahead of their use. A CTA is
+//   16 warps (x is laid out once for all of them; with two CTAs of 8 an SM, 16 tokens took 44 us and now 35), which split
+//   channels and k; clusters of up to 8 CTAs split k when there are few channels or x does not fit. Partial sums meet in
+//   shared memory in a fixed order, so a call always gives the same bits.
+// Measured: one token of 6144 values to 16384 channels 14.4 us (3.7 TB/s; a quarter of it until x is laid out and the first
+// weights are there, then 6 TB/s), to 1536 channels 5.0; 8 tokens of 16384 to 6144 22.9, 16 tokens 37 (tensor tiles at 70% of
+// the legacy instruction's rate in the main loop, x's layout and the sums a third of the time); f32, 3 tokens of 2496 values
+// to 5003 channels 8.0. Tried and slower: all weights asked into L2 at once (18 us instead of 14), 256-byte bulk copies.
 #include <algorithm>
 
 #include "common.cuh"
@@ -505,11 +510,11 @@ cudaError_t launch_matvec(const void* x, const void* wv, void* y, const MatmulAr
   const int nt = toks <= 4 ? 1 : (toks <= 8 ? 2 : (toks <= 16 ? 4 : 8));
   const int WARPS = nt == 8 ? 8 : 16, THREADS = WARPS * 32, rt = 1;  // the instances below
   const int64_t chunks = (a.k + CHUNK - 1) / CHUNK, tiles = (a.n + rt * 16 - 1) / (rt * 16);
-  // How k is split over clusters and warps: the shortest chain of instructions of an SM's warp slot (its share of x's
-  // layout, its steps, its sums and the cluster's, for as many waves of CTAs as it takes).
-  // ROOM: CTAs that 148 SMs hold at a time, 1 or 2 an SM, in clusters of 1 to 8 (cudaOccupancyMaxActiveClusters; a cluster
-  // stays within a GPC). Of the splits of nine shapes, all of them timed, this picks the fastest or one within 5% of it: 8
-  // tokens of 16384 values to 6144 channels take 26.8 us with clusters of 5 and 28.9 with the best power of two.
+  // How k is split over clusters and warps: the shortest chain of a warp (its share of x's layout, its steps, its sums and
+  // the cluster's, for as many waves of CTAs as it takes), in weights fitted to the timed splits.
+  // ROOM: CTAs that 148 SMs hold at a time in clusters of 1 to 8, one CTA an SM (cudaOccupancyMaxActiveClusters; a cluster
+  // stays within a GPC). All splits of 21 shapes were timed: this picks the fastest of 20 and one 7% slower of the other. 8
+  // tokens of 16384 values to 6144 channels take 22.9 us with clusters of 5 and 26.4 with the best power of two.
   static constexpr int ROOM[MAX_CLUSTER] = {148, 148, 135, 132, 130, 132, 105, 120};
   Plan p{};
   int64_t best = -1;
@@ -524,8 +529,8 @@ cudaError_t launch_matvec(const void* x, const void* wv, void* y, const MatmulAr
                               (per_cta * nt * 16 + WARPS * rt * 16 * nt * 4 +
                                (cluster > 1 ? (outs + cluster - 1) / cluster * cluster * THREADS : 0)) * 4;
         if (bytes > 226 * 1024) continue;
-        const int64_t cost = waves * (300 + units * (f32 ? 250 : 110) + (per_cta + wk - 1) / wk * rt * (70 + 20 * nt) +
-                                      outs * (30 + 4 * wk) + (cluster > 1 ? 300 : 0));
+        const int64_t cost = waves * (units * (f32 ? 500 : 400) + (per_cta + wk - 1) / wk * rt * (70 + 20 * nt) +
+                                      outs * (60 + 2 * wk) + (cluster > 1 ? 100 : 0));
         if (best >= 0 && cost > best) continue;
         best = cost;
         p = Plan{wk, cluster, (int)per_cta, (int)per_cta * CHUNK * 2, (int)bytes};
