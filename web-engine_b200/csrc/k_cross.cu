@@ -53,9 +53,10 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {  // of an 8 x 8 til
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-// x as two tf32 terms: the nearest one, and what is left (the product drops its last bits, below 2^-22 of x)
+// x as two tf32 terms: the nearest one (to 11 bits, ties up), and what is left, of whose 12 bits the product drops one.
+// (cvt.rna.tf32 takes several instructions here: 1024 queries x 512 keys of 12 heads 192 us with it.)
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
   lo = __float_as_uint(x - __uint_as_float(hi));
 }
 // d += a b in three products
