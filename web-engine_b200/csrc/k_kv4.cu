@@ -27,6 +27,8 @@ __device__ __forceinline__ int64_t kv4_row(const we_kv4_cache& c, int64_t b, int
 // Rows in and out of the cache. A thread moves 8 values of k or of v a step: 16 bytes (bf16) or 32 on the wide side, a 4-byte
 // word on the packed one, 8 neighbouring lanes a group. It keeps its place within a token (side, head, values) and steps
 // over the tokens of its CTA, whose rows are looked up once, so that a step has little to compute but the values.
+// Measured: 2 x 4099 tokens x 12 heads of 128 in bf16 in 26 us and back in 17 (the bytes of each are 10 us), 16 tokens both
+// ways 4.7 us; a warp per group and a look-up per value took 167 us.
 constexpr int ROW_THREADS = 256, ROW_SPAN = 32;
 struct RowShape {
   int units;       // of 8 values in a token: k's, then v's
