@@ -458,8 +458,11 @@ CrossPlan cross_plan(const we_cross_desc& d, int sms) {
   const int64_t slots = (int64_t)sms * per_sm - 8 * per_sm, tk = std::max<int64_t>(1, d.tk);
   // where the row tiles alone fill the SMs, a CTA takes all keys of its rows
   q.cluster = q.nq == 2 && q.units >= slots ? 1 : 8;
-  const int64_t runs = std::max<int64_t>(1, slots / (q.units * q.cluster));
-  const int64_t chunk = std::max<int64_t>(64, (tk + runs * q.cluster - 1) / (runs * q.cluster));
+  // several runs only where they spare a CTA more than merging them costs, some 150 KB of keys and values: one query to 2048
+  // keys of 12 heads of 128 8.4 us in one run and 9.5 in several, to 8192 20.4 and 16.0
+  const int64_t alone = (tk + q.cluster - 1) / q.cluster, fit = std::max<int64_t>(1, slots / (q.units * q.cluster));
+  const int64_t runs = (alone - alone / fit) * 2 * q.dim * (f32 ? 4 : 2) > 150000 ? fit : 1;
+  const int64_t chunk = std::max<int64_t>(128, (alone + runs - 1) / runs);
   q.chunk = (int)((std::min<int64_t>(chunk, 0x4000000) + 15) / 16 * 16);
   q.runs = (int)((tk + (int64_t)q.chunk * q.cluster - 1) / ((int64_t)q.chunk * q.cluster));
   q.part_floats = q.runs > 1 ? q.units * q.runs * 8 * q.nq * (q.dim + 4) : 0;

@@ -844,12 +844,15 @@ Kv4Plan kv4_plan(const Kv4AttnArgs& a, int sms) {
   q.nq = rows <= 8 ? 1 : 2;
   q.row_tiles = (int)((rows + 8 * q.nq - 1) / (8 * q.nq));
   q.units = a.c.batch * a.c.kv_heads * q.row_tiles;
-  // Four CTAs an SM, less what no cluster of 8 fits into (71 of 74 do). A sequence's length is known on the device only, so runs are cut for the longest possible one, into
-  // about one wave of CTAs; more and shorter ones cost more in their first and last steps than ragged lengths gain (68 us
-  // against 81 with four waves for 16 sequences of 3001 to 16384 keys, 60 against 78 for one of 131000).
-  const int64_t cap = std::max<int64_t>(1, a.c.max_pages * a.c.page);
-  const int64_t runs = std::max<int64_t>(1, (int64_t)(sms * 4 - 24) / (q.units * kv::CLUSTER));
-  const int64_t chunk = std::max<int64_t>(128, (cap + runs * kv::CLUSTER - 1) / (runs * kv::CLUSTER));
+  // Four CTAs an SM, less what no cluster of 8 fits into (71 of 74 do). A sequence's length is known on the device only, so
+  // runs are cut for the longest possible one, into about one wave of CTAs; more and shorter ones cost more in their first
+  // and last steps than ragged lengths gain (68 us against 81 with four waves for 16 sequences of 3001 to 16384 keys, 60
+  // against 78 for one of 131000). Merging runs takes as long as some 800 keys of a CTA, so that many have to be saved: one
+  // sequence of 4096 keys, 12 heads, 9.3 us in one run and 11.4 in five, 8192 13.5 and 13.0, 16384 22.5 and 16.5.
+  const int64_t cap = std::max<int64_t>(1, a.c.max_pages * a.c.page), alone = (cap + kv::CLUSTER - 1) / kv::CLUSTER;
+  const int64_t fit = std::max<int64_t>(1, (int64_t)(sms * 4 - 24) / (q.units * kv::CLUSTER));
+  const int64_t runs = alone - alone / fit > 800 ? fit : 1;
+  const int64_t chunk = std::max<int64_t>(256, (alone + runs - 1) / runs);
   q.chunk = (int)((std::min<int64_t>(chunk, 0x4000000) + 31) / 32 * 32);
   q.runs = (int)((cap + (int64_t)q.chunk * kv::CLUSTER - 1) / ((int64_t)q.chunk * kv::CLUSTER));
   q.part_floats = q.runs > 1 ? q.units * q.runs * 8 * q.nq * (a.c.dim + 4) : 0;
