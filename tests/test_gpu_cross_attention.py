@@ -202,3 +202,12 @@ def test_more_query_tiles_than_resident_blocks(we, graph, dim, out_dtype, tk):
 def test_groups_of_heads_that_share_keys(we, graph, heads, kv_heads, tq):
     """Groups that do not divide a tile of rows, that fill it, and one larger than it."""
     run(we, graph, 2, tq, 333, heads, kv_heads, 64, "bf16", lengths=[333, 130], seed=31, poison=True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("batch,tq,tk,heads,kv_heads,dim", [(2, 1, 20000, 6, 2, 64), (1, 4, 12001, 4, 2, 128), (2, 2, 5003, 4, 1, 256),
+                                                            (1, 11, 9000, 2, 2, 64)])
+def test_keys_shared_by_several_clusters(we, graph, batch, tq, tk, heads, kv_heads, dim, dtype):
+    lengths = [tk, tk // 3][:batch]
+    for seed in (41, 42):
+        run(we, graph, batch, tq, tk, heads, kv_heads, dim, dtype, lengths=lengths, seed=seed)

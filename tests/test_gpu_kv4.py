@@ -412,3 +412,14 @@ def test_create_and_a_decoding_loop(we, graph):
         have += tokens
     assert graph.read(first.lengths, 8, np.int32).tolist() == [have, have]
     graph.release(mark)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("case", [(2, 1, [30000, 9000], 8, 2, 64, 64), (1, 4, [24000], 16, 2, 128, 32), (3, 12, [9001, -1, 20], 6, 2, 64, 16),
+                                  (1, 1, [8300], 3, 1, 256, 48)], ids=str)
+def test_attention_over_several_runs(we, graph, case, dtype):
+    """Sequences long enough that clusters share one, beside short and idle ones; twice, to see the counters left at zero."""
+    mark = graph.mark()
+    for seed in (30, 40):
+        run_attention(we, graph, *case, dtype, seed=seed)
+    graph.release(mark)
