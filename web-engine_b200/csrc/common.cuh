@@ -226,6 +226,12 @@ static inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, unsign
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// dynamic shared memory beyond the 48 KB that every kernel may have
+template <typename Kernel>
+static inline cudaError_t allow_smem(Kernel kernel, int bytes) {
+  return bytes <= 48 * 1024 ? cudaSuccess : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
 // the programmatic-serialization attribute for a launch that sets its own other attributes
 static inline void pdl_attribute(cudaLaunchAttribute& a) {
   a.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -476,7 +476,7 @@ cudaError_t cross_tile(const cross::Params& p, dim3 grid, cudaStream_t st) {
   constexpr int ring = (F32 ? NQ * (D / 8) * 512 : 0) + cross::WARPS * DEPTH * 2 * cross::TILE * D * es;
   constexpr int merge = (cross::WARPS + 1) * 8 * NQ * MERGE_PITCH<D> * 4;
   constexpr int bytes = ring > merge ? ring : merge;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  const cudaError_t e = allow_smem(kern, bytes);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;

@@ -865,7 +865,7 @@ cudaError_t kv4_launch(const kv::Params& p, dim3 grid, cudaStream_t st) {
   constexpr int ring = kv::WARPS * kv::KV_DEPTH * KT * (D * 16 + D);
   constexpr int merge = (kv::WARPS + 1) * 8 * NQ * (D + 4) * 4;
   constexpr int bytes = ring > merge ? ring : merge;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  const cudaError_t e = allow_smem(kern, bytes);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;

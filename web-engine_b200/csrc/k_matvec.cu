@@ -485,7 +485,7 @@ template <int XT, int NT, int RT, int WARPS>
 static cudaError_t matvec_mma(const void* x, const uint8_t* w, void* y, const MatmulArgs& a, const mv::Plan& p, int groups_y,
                               cudaStream_t st) {
   auto kern = matvec_mma_kernel<XT, NT, RT, WARPS>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
+  const cudaError_t e = allow_smem(kern, p.smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p.cluster, (unsigned)groups_y);
@@ -493,12 +493,12 @@ static cudaError_t matvec_mma(const void* x, const uint8_t* w, void* y, const Ma
   cfg.dynamicSmemBytes = (size_t)p.smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)p.cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  pdl_attribute(attr[1]);
+  pdl_attribute(attr[0]);
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = p.cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, x, w, y, a, p);
 }
 
@@ -508,8 +508,8 @@ cudaError_t launch_matvec(const void* x, const void* wv, void* y, const MatmulAr
   const bool f32 = a.x_dtype == WE_F32;
   const int toks = (int)a.m * (f32 ? 2 : 1);
   const int nt = toks <= 4 ? 1 : (toks <= 8 ? 2 : (toks <= 16 ? 4 : 8));
-  const int WARPS = nt == 8 ? 8 : 16, THREADS = WARPS * 32, rt = 1;  // the instances below
-  const int64_t chunks = (a.k + CHUNK - 1) / CHUNK, tiles = (a.n + rt * 16 - 1) / (rt * 16);
+  const int WARPS = nt == 8 ? 8 : 16, THREADS = WARPS * 32;  // the instances below
+  const int chunks = (int)((a.k + CHUNK - 1) / CHUNK), tiles = (int)((a.n + 15) / 16);
   // How k is split over clusters and warps: the shortest chain of a warp (its share of x's layout, its steps, its sums and
   // the cluster's, for as many waves of CTAs as it takes), in weights fitted to the timed splits.
   // ROOM: CTAs that 148 SMs hold at a time in clusters of 1 to 8, one CTA an SM (cudaOccupancyMaxActiveClusters; a cluster
@@ -518,25 +518,29 @@ cudaError_t launch_matvec(const void* x, const void* wv, void* y, const MatmulAr
   static constexpr int ROOM[MAX_CLUSTER] = {148, 148, 135, 132, 130, 132, 105, 120};
   Plan p{};
   int64_t best = -1;
-    for (int cluster = 1; cluster <= MAX_CLUSTER; cluster++)
-      for (int wk = 1; wk <= WARPS; wk *= 2) {
-        const int64_t per_cta = (chunks + cluster - 1) / cluster;
-        if (wk > 1 && wk > per_cta) break;
-        const int64_t rows = WARPS / wk * rt * 16, ctas = (tiles * wk + WARPS - 1) / WARPS * cluster;
-        const int64_t slots = std::max<int64_t>(1, (int64_t)sms * ROOM[cluster - 1] / 148), waves = (ctas + slots - 1) / slots;
-        const int64_t units = (a.m * per_cta * 8 + THREADS - 1) / THREADS, outs = (rows * a.m + THREADS - 1) / THREADS;
-        const int64_t bytes = NOTHING + toks * per_cta * CHUNK * 2 +
-                              (per_cta * nt * 16 + WARPS * rt * 16 * nt * 4 +
-                               (cluster > 1 ? (outs + cluster - 1) / cluster * cluster * THREADS : 0)) * 4;
-        if (bytes > 226 * 1024) continue;
-        const int64_t cost = waves * (units * (f32 ? 500 : 400) + (per_cta + wk - 1) / wk * rt * (70 + 20 * nt) +
-                                      outs * (60 + 2 * wk) + (cluster > 1 ? 100 : 0));
-        if (best >= 0 && cost > best) continue;
-        best = cost;
-        p = Plan{wk, cluster, (int)per_cta, (int)per_cta * CHUNK * 2, (int)bytes};
-      }
+  const int warps_shift = nt == 8 ? 3 : 4, threads_shift = warps_shift + 5, m = (int)a.m;
+  for (int cluster = 1; cluster <= MAX_CLUSTER; cluster++) {
+    const int per_cta = (chunks + cluster - 1) / cluster, slots = std::max(1, sms * ROOM[cluster - 1] / 148);
+    const int64_t x_bytes = (int64_t)toks * per_cta * (CHUNK * 2) + (int64_t)per_cta * (nt * 64);
+    if (x_bytes > 226 * 1024) continue;
+    const int units = (m * per_cta * 8 + THREADS - 1) >> threads_shift;
+    for (int split = 0; split <= warps_shift; split++) {  // log2 of the warps that split k
+      const int wk = 1 << split;
+      if (wk > 1 && wk > per_cta) break;
+      const int rows = 16 << (warps_shift - split), outs = (rows * m + THREADS - 1) >> threads_shift;
+      const int64_t ctas = (((int64_t)tiles << split) + WARPS - 1 >> warps_shift) * cluster, waves = (ctas + slots - 1) / slots;
+      const int64_t bytes = NOTHING + x_bytes + WARPS * 16 * nt * 16 +
+                            (cluster > 1 ? (outs + cluster - 1) / cluster * cluster * THREADS * 4 : 0);
+      if (bytes > 226 * 1024) continue;
+      const int64_t cost = waves * (units * (f32 ? 500 : 400) + ((per_cta + wk - 1) >> split) * (70 + 20 * nt) +
+                                    outs * (60 + 2 * wk) + (cluster > 1 ? 100 : 0));
+      if (best >= 0 && cost > best) continue;
+      best = cost;
+      p = Plan{wk, cluster, per_cta, per_cta * CHUNK * 2, (int)bytes};
+    }
+  }
   const bool ok = best >= 0;
-  const int64_t cta_rows = ok ? WARPS / p.wk * rt * 16 : 1, gy = (a.n + cta_rows - 1) / cta_rows;
+  const int64_t cta_rows = ok ? WARPS / p.wk * 16 : 1, gy = (a.n + cta_rows - 1) / cta_rows;
   if (!ok || gy > 65535) {
     const dim3 grid((unsigned)((a.n + 7) / 8));
     const cudaError_t e = f32 ? launch_pdl(matvec_long_kernel<WE_F32>, grid, 256, 0, st, x, w, y, a)
