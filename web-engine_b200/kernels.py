@@ -28,7 +28,8 @@ class Call:
 
     def __init__(self, graph: Graph, fn, args: tuple, keep=()):
         self.fn, self.ctx, self.keep = fn, graph.ctx, keep
-        self.args = (graph.ctx, *args)
+        # numbers as C values too: converting them in every call costs some tenths of a microsecond
+        self.args = (graph.ctx, *(t(a) if isinstance(a, (int, float)) else a for t, a in zip(fn.argtypes[1:], args)))
 
     def __call__(self) -> None:
         rc = self.fn(*self.args)
