@@ -423,3 +423,23 @@ def test_attention_over_several_runs(we, graph, case, dtype):
     for seed in (30, 40):
         run_attention(we, graph, *case, dtype, seed=seed)
     graph.release(mark)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_append_of_a_long_prompt(we, graph, dtype, shift):
+    """Enough tokens for more blocks than two an SM, with rows of whole 16 bytes and (shift) without."""
+    tokens, kvh, dim, page = 2500, 3, 128, 32
+    stride = kvh * dim + shift
+    x = [bf16_round(randn(tokens * stride, 50 + i)) for i in range(2)]
+    mark = graph.mark()
+    c = Cache(we, graph, 1, tokens + 40, kvh, dim, page)
+    c.set_lengths([33])
+    we.kv4.append(graph, c.c, *(graph.buffer(bits(v, dtype)) for v in x), tokens, dtype=dtype, stride=stride)
+    for name, v in zip("kv", x):
+        rows = v.reshape(tokens, stride)[:, : kvh * dim].reshape(tokens, kvh, dim)
+        q, s = quantise(rows)
+        want = q * np.repeat(s.astype(np.float64), 64, -1).reshape(rows.shape)
+        assert np.array_equal(c.sequence(name, 0, tokens + 33)[33:], want)
+    assert graph.device_error() == 0
+    graph.release(mark)

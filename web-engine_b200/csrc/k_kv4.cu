@@ -27,7 +27,7 @@ __device__ __forceinline__ int64_t kv4_row(const we_kv4_cache& c, int64_t b, int
 // Rows in and out of the cache. A thread moves 8 values of k or of v a step: 16 bytes (bf16) or 32 on the wide side, a 4-byte
 // word on the packed one, 8 neighbouring lanes a group. It keeps its place within a token (side, head, values) and steps
 // over the tokens of its CTA, whose rows are looked up once, so that a step has little to compute but the values.
-// Measured: 2 x 4099 tokens x 12 heads of 128 in bf16 in 26 us and back in 17 (the bytes of each are 10 us), 16 tokens both
+// Measured: 2 x 4099 tokens x 12 heads of 128 in bf16 in 23 us and back in 17 (the bytes of each are 10 us), 16 tokens both
 // ways 4.7 us; a warp per group and a look-up per value took 167 us.
 constexpr int ROW_THREADS = 256, ROW_SPAN = 32;
 struct RowShape {
@@ -121,8 +121,10 @@ __device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], uint16_t* sca
   return word ^ 0x88888888u;
 }
 
-template <int DT, bool WIDE>
-__global__ void __launch_bounds__(ROW_THREADS) kv4_append_kernel(const we_kv4_cache c, const void* __restrict__ k,
+// PER_SM: CTAs an SM at the least: 6 (in 40 registers) where there are more than two for each SM, 1 (in 56) otherwise. Prompts
+// of 2 x 4099 tokens both ways 40.0 us against 43.6, 16 tokens 4.9 against 4.7.
+template <int DT, bool WIDE, int PER_SM>
+__global__ void __launch_bounds__(ROW_THREADS, PER_SM) kv4_append_kernel(const we_kv4_cache c, const void* __restrict__ k,
                                                                  const void* __restrict__ v, int64_t tokens, int64_t stride,
                                                                  const RowShape z, uint32_t* err) {
   pdl_wait();
@@ -820,8 +822,11 @@ cudaError_t launch_kv4_append(const we_kv4_cache& c, const void* k, const void* 
   const RowPlan p = kv4_rows(c, tokens, sms);
   const int64_t es = dt == WE_F32 ? 4 : 2;
   const bool wide = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | (uintptr_t)(stride * es)) & 15) == 0;
-  const auto kernel = dt == WE_F32 ? (wide ? kv4_append_kernel<WE_F32, true> : kv4_append_kernel<WE_F32, false>)
-                                   : (wide ? kv4_append_kernel<WE_BF16, true> : kv4_append_kernel<WE_BF16, false>);
+  const bool many = (int64_t)p.grid.x * p.grid.y > 2 * sms;
+#define APPEND_CASE(DT, WIDE) (many ? kv4_append_kernel<DT, WIDE, 6> : kv4_append_kernel<DT, WIDE, 1>)
+  const auto kernel = dt == WE_F32 ? (wide ? APPEND_CASE(WE_F32, true) : APPEND_CASE(WE_F32, false))
+                                   : (wide ? APPEND_CASE(WE_BF16, true) : APPEND_CASE(WE_BF16, false));
+#undef APPEND_CASE
   const cudaError_t e = launch_pdl(kernel, p.grid, p.threads, 0, st, c, k, v, tokens, stride, p.shape, err);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
