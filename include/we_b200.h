@@ -413,7 +413,7 @@ int we_kv4_unpack(we_ctx* ctx, const we_kv4_cache* cache, void* k, void* v, int3
 /* Attention of each sequence's `tokens` newest tokens over its cache: query i of sequence b stands at position
    lengths[b] + i and sees keys 0 .. lengths[b] + i, so the step's keys have been appended. q [batch, tokens, heads, dim]
    and out alike (q_stride / out_stride values from a token to the next, 0 = heads * dim); heads a multiple of
-   kv_heads, as we_attention groups them; scale 0 = 1 / sqrt(dim). */
+   kv_heads, as we_attention groups them; scale 0 = 1 / sqrt(dim), else any finite value of either sign. */
 int we_kv4_attention(we_ctx* ctx, const we_kv4_cache* cache, const void* q, int32_t dtype, int64_t tokens,
                      int64_t heads, int64_t q_stride, float scale, void* out, int32_t out_dtype, int64_t out_stride);
 /* lengths[b] += tokens for every sequence that is not idle: the end of a step, after its last layer. */
@@ -425,7 +425,8 @@ int we_kv4_advance(we_ctx* ctx, const we_kv4_cache* cache, int64_t tokens);
    token to the next (0 = contiguous heads; k and v cut out of one fused projection have a larger one); a batch entry's
    tokens follow the previous one's. A key j of entry b is seen when j < key_lengths[b] (device int32, NULL = tk) and
    key_mask[b][j] != 0 (device bytes [batch, tk], NULL = all). A row that sees no key gives zeros; values of unseen keys
-   (NaN included) do not reach the output. scale 0 = 1 / sqrt(dim). dim 1..256, f32 or bf16. */
+   (NaN included) do not reach the output. scale 0 = 1 / sqrt(dim), else any finite value of either sign. dim 1..256, f32 or
+   bf16. */
 typedef struct {
   const void* q;
   const void* k;

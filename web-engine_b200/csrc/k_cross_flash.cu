@@ -41,11 +41,12 @@ struct Params {
   int64_t tq, tk, out_stride, items;
   int kv_heads, group, span, q_tiles, splits;  // group: heads per kv head; span: tokens of an item (span * group rows);
                                                // items = batch * kv_heads * q_tiles; splits: CTAs per item
-  float scale_log2;
+  float scale_log2;  // |scale| log2(e); with a negative scale the scores change sign as they are read
   void* out;
   int out_dtype;
   const int32_t* key_lengths;
   const uint8_t* key_mask;
+  int negative;
   uint32_t* err;
 };
 
@@ -303,6 +304,10 @@ __global__ void __launch_bounds__(cf::THREADS, 2)
         tmem_ld32_async(lane_addr + half * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(sc + 32));
         tmem_wait_ld(*reinterpret_cast<uint32_t(*)[32]>(sc));
         reg_fence(*reinterpret_cast<uint32_t(*)[32]>(sc + 32));
+        if (p.negative) {
+#pragma unroll
+          for (int c = 0; c < 64; c++) sc[c] ^= 0x80000000u;
+        }
         if (!whole) {
 #pragma unroll
           for (int c = 0; c < 32; c++) {
@@ -544,7 +549,7 @@ cudaError_t cross_flash(const we_cross_desc& d, uint32_t* err, int sms, cudaStre
   int splits = 1;
   while (splits < 8 && items * splits * 2 <= 2 * sms - 24 && splits * 2 <= tiles) splits *= 2;
   cf::Params p{d.tq, d.tk, d.out_stride, items, (int)d.kv_heads, group, span, (int)q_tiles, splits,
-               d.scale * 1.4426950408889634f, d.out, d.out_dtype, d.key_lengths, d.key_mask, err};
+               fabsf(d.scale) * 1.4426950408889634f, d.out, d.out_dtype, d.key_lengths, d.key_mask, d.scale < 0.f, err};
   constexpr int bytes = cf::Layout<D>::BYTES;
   const auto kernel = splits > 1 ? cross_flash_kernel<D, true> : cross_flash_kernel<D, false>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);

@@ -265,7 +265,8 @@ struct Params {
   int chunk;                       // keys per CTA at most
   int wide_q;                      // rows of q are 16-byte aligned
   int64_t q_stride, out_stride;
-  float scale_log2;
+  float scale_log2;                // |scale| log2(e); its sign goes to q, so that maxima and hidden scores of -inf hold
+  int negative;
   int dtype, out_dtype;
   float* part;                     // [sequence, kv head, row tile][clusters][8 NQ](dim values, maximum, sum), when more than one
   uint32_t* done;                  // [sequence, kv head, row tile]: clusters that have written, zero between calls
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const uint32_t ex = min(max(__float_as_uint(top) >> 23, 16u), 254u);
-    const float up = __uint_as_float((269u - ex) << 23);
+    const float up = __uint_as_float((269u - ex) << 23 | (uint32_t)p.negative << 31);
     float sum[G];
 #pragma unroll
     for (int g = 0; g < G; g++) {
@@ -917,7 +918,8 @@ cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, void* part, uint32_t* don
   p.wide_q = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * (a.dtype == WE_F32 ? 4 : 2))) & 15) == 0;
   p.q_stride = a.q_stride;
   p.out_stride = a.out_stride;
-  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.scale_log2 = fabsf(a.scale) * 1.4426950408889634f;
+  p.negative = a.scale < 0.f;
   p.dtype = a.dtype;
   p.out_dtype = a.out_dtype;
   p.part = static_cast<float*>(part);

@@ -2,6 +2,7 @@
 // K/V cache and its attention, and cross attention. Argument checks and dispatch; the kernels are in k_matvec.cu,
 // k_kv4.cu and k_cross.cu.
 #include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "common.cuh"
@@ -142,6 +143,7 @@ int we_kv4_attention(we_ctx* ctx, const we_kv4_cache* c, const void* q, int32_t 
   if (tokens < 0 || tokens > 0x7fffffff / heads) return we_ctx_fail(ctx, WE_EINVAL, "kv4: tokens * heads must be in 0..2^31-1");
   if ((q_stride && q_stride < heads * c->dim) || (out_stride && out_stride < heads * c->dim))
     return we_ctx_fail(ctx, WE_EINVAL, "kv4: a token stride is shorter than a token's heads");
+  if (!std::isfinite(scale)) return we_ctx_fail(ctx, WE_EINVAL, "kv4: scale must be finite");
   if (tokens == 0 || c->batch == 0) return WE_OK;
   if (!q || !out) return we_ctx_fail(ctx, WE_EINVAL, "kv4: missing q or out");
   if (!aligned(q, dsize(dtype)) || !aligned(out, dsize(out_dtype)))
@@ -199,6 +201,7 @@ int we_cross_attention(we_ctx* ctx, const we_cross_desc* desc) {
   if ((d.q_stride && d.q_stride < qw) || (d.out_stride && d.out_stride < qw) || (d.k_stride && d.k_stride < kw) ||
       (d.v_stride && d.v_stride < kw))
     return we_ctx_fail(ctx, WE_EINVAL, "cross attention: a token stride is shorter than a token's heads");
+  if (!std::isfinite(d.scale)) return we_ctx_fail(ctx, WE_EINVAL, "cross attention: scale must be finite");
   if (d.batch == 0 || d.tq == 0) return WE_OK;
   if (!d.q || !d.out || (d.tk > 0 && (!d.k || !d.v)))
     return we_ctx_fail(ctx, WE_EINVAL, "cross attention: missing buffer");
