@@ -158,28 +158,34 @@ def attention(graph: Graph, q, k, v, tokens: int, heads: int, kv_heads: int, dim
     return Buffer(out.value, tokens * heads * dim * L.DTYPE_BYTES[L.DTYPES[od]])
 
 
-def matvec(graph: Graph, x, w: Linear, m: int, x_dtype: str = "f32", y_dtype: str = "f32", **kw) -> Buffer:
+def matvec(graph: Graph, x, w: Linear, m: int, x_dtype: str = "f32", y_dtype: str = "f32", *, x_stride=None,
+           x_offset: int = 0, act=None, aux_op=None, aux=None, aux_dtype: str = "f32", gate=None) -> Buffer:
     """y[m, n] = x[m, k] . W^T (+ bias) of 1 to 16 rows (a step's single tokens) with int4 group-64 weights, a new
-    buffer; the fused epilogue keywords of kernels.matvec apply (no reference counterpart)."""
+    buffer of contiguous rows; x's stride and the fused epilogue as in kernels.matvec, which also takes y's layout and
+    accumulates (no reference counterpart)."""
     if w.dtype != "int4" or w.lora is not None:
         raise ValueError("matvec takes an int4 group-64 linear without LoRA")
     from . import kernels as K
 
     out = graph.buffer(m * w.n * L.DTYPE_BYTES[L.DTYPES[y_dtype]])
     K.matvec(graph, x, w.buffer, out, m, w.n, w.k, group_scale=w.group_scale, bias=w.bias, x_dtype=x_dtype,
-             y_dtype=y_dtype, **kw)
+             y_dtype=y_dtype, x_stride=x_stride, x_offset=x_offset, act=act, aux_op=aux_op, aux=aux, aux_dtype=aux_dtype,
+             gate=gate)
     return out
 
 
 def cross_attention(graph: Graph, q, k, v, batch: int, tq: int, tk: int, heads: int, kv_heads: int, dim: int,
-                    dtype: str = "f32", out_dtype: str | None = None, **kw) -> Buffer:
-    """softmax(q k^T / sqrt(dim)) v per head over another sequence's k, v [batch, tk, kv_heads, dim] -> a new
-    [batch, tq, heads, dim] (kernels.cross_attention; no reference counterpart)."""
+                    dtype: str = "f32", out_dtype: str | None = None, *, key_lengths=None, key_mask=None, scale: float = 0.0,
+                    q_stride: int = 0, k_stride: int = 0, v_stride: int = 0) -> Buffer:
+    """softmax(q k^T / sqrt(dim)) v per head over another sequence's k, v [batch, tk, kv_heads, dim] -> a new contiguous
+    [batch, tq, heads, dim] (kernels.cross_attention, which also takes the output's stride; no reference counterpart)."""
     from . import kernels as K
 
     od = out_dtype or dtype
     out = graph.buffer(batch * tq * heads * dim * L.DTYPE_BYTES[L.DTYPES[od]])
-    K.cross_attention(graph, q, k, v, out, batch, tq, tk, heads, kv_heads, dim, dtype=dtype, out_dtype=od, **kw)
+    K.cross_attention(graph, q, k, v, out, batch, tq, tk, heads, kv_heads, dim, dtype=dtype, out_dtype=od,
+                      key_lengths=key_lengths, key_mask=key_mask, scale=scale, q_stride=q_stride, k_stride=k_stride,
+                      v_stride=v_stride)
     return out
 
 
