@@ -51,3 +51,32 @@ def test_cross_attention_op_has_an_output_of_its_own_layout(we, host):
     with pytest.raises(TypeError):
         we.cross_attention(host, 1 << 20, 1 << 20, 1 << 20, 1, 2, 3, 2, 1, 64, out_stride=256)
     assert host.log == []
+
+
+def layer(we, host, cfg, width=None):
+    """Weights of a layer by their shapes alone; width: of the states, None for a layer without cross attention."""
+    def lin(n, k):
+        return we.Linear(host.buffer(n * k // 2), "int4", 1.0, n, k, group_scale=host.buffer(n * k // 32))
+
+    qw, kw = cfg.heads * cfg.head_dim, cfg.kv_heads * cfg.head_dim
+    cross = {} if width is None else {"cross_norm": host.buffer(cfg.hidden * 4), "cross_q": lin(qw, cfg.hidden), "cross_k": lin(kw, width),
+                                      "cross_v": lin(kw, width), "cross_o": lin(cfg.hidden, qw)}
+    return we.decoder.DecoderLayer(host.buffer(cfg.hidden * 4), lin(qw, cfg.hidden), lin(kw, cfg.hidden), lin(kw, cfg.hidden), lin(cfg.hidden, qw),
+                                   host.buffer(256), host.buffer(256), host.buffer(cfg.hidden * 4), lin(cfg.mlp, cfg.hidden),
+                                   lin(cfg.mlp, cfg.hidden), lin(cfg.hidden, cfg.mlp), **cross)
+
+
+def decoder(we, host, batch=3, width=None, layers=1):
+    cfg = we.decoder.DecoderConfig(64, 128, 2, 1, 64, page=16)
+    d = we.decoder.Decoder(host, cfg, [layer(we, host, cfg, width) for _ in range(layers)], batch, 32)
+    host.log.clear()
+    return d
+
+
+@pytest.mark.parametrize("sequence", [-1, -3, 3, 100])
+def test_a_prompt_names_a_sequence_of_the_batch(we, host, sequence):
+    """A negative index would put the page table's row and the length before their buffers."""
+    d = decoder(we, host)
+    with pytest.raises(ValueError, match="sequence must be in 0..2"):
+        d.prompt(sequence, 1 << 20, 4)
+    assert host.log == [] and d.lengths == [0, 0, 0]

@@ -189,6 +189,8 @@ class Decoder:
         holds the last layer's output."""
         g, cfg = self.graph, self.cfg
         self._ready()
+        if not 0 <= sequence < self.batch:
+            raise ValueError(f"sequence must be in 0..{self.batch - 1}, got {sequence}")
         if self.lengths[sequence]:
             raise ValueError(f"sequence {sequence} has {self.lengths[sequence]} tokens already")
         if not 0 < tokens <= self.tokens:
