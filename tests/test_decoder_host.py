@@ -80,3 +80,12 @@ def test_a_prompt_names_a_sequence_of_the_batch(we, host, sequence):
     with pytest.raises(ValueError, match="sequence must be in 0..2"):
         d.prompt(sequence, 1 << 20, 4)
     assert host.log == [] and d.lengths == [0, 0, 0]
+
+
+@pytest.mark.parametrize("lengths", [[], [3], [3, 3], [3, 3, 3, 3], np.array([1, 2])])
+def test_states_have_a_length_for_every_sequence(we, host, lengths):
+    """The kernels read one length of each sequence from the device."""
+    d = decoder(we, host, width=64)
+    with pytest.raises(ValueError, match="one length for each of 3"):
+        d.set_states(1 << 20, 3, lengths)
+    assert host.log == []

@@ -113,6 +113,9 @@ class Decoder:
         g, kw = self.graph, self.cfg.kv_heads * self.cfg.head_dim
         if any(w.cross_k is not None for w in self.layers) and tokens < 1:
             raise ValueError("the layers attend to states: at least one token of them")
+        n = [tokens] * self.batch if lengths is None else [int(v) for v in lengths]
+        if len(n) != self.batch:
+            raise ValueError(f"one length for each of {self.batch} sequences, got {len(n)}")
         self._drop()
         for pair in self._states:
             for b in pair or ():
@@ -131,7 +134,6 @@ class Decoder:
                 pair.append(out)
             self._states.append(tuple(pair))
         self._state_tokens = tokens
-        n = [tokens] * self.batch if lengths is None else list(lengths)
         self._state_lengths = g.buffer(np.asarray(n, np.int32))
 
     # ---- one token of every sequence ----
