@@ -89,3 +89,12 @@ def test_states_have_a_length_for_every_sequence(we, host, lengths):
     with pytest.raises(ValueError, match="one length for each of 3"):
         d.set_states(1 << 20, 3, lengths)
     assert host.log == []
+
+
+@pytest.mark.parametrize("shape", [(4, 64), (1, 64), (3, 65), (0,)])
+def test_a_step_takes_one_embedding_of_every_sequence(we, host, shape):
+    """More values would be copied past the end of the step's buffer, fewer would leave the last step's output in it."""
+    d = decoder(we, host)
+    with pytest.raises(ValueError, match="x must hold 3 x 64 values"):
+        d.step(np.zeros(shape, np.float32))
+    assert host.log == [] and d.lengths == [0, 0, 0]

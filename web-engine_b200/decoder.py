@@ -144,10 +144,14 @@ class Decoder:
         self._ready()
         if max(self.lengths) >= self.tokens:
             raise ValueError(f"a sequence is full ({self.tokens} tokens)")
+        if x is not None:
+            x = np.ascontiguousarray(x, np.float32)
+            if x.size != self.batch * cfg.hidden:
+                raise ValueError(f"x must hold {self.batch} x {cfg.hidden} values, got {x.size}")
         cos, sin, _ = K.rope_tables(np.asarray(self.lengths), (cfg.head_dim,), cfg.theta)
         g.write(self._rope, np.concatenate([cos, sin]))
         if x is not None:
-            g.write(self.x, np.ascontiguousarray(x, np.float32))
+            g.write(self.x, x)
         if self._captured is None:
             with g.capture() as cap:
                 self._layers_of_step()
