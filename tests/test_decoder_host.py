@@ -98,3 +98,22 @@ def test_a_step_takes_one_embedding_of_every_sequence(we, host, shape):
     with pytest.raises(ValueError, match="x must hold 3 x 64 values"):
         d.step(np.zeros(shape, np.float32))
     assert host.log == [] and d.lengths == [0, 0, 0]
+
+
+def test_states_that_fail_half_way_leave_none(we, host, monkeypatch):
+    """The old states are gone by then: a step asks for new ones, and nothing is freed twice or kept."""
+    monkeypatch.setattr(we.kernels, "matmul", lambda *a, **k: None)
+    d = decoder(we, host, width=64, layers=2)
+    owned = set(host.owned)
+    d.set_states(1 << 20, 3)
+    assert len(set(host.owned) - owned) == 5
+    for fail_at in (0, 3, 4):
+        host.fail_at = fail_at
+        with pytest.raises(MemoryError):
+            d.set_states(1 << 20, 5)
+        assert set(host.owned) == owned
+        with pytest.raises(ValueError, match="call set_states first"):
+            d.step(np.zeros((3, 64), np.float32))
+    host.fail_at = None
+    d.set_states(1 << 20, 4, [4, 0, 2])
+    assert len(set(host.owned) - owned) == 5 and d._state_tokens == 4

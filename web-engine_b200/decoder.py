@@ -122,19 +122,24 @@ class Decoder:
                 g.free(b)
         if self._state_lengths is not None:
             g.free(self._state_lengths)
-        self._states = []
-        for w in self.layers:
-            if w.cross_k is None:
-                self._states.append(None)
-                continue
-            pair = []
-            for m in (w.cross_k, w.cross_v):
-                out = g.buffer(self.batch * tokens * kw * 2)
-                self._matmul(states, m, out, self.batch * tokens)
-                pair.append(out)
-            self._states.append(tuple(pair))
-        self._state_tokens = tokens
-        self._state_lengths = g.buffer(np.asarray(n, np.int32))
+        self._states, self._state_lengths = [], None  # (none, should what follows fail)
+        made: list[Buffer] = []
+        try:
+            pairs = []
+            for w in self.layers:
+                if w.cross_k is None:
+                    pairs.append(None)
+                    continue
+                for m in (w.cross_k, w.cross_v):
+                    made.append(g.buffer(self.batch * tokens * kw * 2))
+                    self._matmul(states, m, made[-1], self.batch * tokens)
+                pairs.append((made[-2], made[-1]))
+            of_each = g.buffer(np.asarray(n, np.int32))
+        except BaseException:
+            for b in made:
+                g.free(b)
+            raise
+        self._states, self._state_tokens, self._state_lengths = pairs, tokens, of_each
 
     # ---- one token of every sequence ----
     def step(self, x=None) -> Buffer:
