@@ -117,3 +117,22 @@ def test_states_that_fail_half_way_leave_none(we, host, monkeypatch):
     host.fail_at = None
     d.set_states(1 << 20, 4, [4, 0, 2])
     assert len(set(host.owned) - owned) == 5 and d._state_tokens == 4
+
+
+def test_a_prompt_needs_the_same_memory_whatever_the_layers(we, host, monkeypatch):
+    """The residuals are added in place by the linears: a long prompt takes no new buffers layer by layer."""
+    for name in ("rmsnorm", "matmul", "qknorm_rope", "attention", "cross_attention"):
+        monkeypatch.setattr(we.kernels, name, lambda *a, **k: None)
+    for name in ("append", "unpack", "advance"):
+        monkeypatch.setattr(we.kv4, name, lambda *a, **k: None)
+    monkeypatch.setattr(we.ops, "add", lambda g, x, y, n: g.buffer(n * 4))
+    host.mark, host.release, host.copy = lambda: 0, lambda mark: None, lambda *a: None
+    took = {}
+    for layers in (1, 4):
+        d = decoder(we, host, width=64, layers=layers)
+        d.set_states(1 << 20, 3)
+        host.log.clear()
+        d.prompt(1, 1 << 20, 20)
+        took[layers] = sum(n for what, n in host.log if what == "buffer")
+        assert d.lengths == [0, 20, 0]
+    assert took[1] == took[4]

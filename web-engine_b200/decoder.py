@@ -207,20 +207,14 @@ class Decoder:
         if not 0 < tokens <= self.tokens:
             raise ValueError(f"a prompt has 1 to {self.tokens} tokens, got {tokens}")
         qw, kw = cfg.heads * cfg.head_dim, cfg.kv_heads * cfg.head_dim
+        residual = {"y_dtype": "f32", "accumulate": True}
         mark = g.mark()
         try:
             cos, sin, _ = K.rope_tables(np.arange(tokens), (cfg.head_dim,), cfg.theta)
             cos, sin = g.buffer(cos), g.buffer(sin)
             bf = lambda n: g.buffer(tokens * n * 2)  # noqa: E731
             h, q, k, v, qr, kr, a = bf(cfg.hidden), bf(qw), bf(kw), bf(kw), bf(qw), bf(kw), bf(qw)
-            gate, u, y = bf(cfg.mlp), bf(cfg.mlp), g.buffer(tokens * cfg.hidden * 4)
-            n = tokens * cfg.hidden
-
-            def residual(inp, w):
-                self._matmul(inp, w, y, tokens, y_dtype="f32")
-                add = ops.add(g, x, y, n)
-                g.copy(add, 0, x, 0, n * 4)
-
+            gate, u = bf(cfg.mlp), bf(cfg.mlp)
             for i, w in enumerate(self.layers):
                 cache = self._of(self.caches[i], sequence)
                 self._norm(x, w.norm, tokens, h)
@@ -233,7 +227,7 @@ class Decoder:
                 kv4.unpack(g, cache, k, v, tokens)  # what later tokens will see of these
                 K.attention(g, qr, k, v, tokens, cfg.heads, cfg.kv_heads, cfg.head_dim, a, causal=True, dtype="bf16",
                             out_dtype="bf16")
-                residual(a, w.o)
+                self._matmul(a, w.o, x, tokens, **residual)
                 if w.cross_q is not None:
                     self._norm(x, w.cross_norm, tokens, h)
                     self._matmul(h, w.cross_q, q, tokens)
@@ -241,11 +235,11 @@ class Decoder:
                     ck, cv = (Binding(b, sequence * each, each) for b in self._states[i])
                     K.cross_attention(g, q, ck, cv, a, 1, tokens, self._state_tokens, cfg.heads, cfg.kv_heads, cfg.head_dim,
                                       key_lengths=Binding(self._state_lengths, sequence * 4, 4), dtype="bf16", out_dtype="bf16")
-                    residual(a, w.cross_o)
+                    self._matmul(a, w.cross_o, x, tokens, **residual)
                 self._norm(x, w.mlp_norm, tokens, h)
                 self._matmul(h, w.gate, gate, tokens)
                 self._matmul(h, w.up, u, tokens, aux_op="swiglu", aux=gate, aux_dtype="bf16")
-                residual(u, w.down)
+                self._matmul(u, w.down, x, tokens, **residual)
             if self.caches:
                 kv4.advance(g, self._of(self.caches[0], sequence), tokens)
         finally:
