@@ -93,6 +93,7 @@ __device__ __forceinline__ void merge_parts(float* mem, float* part_base, uint32
   if (runs == 1) return;
   // the last cluster of the unit to get here merges all of its parts, in the order of the runs
   if (rank == 0 && threadIdx.x == 0) {
+    __threadfence();  // behind the barrier: what the whole cluster has written is out before the count says so
     const int is_last = atomicAdd(done + unit, 1u) == (uint32_t)runs - 1u;
     if (is_last) done[unit] = 0u;
     __threadfence();
