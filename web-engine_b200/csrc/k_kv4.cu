@@ -357,12 +357,13 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
       }
   }
 
-  const int have = p.c.lengths[b];
+  const int length = p.c.lengths[b];
   const int64_t room = p.c.max_pages * p.c.page;
-  const int64_t want = (int64_t)have + min(p.tokens, (rtile * QROWS + QROWS - 1) / p.group + 1);  // keys of the tile's last row
+  const int have = (int)min((int64_t)length, room);  // (a length may be any 32 bits; past the table all its keys are seen)
+  const int64_t want = (int64_t)length + min(p.tokens, (rtile * QROWS + QROWS - 1) / p.group + 1);  // keys of the tile's last row
   const int keys = have < 0 ? 0 : (int)min(want, room);
   if (have >= 0 && want > room && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(p.err, 0u, (uint32_t)DEV_ERR_KV_FULL);
-  const int runs = max(1, (keys + CLUSTER * p.chunk - 1) / (CLUSTER * p.chunk));
+  const int runs = max(1, (int)(((uint32_t)keys + CLUSTER * p.chunk - 1) / (uint32_t)(CLUSTER * p.chunk)));
   if (run >= runs) return;  // (the whole cluster)
   const int share = ((keys + runs * CLUSTER - 1) / (runs * CLUSTER) + STEP - 1) / STEP * STEP;  // keys of each CTA
   const int key0 = min(keys, (run * CLUSTER + rank) * share), key1 = min(keys, key0 + share);

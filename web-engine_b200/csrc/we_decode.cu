@@ -26,6 +26,8 @@ namespace {
     we_ctx_count_launch(ctx);                                                                                  \
   } while (0)
 
+// Most keys of a sequence: the kernels count places in 31 bits, up to some thousands past the last key.
+constexpr int64_t MAX_KEYS = 0x7fffffff - (1 << 24);
 bool act_dtype_ok(int dt) { return dt == WE_F32 || dt == WE_BF16; }
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 size_t dsize(int dt) { return dt == WE_F32 ? 4 : 2; }
@@ -41,8 +43,8 @@ int cache_check(we_ctx* ctx, const we_kv4_cache* c) {
     return we_ctx_fail(ctx, WE_EINVAL, "kv4: batch, pages and max_pages must not be negative, kv_heads positive");
   if (c->batch > 65535 || c->kv_heads > 65535)
     return we_ctx_fail(ctx, WE_EINVAL, "kv4: at most 65535 sequences and kv heads");
-  if (c->pages > 0x7fffffff || c->max_pages > 0x7fffffff / c->page)
-    return we_ctx_fail(ctx, WE_EINVAL, "kv4: pages and tokens per sequence must fit 31 bits");
+  if (c->pages > 0x7fffffff || c->max_pages > MAX_KEYS / c->page)
+    return we_ctx_fail(ctx, WE_EINVAL, "kv4: pages must fit 31 bits, tokens per sequence be at most " + std::to_string(MAX_KEYS));
   if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4) ||
       !aligned(c->page_table, 4) || !aligned(c->lengths, 4))
     return we_ctx_fail(ctx, WE_EINVAL, "kv4: k and v must be 16-byte, scales, page table and lengths 4-byte aligned");
@@ -195,8 +197,8 @@ int we_cross_attention(we_ctx* ctx, const we_cross_desc* desc) {
     return we_ctx_fail(ctx, WE_EINVAL, "heads must be a multiple of kvHeads");
   if (d.dim <= 0 || d.dim > 256) return we_ctx_fail(ctx, WE_EINVAL, "dim must be in 1..256");
   if (d.batch < 0 || d.tq < 0 || d.tk < 0) return we_ctx_fail(ctx, WE_EINVAL, "cross attention: negative size");
-  if (d.batch > 65535 || d.heads > 65535 || d.tq > 0x7fffffff || d.tk > 0x7fffffff)
-    return we_ctx_fail(ctx, WE_EINVAL, "cross attention: at most 65535 batch entries and heads, 2^31-1 tokens");
+  if (d.batch > 65535 || d.heads > 65535 || d.tq > MAX_KEYS || d.tk > MAX_KEYS)
+    return we_ctx_fail(ctx, WE_EINVAL, "cross attention: at most 65535 batch entries and heads, " + std::to_string(MAX_KEYS) + " tokens");
   const int64_t qw = d.heads * d.dim, kw = d.kv_heads * d.dim;
   if ((d.q_stride && d.q_stride < qw) || (d.out_stride && d.out_stride < qw) || (d.k_stride && d.k_stride < kw) ||
       (d.v_stride && d.v_stride < kw))
