@@ -243,7 +243,8 @@ __global__ void kv4_advance_kernel(int32_t* lengths, int64_t batch, int32_t toke
 // - f32 q or out (TERMS = 2): q and the weights are two f16 terms each (22 bits), and codes become signed f16 by one more
 //   operation, because the offset's sums would cost 2 bits of a score and, weights being positive, up to 5 of an output.
 // - A warp takes 16 or 32 keys at a time through a ring of its own (cp.async), with its own running maximum; the O and
-//   sums are only rescaled when the maximum grows by more than 2^8 or v's scales outgrow their power of two.
+//   sums are only rescaled when the maximum grows by more than 2^8 or v's scales outgrow their power of two. Values of v of
+//   very different magnitudes take a second sweep with powers for each row and group (sweep()).
 // - A cluster of 8 CTAs shares the keys of a sequence evenly and merges over distributed shared memory; a longer sequence
 //   takes several clusters, whose parts the last one to finish merges. Every merge is in a fixed order.
 namespace kv {
@@ -298,6 +299,14 @@ __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 __device__ __forceinline__ float2 halves(uint32_t u) { return __half22float2(as_half2(u)); }
 
+// 2^(11 - e) (one term; the weights are held times 2^6) or 2^(17 - e) (two) from (31 - e) << 10
+__device__ __forceinline__ float power_up(uint32_t power, int terms) {
+  return __uint_as_float((power << 13) + ((terms == 1 ? 107u : 113u) << 23));
+}
+__device__ __forceinline__ float power_down(uint32_t power, int terms) {  // 1 over it
+  return __uint_as_float(((terms == 1 ? 147u : 141u) << 23) - (power << 13));
+}
+
 // Where the 32 bytes of group g of row `row` (0..15) of a tile lie: so that the rows that lanes read together
 // ({0 4 1 5}, {2 6 3 7} for k, {0 1 2 3}, {4 5 6 7} for v, and 8 more) are on different banks.
 template <int D>
@@ -307,30 +316,11 @@ __device__ __forceinline__ int segment(int row, int g) {
   if (D == 128) return ((row >> 1) * 4 + (row & 1) * 2 + (g ^ (h >> 1))) * 32;
   return (row * 4 + (g ^ h)) * 32;
 }
-}  // namespace kv
-
-// D: dim; NQ: tiles of 8 q rows; KT: tiles of 16 keys of a step; TERMS: f16 terms of q and of the weights.
-template <int D, int NQ, int KT, int TERMS>
-__global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Params p) {
-  using namespace kv;
-  constexpr int G = D / 64, STEP = KT * 16, ROW = D / 2, TILE = 16 * ROW, QROWS = 8 * NQ;
-  constexpr int STAGE = KT * (2 * TILE + 2 * 16 * G * 2), DEPTH = ring_depth<D, KT>();
-  constexpr int MTILES = D / 16;
-  constexpr float UP = TERMS == 1 ? 6.f : 0.f;  // weights are kept times 2^UP
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int last;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3, u = lane >> 2;
-  const int rank = blockIdx.x % CLUSTER, run = blockIdx.x / CLUSTER, b = blockIdx.z;  // CTA of the cluster, run of keys
-  const int head = blockIdx.y / p.row_tiles, rtile = blockIdx.y % p.row_tiles;  // kv head, tile of q rows
-  const int unit = (b * gridDim.y) + blockIdx.y;
-  pdl_launch_dependents();
-  pdl_wait();
-
-  // the page table's row is asked for beside the length, not behind it
-  if (warp == 0 && lane * 32 < p.c.max_pages)
-    asm volatile("prefetch.global.L2 [%0];" ::"l"(p.c.page_table + (int64_t)b * p.c.max_pages + lane * 32));
-  // this lane's q values (see below) come first: they need no length
-  uint4 q_raw[NQ][G][4];
+// This lane's values of q: 16 of each group of the rows nq * 8 + lane / 4 of its tile.
+template <int D, int NQ>
+__device__ __forceinline__ void load_q(const Params& p, int b, int head, int rtile, uint4 (&q_raw)[NQ][D / 64][4]) {
+  constexpr int G = D / 64, QROWS = 8 * NQ;
+  const int c = threadIdx.x & 3, u = (threadIdx.x >> 2) & 7;
 #pragma unroll
   for (int nq = 0; nq < NQ; nq++) {
     const int r = rtile * QROWS + nq * 8 + u;
@@ -356,17 +346,39 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
         q_raw[nq][g][j] = make_uint4(w[0], w[1], w[2], w[3]);
       }
   }
+}
 
-  const int length = p.c.lengths[b];
-  const int64_t room = p.c.max_pages * p.c.page;
-  const int have = (int)min((int64_t)length, room);  // (a length may be any 32 bits; past the table all its keys are seen)
-  const int64_t want = (int64_t)length + min(p.tokens, (rtile * QROWS + QROWS - 1) / p.group + 1);  // keys of the tile's last row
-  const int keys = have < 0 ? 0 : (int)min(want, room);
-  if (have >= 0 && want > room && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(p.err, 0u, (uint32_t)DEV_ERR_KV_FULL);
-  const int runs = max(1, (int)(((uint32_t)keys + CLUSTER * p.chunk - 1) / (uint32_t)(CLUSTER * p.chunk)));
-  if (run >= runs) return;  // (the whole cluster)
-  const int share = ((keys + runs * CLUSTER - 1) / (runs * CLUSTER) + STEP - 1) / STEP * STEP;  // keys of each CTA
-  const int key0 = min(keys, (run * CLUSTER + rank) * share), key1 = min(keys, key0 + share);
+// What a warp's keys give its tile of q rows.
+template <int D, int NQ>
+struct Part {
+  float o[NQ][D / 16][4], w_sum[NQ][D / 64][4];  // O, and the sums of weights (times 8: the codes' offset) by groups
+  float down[NQ][D / 64][2];                     // what O is to be multiplied by
+  float m[NQ][2], l[NQ][2];
+};
+
+// One sweep over this warp's keys.
+// EXACT false: the weights times scales of v, and O, are held over ONE power of two, that of the largest scale so far. With
+// scales down to 2^-RANGE of that a row's largest product is at least 2^-5 (TERMS 2: 2^-2) and every other is within 2^-11 (2^-22)
+// of itself or an absolute 2^-25. A smaller scale, or one that is not finite, ends the sweep (false), and the CTA begins again:
+// EXACT: every row and group has a power of its own, by the largest product of a weight and a scale that it has met, so that a
+// key of large values to which a row gives no weight takes no bits from the row's other keys (with one power for all, values
+// 10^7 below such a key's came out as zeros, or with a few bits in f32).
+// Choosing between the two step by step cost every call 5% (16 sequences of 3001 to 16384 keys, 48 heads on 12: 68.4 us against
+// 65.0); the check of the range and the code beside it cost it nothing, a call of one short sequence 0.2 us of 6.2. Values that
+// need the second sweep take about twice the time. (256-wide heads with more than 8 rows, which spilled before, lost 6%: 8 tokens of
+// 32 heads on 8, 4 x 4000 keys, 62.7 us against 58.9.)
+template <int D, int NQ, int KT, int TERMS, bool EXACT>
+__device__ __forceinline__ bool sweep(const Params& p, int b, int head, int rtile, int have, int key0, int key1, uint8_t* smem,
+                                      const uint4 (&q_raw)[NQ][D / 64][4], Part<D, NQ>& part) {
+  constexpr int G = D / 64, STEP = KT * 16, ROW = D / 2, TILE = 16 * ROW, QROWS = 8 * NQ;
+  constexpr int STAGE = KT * (2 * TILE + 2 * 16 * G * 2), DEPTH = ring_depth<D, KT>();
+  constexpr int MTILES = D / 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3, u = lane >> 2;
+  float(&o)[NQ][MTILES][4] = part.o;
+  float(&w_sum)[NQ][G][4] = part.w_sum;
+  float(&down)[NQ][G][2] = part.down;
+  float(&m)[NQ][2] = part.m;
+  float(&l)[NQ][2] = part.l;
 
   // this warp's steps: key0 + (warp + WARPS i) STEP
   const int steps = (key1 - key0 + STEP - 1) / STEP;
@@ -387,12 +399,13 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
       else at16 = ((uint32_t)id * (uint32_t)p.c.kv_heads + head) * (uint32_t)(page / 16) + (key - slot * page) / 16;
     }
   };
-  uint32_t copy_to[TILE / 512];  // where a lane's 16-byte pieces of a tile go
-#pragma unroll
-  for (int j = 0; j < TILE / 512; j++) {
+  auto piece_to = [&](int j) {  // where a lane's j-th 16-byte piece of a tile goes
     const int at = j * 32 + lane, r = at / (ROW / 16), ch = at % (ROW / 16);  // piece `ch` of row r
-    copy_to[j] = segment<D>(r, ch >> 1) + (ch & 1) * 16;
-  }
+    return segment<D>(r, ch >> 1) + (ch & 1) * 16;
+  };
+  uint32_t copy_to[D == 128 ? 1 : TILE / 512];  // (dim 128: 8 rows on is 512 bytes on)
+#pragma unroll
+  for (int j = 0; j < (D == 128 ? 1 : TILE / 512); j++) copy_to[j] = piece_to(j);
   uint32_t there = 0;  // bit per tile of the ring's stages: its page exists
   auto copy = [&](int i) {
     if (i < mine) {
@@ -410,7 +423,7 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
         for (int side = 0; side < 2; side++) {
           const uint8_t* from = (side ? p.c.v : p.c.k) + (uint64_t)at * TILE + lane * 16;
 #pragma unroll
-          for (int j = 0; j < TILE / 512; j++) cp_async16(to + (t * 2 + side) * TILE + copy_to[j], from + j * 512);
+          for (int j = 0; j < TILE / 512; j++) cp_async16(to + (t * 2 + side) * TILE + (D == 128 ? copy_to[0] + j * 512 : copy_to[j]), from + j * 512);
         }
         // scales: 4-byte words, 8 G of k then 8 G of v
 #pragma unroll
@@ -495,7 +508,30 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
     }
   }
 
-  float o[NQ][MTILES][4], w_sum[NQ][G][4], m[NQ][2], l[NQ][2];
+  uint32_t low = 0x000f000fu, high = 0x00f000f0u;  // in registers: a pair of codes is one operation with its other constant
+  asm volatile("" : "+r"(low), "+r"(high));
+  const __half2 sub1 = __float2half2_rn(-1032.f), sub16 = __float2half2_rn(-1152.f);
+  const int full = have + (rtile * QROWS) / p.group + 1;  // keys below are seen by every row of the tile
+
+  // offsets of this lane's pieces of a tile: for k words 2 c, 2 c + 1 of a group of its key and (+ 8 rows) the other; for v
+  // word u of the keys of rows 2 c and (+ 8 rows) 2 c + 8, and of rows 2 c + 1 and 2 c + 9
+  const int k0 = (u >> 1) + 4 * (u & 1);  // row r of a tile of S^T is key r / 2 + 4 (r & 1) (+ 8)
+  int k_at[G], v_at[G], v_next = 0;
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    k_at[g] = segment<D>(k0, g) + c * 8;
+    v_at[g] = TILE + segment<D>(c, g) + u * 4;
+  }
+  if (D == 64) v_next = TILE + segment<D>(c + 4, 0) + u * 4;
+  // row c + 4 (dim 128: as segment() puts it, the other group's place of row c and 256 bytes on)
+  auto v_at_4 = [&](int g) { return D == 64 ? v_next : D == 128 ? v_at[g ^ 1] + 256 : TILE + segment<D>(c + 4, g) + u * 4; };
+  const int s_at = KT * 2 * TILE + k0 * (2 * G);
+
+  constexpr uint32_t RANGE = TERMS == 1 ? 10 : 7;
+  // EXACT: scales of v are kept times 2^(11 - e) (TERMS 2: 2^(17 - e)), e a row's and group's power as an f16 exponent: for scales
+  // up to 2^ABOVE above it and weights of up to 2^8 the products stay below 2^15.
+  constexpr int ABOVE = 4;
+  constexpr float UP = TERMS == 1 ? 6.f : 0.f;  // weights are kept times 2^UP
 #pragma unroll
   for (int nq = 0; nq < NQ; nq++) {
 #pragma unroll
@@ -505,24 +541,18 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
     m[nq][0] = m[nq][1] = NONE;
     l[nq][0] = l[nq][1] = 0.f;
   }
-  uint32_t v_top = 1u << 10;  // the largest scale of v so far, as f16 bits (at least the smallest normal one)
-  uint32_t low = 0x000f000fu, high = 0x00f000f0u;  // in registers: a pair of codes is one operation with its other constant
-  asm volatile("" : "+r"(low), "+r"(high));
-  const __half2 sub1 = __float2half2_rn(-1032.f), sub16 = __float2half2_rn(-1152.f);
-  const int full = have + (rtile * QROWS) / p.group + 1;  // keys below are seen by every row of the tile
-
-  // offsets of this lane's pieces of a tile: for k words 2 c, 2 c + 1 of a group of its key and (+ 8 rows) the other; for v
-  // word u of the keys of rows 2 c and (+ 8 rows) 2 c + 8, and of rows 2 c + 1 and 2 c + 9
-  const int k0 = (u >> 1) + 4 * (u & 1);  // row r of a tile of S^T is key r / 2 + 4 (r & 1) (+ 8)
-  int k_at[G], v_at[2][G];
+  // scales of v, as f16 bits, that need no change: up to the upper half (whose exponent field is O's power: that of the
+  // largest scale so far, at least 1), and from the lower half on
+  uint32_t v_range = 0x07ff0000u;
+  // power[nq][g]: (31 - e) << 10 of this lane's two columns, e in 1..30.
+  // limit: the scales of v, as f16 bits of two groups a word, up to which no power has to move
+  uint32_t power[NQ][G], limit[(G + 1) / 2];
 #pragma unroll
-  for (int g = 0; g < G; g++) {
-    k_at[g] = segment<D>(k0, g) + c * 8;
-    v_at[0][g] = TILE + segment<D>(c, g) + u * 4;
-    v_at[1][g] = TILE + segment<D>(c + 4, g) + u * 4;
-  }
-  const int s_at = KT * 2 * TILE + k0 * (2 * G);
-
+  for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+    for (int g = 0; g < G; g++) power[nq][g] = 0x78007800u;
+#pragma unroll
+  for (int g = 0; g < (G + 1) / 2; g++) limit[g] = 0x17ff17ffu;  // e = 1 + ABOVE
   for (int i = 0; i < mine; i++) {
     copy(i + DEPTH - 1);
     cp_async_wait<DEPTH - 1>();
@@ -623,49 +653,158 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
         mt[nq][k] = x * q_back[nq][k];
         grow = grow || mt[nq][k] > m[nq][k] + 8.f;
       }
-    uint32_t vt = 0;
+    if constexpr (EXACT) {
+      uint32_t vt[(G + 1) / 2];
+      bool large = false;
 #pragma unroll
-    for (int t = 0; t < KT; t++)
+      for (int g = 0; g < (G + 1) / 2; g++) {
+        vt[g] = 0;
 #pragma unroll
-      for (int h = 0; h < 2; h++)
+        for (int t = 0; t < KT; t++)
 #pragma unroll
-        for (int g = 0; g < (G + 1) / 2; g++) vt = __vmaxu2(vt, vs[t][h][g] & 0x7fff7fffu);
-    vt = max(vt & 0xffffu, vt >> 16);
-    if (__any_sync(0xffffffffu, grow || vt > (v_top | 0x3ffu))) {
-      // O and the sums of weights are kept over 2^(exponent of the largest scale)
-      vt = max(__reduce_max_sync(0xffffffffu, vt), v_top);
-      const float f = __uint_as_float((127u + (v_top >> 10) - (vt >> 10)) << 23);
-      v_top = vt;
+          for (int h = 0; h < 2; h++) vt[g] = __vmaxu2(vt[g], vs[t][h][g] & 0x7fff7fffu);
+        large = large || __vmaxu2(vt[g], limit[g]) != limit[g];
+      }
+      if (__any_sync(0xffffffffu, grow || large)) {
+        int least[G], most[G];  // the lowest power of the warp's columns, the exponent of the step's largest scale
+        uint32_t top[NQ][G];    // both columns' largest product of a weight and a scale in the step, upper halves of f32
+        float old[NQ][2];       // what the maximum's growth takes from a column, as a factor and (at most that) as a power
+        int drop[NQ][2];
+        // (all columns side by side, so that their exchanges overlap)
 #pragma unroll
-      for (int nq = 0; nq < NQ; nq++) {
-        float corr[2];
+        for (int away = 4; away <= 16; away *= 2)
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-          float x = mt[nq][k];
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          corr[k] = 1.f;
-          if (x > m[nq][k]) {
-            corr[k] = ex2_ftz(m[nq][k] - x);
-            m[nq][k] = x;
+          for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) mt[nq][k] = fmaxf(mt[nq][k], __shfl_xor_sync(0xffffffffu, mt[nq][k], away));
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) {
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            const float now = fmaxf(mt[nq][k], m[nq][k]);
+            old[nq][k] = now > m[nq][k] ? ex2_ftz(m[nq][k] - now) : 1.f;
+            drop[nq][k] = now > m[nq][k] ? (int)fminf(now - m[nq][k], 64.f) : 0;
+            m[nq][k] = now;
+            l[nq][k] *= old[nq][k];
           }
-          l[nq][k] *= corr[k];
-          corr[k] *= f;
+          uint32_t of[G][2] = {};
+#pragma unroll
+          for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const float p = ex2_ftz(fmaf(s[t][nq][e], q_back[nq][e & 1], -m[nq][e & 1]));
+#pragma unroll
+              for (int g = 0; g < G; g++) {
+                const uint32_t raw = vs[t][e >> 1][g / 2];
+                const float sv = __half2float(__ushort_as_half((uint16_t)((g & 1) ? raw >> 16 : raw)));
+                of[g][e & 1] = max(of[g][e & 1], p > 0.f ? __float_as_uint(p * sv) & 0x7fffffffu : 0u);
+              }
+            }
+#pragma unroll
+          for (int g = 0; g < G; g++) top[nq][g] = __byte_perm(of[g][0], of[g][1], 0x7632);
         }
 #pragma unroll
-        for (int t = 0; t < MTILES; t++)
+        for (int away = 4; away <= 16; away *= 2)
 #pragma unroll
-          for (int e = 0; e < 4; e++) o[nq][t][e] *= corr[e & 1];
+          for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
-        for (int g = 0; g < G; g++)
+            for (int g = 0; g < G; g++) top[nq][g] = __vmaxu2(top[nq][g], __shfl_xor_sync(0xffffffffu, top[nq][g], away));
 #pragma unroll
-          for (int e = 0; e < 4; e++) w_sum[nq][g][e] *= corr[e & 1];
+        for (int g = 0; g < G; g++) most[g] = (int)(__reduce_max_sync(0xffffffffu, (g & 1) ? vt[g / 2] >> 16 : vt[g / 2] & 0xffffu) >> 10);
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          least[g] = 30;
+#pragma unroll
+          for (int nq = 0; nq < NQ; nq++) {
+            float corr[2];
+            uint32_t field = 0;
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              // the exponent that the largest product needs, as a scale's: with up to 2^ABOVE of room for larger scales
+              const int need = (int)((top[nq][g] >> (16 * k + 7)) & 255u) - 112, had = 31 - (int)((power[nq][g] >> (16 * k + 10)) & 31u);
+              const int now = min(max(max(had - drop[nq][k], max(need, min(most[g], need + ABOVE))), 1), 30);
+              least[g] = min(least[g], now);
+              corr[k] = old[nq][k] * __uint_as_float((uint32_t)(127 + had - now) << 23);
+              field |= (uint32_t)(31 - now) << (16 * k + 10);
+            }
+            power[nq][g] = field;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+#pragma unroll
+              for (int t = 0; t < 4; t++) o[nq][g * 4 + t][e] *= corr[e & 1];
+              w_sum[nq][g][e] *= corr[e & 1];
+            }
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          // (scales of NaN and infinities always pass the limit)
+          const int upto = min(__reduce_min_sync(0xffffffffu, least[g]) + ABOVE, 30);
+          const uint32_t bits = (uint32_t)upto << 10 | 0x3ffu;
+          limit[g / 2] = (g & 1) ? (limit[g / 2] & 0xffffu) | bits << 16 : bits;
+        }
+      }
+    } else {
+      uint32_t vt = 0, vb = 0xffffffffu;
+#pragma unroll
+      for (int t = 0; t < KT; t++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int g = 0; g < (G + 1) / 2; g++) {
+            vt = G == 1 ? max(vt, vs[t][h][g]) : __vmaxu2(vt, vs[t][h][g]);
+            vb = G == 1 ? min(vb, vs[t][h][g]) : __vminu2(vb, vs[t][h][g]);
+          }
+      if (G > 1) vt = max(vt & 0xffffu, vt >> 16), vb = min(vb & 0xffffu, vb >> 16);
+      if (__any_sync(0xffffffffu, grow || vt > v_range >> 16 || vb < (v_range & 0xffffu))) {
+        // O and the sums of weights are kept over 2^(exponent of the largest scale)
+        const uint32_t had = v_range >> 26, top = max(__reduce_max_sync(0xffffffffu, vt), had << 10), e = top >> 10;
+        // the smallest scale that is held well beside it: 2^-RANGE of it (smaller ones before it are in O, in f32)
+        const uint32_t least = e > RANGE ? top - (RANGE << 10) : 0x400u >> min(RANGE + 1u - e, 11u);
+        v_range = (top | 0x3ffu) << 16 | least;
+        bool small = false;  // (zeros are no values)
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+              const uint32_t bits = (g & 1) ? vs[t][h][g / 2] >> 16 : vs[t][h][g / 2] & 0xffffu;
+              small = small || (bits != 0 && bits < least);
+            }
+        if (top >= 0x7c00u || __any_sync(0xffffffffu, small)) return false;  // (a negative scale is one of the former)
+        const float f = __uint_as_float((127u + had - e) << 23);
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) {
+          float corr[2];
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            float x = mt[nq][k];
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            corr[k] = 1.f;
+            if (x > m[nq][k]) {
+              corr[k] = ex2_ftz(m[nq][k] - x);
+              m[nq][k] = x;
+            }
+            l[nq][k] *= corr[k];
+            corr[k] *= f;
+          }
+#pragma unroll
+          for (int t = 0; t < MTILES; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[nq][t][e] *= corr[e & 1];
+#pragma unroll
+          for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) w_sum[nq][g][e] *= corr[e & 1];
+        }
       }
     }
     // scales of v times 2^(15 - e) (TERMS 2: 2^(21 - e)), e the exponent field of the largest: below 2, so that a weight of
     // 2^(8 + UP) at most times it stays below 2^15 (2^15)
-    const float v_up = __uint_as_float((148u - (v_top >> 10)) << 23);
+    const float v_up = __uint_as_float((148u - (v_range >> 26)) << 23);
     const __half2 v_up2 = __float2half2_rn(v_up * 0.015625f);
 #pragma unroll
     for (int t = 0; t < KT; t++) {
@@ -681,7 +820,7 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
       // TERMS 1: weights and scales as f16, their products rounded once more (2^-11 each)
       __half2 ph[NQ][2];
       uint32_t vn[2][(G + 1) / 2];
-      if constexpr (TERMS == 1) {
+      if constexpr (TERMS == 1 && !EXACT) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
 #pragma unroll
@@ -696,20 +835,30 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
         uint32_t bw[NQ][TERMS][2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          if constexpr (TERMS == 1) {
+          if constexpr (TERMS == 1 && !EXACT) {
             const __half2 both = as_half2(vn[h][g / 2]), sv = (g & 1) ? __high2half2(both) : __low2half2(both);
 #pragma unroll
             for (int nq = 0; nq < NQ; nq++) bw[nq][0][h] = transposed(as_u32(__hmul2(ph[nq][h], sv)));
           } else {
             const uint32_t raw = vs[t][h][g / 2];
-            const float sv = __half2float(__ushort_as_half((uint16_t)((g & 1) ? raw >> 16 : raw))) * v_up;
+            const float sv = __half2float(__ushort_as_half((uint16_t)((g & 1) ? raw >> 16 : raw)));
 #pragma unroll
             for (int nq = 0; nq < NQ; nq++) {
-              const float x0 = pw[nq][h * 2] * sv, x1 = pw[nq][h * 2 + 1] * sv;
+              float x0, x1;
+              if constexpr (EXACT) {  // (a scale of NaN is its key's rows' alone)
+                x0 = s[t][nq][h * 2] == -INFINITY ? 0.f : pw[nq][h * 2] * (sv * power_up(power[nq][g] & 0xffffu, TERMS));
+                x1 = s[t][nq][h * 2 + 1] == -INFINITY ? 0.f : pw[nq][h * 2 + 1] * (sv * power_up(power[nq][g] >> 16, TERMS));
+              } else {
+                x0 = pw[nq][h * 2] * (sv * v_up), x1 = pw[nq][h * 2 + 1] * (sv * v_up);
+              }
               const __half2 v = __floats2half2_rn(x0, x1);
+              if constexpr (TERMS == 1) {
+                bw[nq][0][h] = transposed(as_u32(v));
+                continue;
+              }
               const float2 f = __half22float2(v);
               bw[nq][0][h] = transposed(as_u32(v));
-              bw[nq][1][h] = transposed(as_u32(__floats2half2_rn(x0 - f.x, x1 - f.y)));
+              bw[nq][TERMS - 1][h] = transposed(as_u32(__floats2half2_rn(x0 - f.x, x1 - f.y)));
             }
           }
         }
@@ -719,10 +868,10 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
           for (int nq = 0; nq < NQ; nq++) mma_f16(w_sum[nq][g], ones, bw[nq][0][0], bw[nq][0][1]);
         }
         // v: word u (dims 8 u .. 8 u + 7 of the group) of the keys of rows 2 c, 2 c + 1, 2 c + 8, 2 c + 9
-        const uint32_t v0 = *reinterpret_cast<const uint32_t*>(kt + v_at[0][g]);
-        const uint32_t v1 = *reinterpret_cast<const uint32_t*>(kt + v_at[1][g]);
-        const uint32_t v2 = *reinterpret_cast<const uint32_t*>(kt + v_at[0][g] + 8 * ROW);
-        const uint32_t v3 = *reinterpret_cast<const uint32_t*>(kt + v_at[1][g] + 8 * ROW);
+        const uint32_t v0 = *reinterpret_cast<const uint32_t*>(kt + v_at[g]);
+        const uint32_t v1 = *reinterpret_cast<const uint32_t*>(kt + v_at_4(g));
+        const uint32_t v2 = *reinterpret_cast<const uint32_t*>(kt + v_at[g] + 8 * ROW);
+        const uint32_t v3 = *reinterpret_cast<const uint32_t*>(kt + v_at_4(g) + 8 * ROW);
 #pragma unroll
         for (int h = 0; h < 2; h++) {  // dims 8 u + 4 h ..
           const uint32_t x = __byte_perm(v0, v1, h ? 0x7632 : 0x5410), y = __byte_perm(v2, v3, h ? 0x7632 : 0x5410);
@@ -749,36 +898,79 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
     }
     __syncwarp();  // every lane has read the stage that is copied into next
   }
+#pragma unroll
+  for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int k = 0; k < 2; k++)  // (2^-(15 - e), 2^-(21 - e) in a first sweep)
+        down[nq][g][k] = EXACT ? power_down((power[nq][g] >> (16 * k)) & 0xffffu, TERMS)
+                               : __uint_as_float(((v_range >> 26) + (TERMS == 1 ? 112u : 106u)) << 23);
+  return true;
+}
+
+// What a CTA does: its share of the keys of a sequence, for one tile of q rows of a kv head, and its part of the merge.
+// D: dim; NQ: tiles of 8 q rows; KT: tiles of 16 keys of a step; TERMS: f16 terms of q and of the weights.
+template <int D, int NQ, int KT, int TERMS, bool EXACT>
+__device__ __forceinline__ void attend_tile(const Params& p) {
+  constexpr int STEP = KT * 16, QROWS = 8 * NQ, MTILES = D / 16, PITCH = MERGE_PITCH<D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3, u = lane >> 2;
+  const int rank = blockIdx.x % CLUSTER, run = blockIdx.x / CLUSTER, b = blockIdx.z;  // CTA of the cluster, run of keys
+  const int head = blockIdx.y / p.row_tiles, rtile = blockIdx.y % p.row_tiles;  // kv head, tile of q rows
+  const int unit = (b * gridDim.y) + blockIdx.y;
+
+  // the page table's row is asked for beside the length, not behind it
+  if (warp == 0 && lane * 32 < p.c.max_pages)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(p.c.page_table + (int64_t)b * p.c.max_pages + lane * 32));
+  // this lane's q values (see below) come first: they need no length
+  uint4 q_raw[NQ][D / 64][4];
+  load_q<D, NQ>(p, b, head, rtile, q_raw);
+
+  const int length = p.c.lengths[b];
+  const int64_t room = p.c.max_pages * p.c.page;
+  const int have = (int)min((int64_t)length, room);  // (a length may be any 32 bits; past the table all its keys are seen)
+  const int64_t want = (int64_t)length + min(p.tokens, (rtile * QROWS + QROWS - 1) / p.group + 1);  // keys of the tile's last row
+  const int keys = have < 0 ? 0 : (int)min(want, room);
+  if (have >= 0 && want > room && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(p.err, 0u, (uint32_t)DEV_ERR_KV_FULL);
+  const int runs = max(1, (int)(((uint32_t)keys + CLUSTER * p.chunk - 1) / (uint32_t)(CLUSTER * p.chunk)));
+  if (run >= runs) return;  // (the whole cluster)
+  const int share = ((keys + runs * CLUSTER - 1) / (runs * CLUSTER) + STEP - 1) / STEP * STEP;  // keys of each CTA
+  const int key0 = min(keys, (run * CLUSTER + rank) * share), key1 = min(keys, key0 + share);
 
   // The warps' O, maxima and sums, merged in shared memory (the rings are done): [warp][row](D values, m, l)
-  cp_async_wait<0>();
-  __syncthreads();
-  constexpr int PITCH = MERGE_PITCH<D>;
   float* mem = reinterpret_cast<float*>(smem);
-  const float v_down = __uint_as_float(((v_top >> 10) + (TERMS == 1 ? 112u : 106u)) << 23);  // 2^-(15 - e), 2^-(21 - e)
+  Part<D, NQ> part;
+  const bool done = sweep<D, NQ, KT, TERMS, EXACT>(p, b, head, rtile, have, key0, key1, smem, q_raw, part);
+  cp_async_wait<0>();
+  if (__builtin_expect(__syncthreads_or(!done), 0)) {
+    if constexpr (!EXACT) attend_tile<D, NQ, KT, TERMS, true>(p);
+    return;
+  }
 #pragma unroll
   for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-      float sum = l[nq][k];
+      float sum = part.l[nq][k];
       sum += __shfl_xor_sync(0xffffffffu, sum, 4);
       sum += __shfl_xor_sync(0xffffffffu, sum, 8);
       sum += __shfl_xor_sync(0xffffffffu, sum, 16);
       float* to = mem + (warp * QROWS + nq * 8 + c * 2 + k) * PITCH;
 #pragma unroll
       for (int t = 0; t < MTILES; t++) {  // group t / 4, dims 8 u + 2 (t % 4) and the next
-        float x0 = o[nq][t][k], x1 = o[nq][t][2 + k];
+        float x0 = part.o[nq][t][k], x1 = part.o[nq][t][2 + k];
         if constexpr (TERMS == 1) {
-          const float off = 8.f * w_sum[nq][t / 4][k];
+          const float off = 8.f * part.w_sum[nq][t / 4][k];
           x0 = fmaf(x0, 16777216.f, -off);
           x1 = fmaf(x1, 1048576.f, -off);
         } else {
           x1 *= 0.0625f;
         }
-        *reinterpret_cast<float2*>(to + (t / 4) * 64 + u * 8 + (t % 4) * 2) = make_float2(x0 * v_down, x1 * v_down);
+        *reinterpret_cast<float2*>(to + (t / 4) * 64 + u * 8 + (t % 4) * 2) = make_float2(x0 * part.down[nq][t / 4][k], x1 * part.down[nq][t / 4][k]);
       }
       if (u == 0) {
-        to[D] = m[nq][k];
+        to[D] = part.m[nq][k];
         to[D + 1] = sum;
       }
     }
@@ -796,6 +988,15 @@ __global__ void __launch_bounds__(kv::THREADS) kv4_attention_kernel(const kv::Pa
     }
   };
   merge_parts<D, QROWS, WARPS, CLUSTER>(mem, p.part, p.done, &last, unit, (int)gridDim.x / CLUSTER, runs, run, rank, finish);
+}
+}  // namespace kv
+
+// PER_SM: CTAs that an SM holds by their registers.
+template <int D, int NQ, int KT, int TERMS, int PER_SM>
+__global__ void __launch_bounds__(kv::THREADS, PER_SM) kv4_attention_kernel(const __grid_constant__ kv::Params p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  kv::attend_tile<D, NQ, KT, TERMS, false>(p);
 }
 
 // How rows are cut: a token over as many threads as it has units, evenly over several rounds of at most ROW_THREADS (over
@@ -874,9 +1075,17 @@ Kv4Plan kv4_plan(const Kv4AttnArgs& a, int sms) {
   return q;
 }
 
-template <int D, int NQ, int KT, int TERMS>
+// CTAs an SM by registers. f32: three (4 sequences of 16000 keys, 48 heads of 128 on 12, took 52 us with four and take 40). bf16:
+// four, for which 128-wide heads spill 16 bytes; calls of so few CTAs that three an SM hold them do better with three (2
+// sequences of 4096 keys, 8 heads: 10.4 us against 12.5; 16 of 3001 to 16384, 48 on 12: 75.1 against 65.3).
+template <int D, int NQ, int TERMS>
+constexpr int per_sm() {
+  return D * NQ == 512 ? 1 : D * NQ == 256 ? 2 : TERMS == 2 ? 3 : 4;
+}
+
+template <int D, int NQ, int KT, int TERMS, int PER_SM = per_sm<D, NQ, TERMS>()>
 cudaError_t kv4_launch(const kv::Params& p, dim3 grid, cudaStream_t st) {
-  auto kern = kv4_attention_kernel<D, NQ, KT, TERMS>;
+  auto kern = kv4_attention_kernel<D, NQ, KT, TERMS, PER_SM>;
   constexpr int ring = kv::WARPS * kv::ring_depth<D, KT>() * KT * (D * 16 + D);
   constexpr int merge = (kv::WARPS + 1) * 8 * NQ * (D + 4) * 4;
   constexpr int bytes = ring > merge ? ring : merge;
@@ -933,6 +1142,7 @@ cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, void* part, uint32_t* don
   e = f32 ? (q.nq == 1 ? kv4_launch<D, 1, 1, 2>(p, grid, st) : kv4_launch<D, 2, 1, 2>(p, grid, st))             \
           : (q.nq == 1 ? kv4_launch<D, 1, D == 256 ? 1 : 2, 1>(p, grid, st) : kv4_launch<D, 2, 1, 1>(p, grid, st))
   if (a.c.dim == 64) KV4_CASE(64);
+  else if (a.c.dim == 128 && !f32 && q.nq == 1 && (int64_t)grid.x * grid.y * grid.z <= 3 * sms - 24) e = kv4_launch<128, 1, 2, 1, 3>(p, grid, st);
   else if (a.c.dim == 128) KV4_CASE(128);
   else KV4_CASE(256);
 #undef KV4_CASE
