@@ -385,7 +385,8 @@ int we_matvec(we_ctx* ctx, const we_matmul_desc* desc, const void* x, const void
 /* ---------------- single tokens: a paged 4-bit K/V cache (no reference counterpart) ----------------
    One layer's cache: every (token, kv head) row of `dim` values is WE_INT4G64, i.e. two's complement codes packed two
    per byte (low nibble = even value) and one f16 scale per 64 values: s = f16(max|x| / 7), at most 65504, and
-   q = clamp(rint(x / s), -8, 7), 0 where s is 0. Rows live in pages of `page` tokens, laid out
+   q = clamp(rint(x / s), -8, 7), 0 where s is 0; a NaN makes its group's scale NaN, and so its values where they are
+   read. Rows live in pages of `page` tokens, laid out
    [pages, kv_heads, page, dim / 2] (scales [pages, kv_heads, page, dim / 64]); token t of sequence b is row t % page
    of page page_table[b][t / page]. `lengths` holds each sequence's tokens BEFORE the current step; all three arrays
    are read on the device, in stream order. A negative length marks an idle sequence: nothing is written for it and its

@@ -49,11 +49,6 @@ __device__ __forceinline__ void find_rows(const we_kv4_cache& c, int64_t* rows, 
   rows[threadIdx.x] = row < 0 ? row : row << head_shift;
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
 __device__ __forceinline__ float rcp_approx(float x) {  // to 1 ulp
   float d;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
@@ -64,23 +59,33 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {  // keeps
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 
 // The codes of 8 values, 8 lanes to a group of 64, and the group's scale: s = f16(max|x| / 7), q = rint(x / s) in -8..7.
 // The first division is by a constant: q + (a - 7 q) / 7 with q = a / 7 to a rounding is the rounded quotient (Markstein).
 // For the second, x (1 / s) added to 1.5 2^23 is rounded to an integer q, the quotient's own rounding unless |x - q s| is
 // within 2e-6 s of s / 2 (1 / s is to 2^-23, the quotient to 2^-24). Halves are common where few-bit values meet (one in 650
 // bf16 values): where x - q s is exactly s / 2, q goes to the even side. What is left takes the division (f32 values close
-// to a half), as do values that need the clamp: NaN, infinities, and groups whose s is not a normal f16 (in all others
-// |x / s| <= 7.01). The q + 8 of four values add up to 16 bits in f32.
+// to a half), as do values that need the clamp: infinities, and groups whose s is not a normal f16 (in all others
+// |x / s| <= 7.01). A NaN makes its group's scale NaN. The q + 8 of four values add up to 16 bits in f32.
 __device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], uint16_t* scale) {
   float top = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; j += 2) top = max3(top, fabsf(x[j]), fabsf(x[j + 1]));
+  for (int j = 0; j < 8; j += 2) top = max3_nan(top, fabsf(x[j]), fabsf(x[j + 1]));
 #pragma unroll
-  for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  constexpr float SEVENTH = 1.f / 7.f, MAGIC = 12582912.f;
-  const float near = top * SEVENTH, want = fmaf(fmaf(-7.f, near, top), SEVENTH, near);
-  const __half s16 = __float2half_rn(fminf(want, 65504.f));
+  for (int o = 4; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  constexpr float SEVENTH = 1.f / 7.f, MAGIC = 12582912.f, MOST = 7.f * 65504.f;
+  const float held = min_nan(top, MOST), near = held * SEVENTH;
+  const __half s16 = __float2half_rn(fmaf(fmaf(-7.f, near, held), SEVENTH, near));
   const float s = __half2float(s16), inv = rcp_approx(s);
   *scale = __half_as_ushort(s16);
   const float2 inv2 = make_float2(inv, inv), magic2 = make_float2(MAGIC, MAGIC), back2 = make_float2(-MAGIC, -MAGIC),
@@ -97,9 +102,9 @@ __device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], uint16_t* sca
     sum[j / 2] = __ffma2_rn(q, make_float2(w, 16.f * w), j & 1 ? sum[j / 2] : make_float2(34952.f + 8388608.f, 0.f));
   }
   uint32_t word = __byte_perm(__float_as_uint(sum[0].x + sum[0].y), __float_as_uint(sum[1].x + sum[1].y), 0x5410);
-  if (!(far <= 0.499998f * s && s >= 6.104e-5f && want <= 65504.f)) {
-    if (s == 0.f) return 0;
-    bool rest = !(far <= s && s >= 6.104e-5f && want <= 65504.f);
+  if (!(far <= 0.499998f * s && s >= 6.104e-5f && top <= MOST)) {
+    if (!(s > 0.f)) return 0;  // (0 or NaN)
+    bool rest = !(far <= s && s >= 6.104e-5f && top <= MOST);
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       const float r = fmaf(x[j], inv, MAGIC), e = fmaf(__fadd_rn(r, -MAGIC), -s, x[j]), twice = 2.f * fabsf(e);
