@@ -136,3 +136,13 @@ def test_a_prompt_needs_the_same_memory_whatever_the_layers(we, host, monkeypatc
         took[layers] = sum(n for what, n in host.log if what == "buffer")
         assert d.lengths == [0, 20, 0]
     assert took[1] == took[4]
+
+
+def test_no_kernel_of_these_operators_is_chosen_by_the_environment(we):
+    """Sizes, types and alignment decide: a variable would change a call's rounding behind its caller's back."""
+    import os
+
+    csrc = os.path.join(os.path.dirname(we.__file__), "csrc")
+    for name in ("we_decode.cu", "k_matvec.cu", "k_kv4.cu", "k_cross.cu", "k_cross_flash.cu", "attn_merge.cuh"):
+        with open(os.path.join(csrc, name)) as f:
+            assert "getenv" not in f.read(), name

@@ -221,11 +221,7 @@ int we_cross_attention(we_ctx* ctx, const we_cross_desc* desc) {
   // From 9 rows (tokens x heads of a group) on the tcgen05 kernel: its steps cost the same for 1 to 128 rows, the tiles' for
   // 1 to 8. us, tiles / tcgen05: 8 x 4096 keys, 24 heads, 8 rows 73.7 / 80.7, 9 rows 93.0 / 80.9; 4 x 1500 keys, 4 groups of
   // 4 heads, 8 rows 10.1 / 11.4, 16 rows 19.1 / 12.6.
-  static const int64_t from = [] {
-    const char* env = getenv("WE_CROSS_FLASH");  // test / tuning override: query rows from which it is used
-    return env ? (int64_t)atoi(env) : (int64_t)9;
-  }();
-  if (d.tq * group >= from && we::cross_flash_supported(d)) {
+  if (d.tq * group >= 9 && we::cross_flash_supported(d)) {
     const cudaError_t e = we::launch_cross_flash(d, we_ctx_dev_err(ctx), we_num_sms(ctx), we_ctx_stream(ctx));
     if (e != cudaErrorNotSupported) {
       DLK(e, "cross attention");
