@@ -417,7 +417,7 @@ int we_kv4_unpack(we_ctx* ctx, const we_kv4_cache* cache, void* k, void* v, int3
    kv_heads, as we_attention groups them; scale 0 = 1 / sqrt(dim), else any finite value of either sign. */
 int we_kv4_attention(we_ctx* ctx, const we_kv4_cache* cache, const void* q, int32_t dtype, int64_t tokens,
                      int64_t heads, int64_t q_stride, float scale, void* out, int32_t out_dtype, int64_t out_stride);
-/* lengths[b] += tokens for every sequence that is not idle: the end of a step, after its last layer. */
+/* lengths[b] += tokens (2^31 - 1 at most) for every sequence that is not idle: the end of a step, after its last layer. */
 int we_kv4_advance(we_ctx* ctx, const we_kv4_cache* cache, int64_t tokens);
 
 /* ---------------- cross attention: queries of one sequence, keys and values of another ----------------

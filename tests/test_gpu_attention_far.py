@@ -92,3 +92,13 @@ def test_more_keys_are_refused(we, graph):
         with pytest.raises(E, match="tokens"):
             we.kernels.cross_attention(graph, b, b, b, b, 1, kw.get("tq", 1), kw.get("tk", 1), 1, 1, 1, dtype="bf16", out_dtype="bf16")
     assert graph.device_error() == 0
+
+
+def test_advance_stops_at_the_end_of_its_type(we, graph):
+    """A length that would pass 31 bits stays a length: a negative one would mark the sequence idle."""
+    c = Cache(we, graph, 4, 16, 1, 64, 16, 3)
+    c.set_lengths([2**31 - 10, 5, -1, 2**31 - 1])
+    we.kv4.advance(graph, c.c, 100)
+    assert graph.read(c.lengths, 16, np.int32).tolist() == [2**31 - 1, 105, -1, 2**31 - 1]
+    we.kv4.advance(graph, c.c, 2**31 - 1)
+    assert graph.read(c.lengths, 16, np.int32).tolist() == [2**31 - 1, 2**31 - 1, -1, 2**31 - 1]

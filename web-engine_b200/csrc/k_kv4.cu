@@ -230,7 +230,7 @@ __global__ void kv4_advance_kernel(int32_t* lengths, int64_t batch, int32_t toke
   pdl_wait();
   pdl_launch_dependents();
   for (int64_t b = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; b < batch; b += (int64_t)gridDim.x * blockDim.x)
-    if (lengths[b] >= 0) lengths[b] += tokens;
+    if (lengths[b] >= 0) lengths[b] = (int32_t)min((int64_t)lengths[b] + tokens, (int64_t)0x7fffffff);  // (never to idle)
 }
 
 // ---------------- attention ----------------
