@@ -369,8 +369,9 @@ struct Part {
 // key of large values to which a row gives no weight takes no bits from the row's other keys (with one power for all, values
 // 10^7 below such a key's came out as zeros, or with a few bits in f32).
 // Choosing between the two step by step cost every call 5% (16 sequences of 3001 to 16384 keys, 48 heads on 12: 68.4 us against
-// 65.0); the check of the range and the code beside it cost it nothing, a call of one short sequence 0.2 us of 6.2. Values that
-// need the second sweep take about twice the time. (256-wide heads with more than 8 rows, which spilled before, lost 6%: 8 tokens of
+// 65.0); the check of the range and the code beside it cost it nothing, a call of one short sequence 0.2 us of 6.2. Values
+// that need the second sweep: 4 sequences of 16000 keys 28.6 -> 35.7 us, in f32 40.2 -> 47.3 (scales of zero cost a check each step,
+// 30.8 and 43.2). (256-wide heads with more than 8 rows, which spilled before, lost 6%: 8 tokens of
 // 32 heads on 8, 4 x 4000 keys, 62.7 us against 58.9.)
 template <int D, int NQ, int KT, int TERMS, bool EXACT>
 __device__ __forceinline__ bool sweep(const Params& p, int b, int head, int rtile, int have, int key0, int key1, uint8_t* smem,
@@ -761,13 +762,15 @@ __device__ __forceinline__ bool sweep(const Params& p, int b, int head, int rtil
             vb = G == 1 ? min(vb, vs[t][h][g]) : __vminu2(vb, vs[t][h][g]);
           }
       if (G > 1) vt = max(vt & 0xffffu, vt >> 16), vb = min(vb & 0xffffu, vb >> 16);
-      if (__any_sync(0xffffffffu, grow || vt > v_range >> 16 || vb < (v_range & 0xffffu))) {
+      const bool move = grow || vt > v_range >> 16;
+      if (__any_sync(0xffffffffu, move || vb < (v_range & 0xffffu))) {
+        const bool rescale = __any_sync(0xffffffffu, move);  // (else some scales are 0, which are no values, or too small)
         // O and the sums of weights are kept over 2^(exponent of the largest scale)
         const uint32_t had = v_range >> 26, top = max(__reduce_max_sync(0xffffffffu, vt), had << 10), e = top >> 10;
         // the smallest scale that is held well beside it: 2^-RANGE of it (smaller ones before it are in O, in f32)
         const uint32_t least = e > RANGE ? top - (RANGE << 10) : 0x400u >> min(RANGE + 1u - e, 11u);
         v_range = (top | 0x3ffu) << 16 | least;
-        bool small = false;  // (zeros are no values)
+        bool small = false;
 #pragma unroll
         for (int t = 0; t < KT; t++)
 #pragma unroll
@@ -780,7 +783,7 @@ __device__ __forceinline__ bool sweep(const Params& p, int b, int head, int rtil
         if (top >= 0x7c00u || __any_sync(0xffffffffu, small)) return false;  // (a negative scale is one of the former)
         const float f = __uint_as_float((127u + had - e) << 23);
 #pragma unroll
-        for (int nq = 0; nq < NQ; nq++) {
+        for (int nq = 0; nq < NQ && rescale; nq++) {
           float corr[2];
 #pragma unroll
           for (int k = 0; k < 2; k++) {
