@@ -1057,6 +1057,13 @@ cudaError_t launch_kv4_advance(const we_kv4_cache& c, int64_t tokens, cudaStream
 }
 
 namespace {
+// CTAs an SM by registers. f32: three (4 sequences of 16000 keys, 48 heads of 128 on 12, took 52 us with four and take 40). bf16:
+// four, for which 128-wide heads spill 16 bytes; calls of so few CTAs that three an SM hold them do better with three (2
+// sequences of 4096 keys, 8 heads: 10.4 us against 12.5; 16 of 3001 to 16384, 48 on 12: 75.1 against 65.3).
+constexpr int kv4_per_sm(int dim, int nq, int terms) {
+  return dim * nq == 512 ? 1 : dim * nq == 256 ? 2 : terms == 2 ? 3 : 4;
+}
+
 // How the work of a call is cut: q rows into tiles of 8 or 16, keys into chunks of a CTA.
 struct Kv4Plan {
   int nq, row_tiles, runs, chunk;
@@ -1068,14 +1075,19 @@ Kv4Plan kv4_plan(const Kv4AttnArgs& a, int sms) {
   q.nq = rows <= 8 ? 1 : 2;
   q.row_tiles = (int)((rows + 8 * q.nq - 1) / (8 * q.nq));
   q.units = a.c.batch * a.c.kv_heads * q.row_tiles;
-  // Four CTAs an SM, less what no cluster of 8 fits into (71 of 74 do). A sequence's length is known on the device only, so
-  // runs are cut for the longest possible one, into about one wave of CTAs; more and shorter ones cost more in their first
-  // and last steps than ragged lengths gain (68 us against 81 with four waves for 16 sequences of 3001 to 16384 keys, 60
-  // against 78 for one of 131000). Merging runs takes as long as some 800 keys of a CTA, so that many have to be saved: one
-  // sequence of 4096 keys, 12 heads, 9.3 us in one run and 11.4 in five, 8192 13.5 and 13.0, 16384 22.5 and 16.5.
+  // The CTAs that the SMs hold, four an SM (f32: three), less what no cluster of 8 fits into (71 of 74 do). A sequence's length is
+  // known on the device only, so runs are cut for the longest possible one, into about one wave of CTAs; more and shorter ones
+  // cost more in their first and last steps than ragged lengths gain (68 us against 81 with four waves for 16 sequences of 3001
+  // to 16384 keys, 60 against 78 for one of 131000). Merging runs takes as long as some 800 keys of a CTA (500 in f32, whose keys
+  // take longer), so that many have to be saved. One sequence, 12 kv heads, in one run and in as many as fit: bf16, dim 128: 4096
+  // keys 9.8 and 11.7, 8192 13.4 and 14.0, 16384 21.1 and 17.3 us; dim 64: 8.2 and 10.8, 11.1 and 11.6, 16.7 and 13.8; f32, dim
+  // 128: 4096 12.1 and 12.9, 8192 17.8 and 14.2; dim 64: 9.7 and 11.1, 13.8 and 11.9. Where one more run would take a few CTAs more
+  // than three an SM, f32 stays below (2 sequences of 16384 keys, 16 heads of 128: 40 us, 46 in two runs).
   const int64_t cap = std::max<int64_t>(1, a.c.max_pages * a.c.page), alone = (cap + kv::CLUSTER - 1) / kv::CLUSTER;
-  const int64_t fit = std::max<int64_t>(1, (int64_t)(sms * 4 - 24) / (q.units * kv::CLUSTER));
-  const int64_t runs = alone - alone / fit > 800 ? fit : 1;
+  const bool three = (a.dtype == WE_F32 || a.out_dtype == WE_F32) && a.c.dim <= 128;
+  const int per_sm = three ? 3 : 4;
+  const int64_t fit = std::max<int64_t>(1, (int64_t)(sms - 6) * per_sm / (q.units * kv::CLUSTER));
+  const int64_t runs = alone - alone / fit > (three ? 500 : 800) ? fit : 1;
   const int64_t chunk = std::max<int64_t>(256, (alone + runs - 1) / runs);
   q.chunk = (int)((std::min<int64_t>(chunk, 0x4000000) + 31) / 32 * 32);
   q.runs = (int)((cap + (int64_t)q.chunk * kv::CLUSTER - 1) / ((int64_t)q.chunk * kv::CLUSTER));
@@ -1083,15 +1095,7 @@ Kv4Plan kv4_plan(const Kv4AttnArgs& a, int sms) {
   return q;
 }
 
-// CTAs an SM by registers. f32: three (4 sequences of 16000 keys, 48 heads of 128 on 12, took 52 us with four and take 40). bf16:
-// four, for which 128-wide heads spill 16 bytes; calls of so few CTAs that three an SM hold them do better with three (2
-// sequences of 4096 keys, 8 heads: 10.4 us against 12.5; 16 of 3001 to 16384, 48 on 12: 75.1 against 65.3).
-template <int D, int NQ, int TERMS>
-constexpr int per_sm() {
-  return D * NQ == 512 ? 1 : D * NQ == 256 ? 2 : TERMS == 2 ? 3 : 4;
-}
-
-template <int D, int NQ, int KT, int TERMS, int PER_SM = per_sm<D, NQ, TERMS>()>
+template <int D, int NQ, int KT, int TERMS, int PER_SM = kv4_per_sm(D, NQ, TERMS)>
 cudaError_t kv4_launch(const kv::Params& p, dim3 grid, cudaStream_t st) {
   auto kern = kv4_attention_kernel<D, NQ, KT, TERMS, PER_SM>;
   constexpr int ring = kv::WARPS * kv::ring_depth<D, KT>() * KT * (D * 16 + D);
