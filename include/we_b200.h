@@ -378,7 +378,7 @@ int we_attend(we_ctx* ctx, const void* q, const void* k, const void* v, int32_t 
    we_matmul applies them. x and y f32 or bf16 with row strides and offsets in values; w contiguous [n, k / 2] and
    16-byte aligned, f16 group scales [n, k / 64], k a multiple of 64; scale, chan_scale and k_split do not apply (scale is
    ignored, the others are refused). flags: WE_MM_ACCUMULATE. Within a group of 64 values of a row, bits below 2^-36 of
-   the largest are lost; a row that holds a NaN or an infinity gives NaN. */
+   the largest are lost; a row that holds a NaN gives NaN, one that holds an infinity NaN or infinities. */
 #define WE_MATVEC_MAX_ROWS 16
 int we_matvec(we_ctx* ctx, const we_matmul_desc* desc, const void* x, const void* w, void* y);
 
@@ -414,7 +414,10 @@ int we_kv4_unpack(we_ctx* ctx, const we_kv4_cache* cache, void* k, void* v, int3
 /* Attention of each sequence's `tokens` newest tokens over its cache: query i of sequence b stands at position
    lengths[b] + i and sees keys 0 .. lengths[b] + i, so the step's keys have been appended. q [batch, tokens, heads, dim]
    and out alike (q_stride / out_stride values from a token to the next, 0 = heads * dim); heads a multiple of
-   kv_heads, as we_attention groups them; scale 0 = 1 / sqrt(dim), else any finite value of either sign. */
+   kv_heads, as we_attention groups them; scale 0 = 1 / sqrt(dim), else any finite value of either sign. Products of q and
+   codes are exact to 2^-22, but that values of q below 2^-36 of their row's largest are lost; sums are f32. Where q and out
+   are bf16 the weights and their products with v's scales are rounded to f16 (2^-11 each), else held to 2^-22. A sequence
+   has room for 2^31 - 2^24 - 1 tokens at most. */
 int we_kv4_attention(we_ctx* ctx, const we_kv4_cache* cache, const void* q, int32_t dtype, int64_t tokens,
                      int64_t heads, int64_t q_stride, float scale, void* out, int32_t out_dtype, int64_t out_stride);
 /* lengths[b] += tokens (2^31 - 1 at most) for every sequence that is not idle: the end of a step, after its last layer. */
@@ -427,7 +430,9 @@ int we_kv4_advance(we_ctx* ctx, const we_kv4_cache* cache, int64_t tokens);
    tokens follow the previous one's. A key j of entry b is seen when j < key_lengths[b] (device int32, NULL = tk) and
    key_mask[b][j] != 0 (device bytes [batch, tk], NULL = all). A row that sees no key gives zeros; values of unseen keys
    (NaN included) do not reach the output. scale 0 = 1 / sqrt(dim), else any finite value of either sign. dim 1..256, f32 or
-   bf16. */
+   bf16; tq and tk at most 2^31 - 2^24 - 1. bf16 q, k, v: products exact, sums in f32, the weights rounded to bf16 (2^-9)
+   before their product with v, whatever out's type. f32: operands are held to 2^-22; a seen infinity, or a
+   magnitude of 2^128 (1 - 2^-12) or more, gives NaN where it enters. */
 typedef struct {
   const void* q;
   const void* k;

@@ -12,8 +12,10 @@
 // shared memory before they hand P over, so that nothing of them reaches a product; tiles without any skip both.
 // Calls whose items would leave SMs idle give each item to a cluster, its CTAs a share of the keys each, merged over
 // distributed shared memory.
-// Measured: 2 x 4096 queries x (512, 333) keys, 24 heads of 128: 67 us, 635 TFLOP/s; 2048 x 4096 keys 138 us (750 TFLOP/s),
-// 179 us with a random mask; 128 x 4096 keys 22.7 us (64 without the clusters). A step of a CTA takes about 4600 cycles:
+// P is rounded to bf16 (2^-9 each, sums in f32), as V is stored: kind::f16 takes both operands of one type.
+// Measured in recorded graphs: 2 x 4096 queries x (512, 333) keys, 24 heads of 128: 69 us, 613 TFLOP/s (76 as single calls on
+// inputs that were not read just before; 67.8 when a tile held one head's rows only); 2048 x 4096 keys 140 us (735 TFLOP/s),
+// 180 us with a random mask; 128 x 4096 keys 22.7 us (64 without the clusters). A step of a CTA takes about 4600 cycles:
 // from P to the next S 2000 (the products are 1024 of it, more when the other CTA's are in front), reading S and the maxima
 // 500, exponentials 1650, P's way to TMEM 400. Storing each lane's row by itself took 10400 cycles an item; one CTA per item
 // without the next one's loads and S in flight 87 us instead of 82.

@@ -28,7 +28,7 @@ __device__ __forceinline__ int64_t kv4_row(const we_kv4_cache& c, int64_t b, int
 // word on the packed one, 8 neighbouring lanes a group. It keeps its place within a token (side, head, values) and steps
 // over the tokens of its CTA, whose rows are looked up once, so that a step has little to compute but the values.
 // Measured: 2 x 4099 tokens x 12 heads of 128 in bf16 in 23 us and back in 17 (the bytes of each are 10 us), 16 tokens both
-// ways 4.7 us; a warp per group and a look-up per value took 167 us.
+// ways 4.7 us in a recorded graph (5.9 as two calls from Python); a warp per group and a look-up per value took 167 us.
 constexpr int ROW_THREADS = 256, ROW_SPAN = 32;
 struct RowShape {
   int units;       // of 8 values in a token: k's, then v's
@@ -235,12 +235,13 @@ __global__ void kv4_advance_kernel(int32_t* lengths, int64_t batch, int32_t toke
 
 // ---------------- attention ----------------
 // Per (sequence, kv head): q rows (the new tokens times the heads of the group) over that head's keys. The cache is read
-// once and bounds the call (dim / 2 + dim / 32 bytes per key, for k and for v); the products run on 16 x 8 x 16 tensor
+// once for every 8 or 16 rows (dim / 2 + dim / 32 bytes per key, for k and for v); the products run on 16 x 8 x 16 tensor
 // tiles with KEYS (for v: dims) as the 16 rows and up to 8 q rows as the columns, so a tile has no more idle rows than
 // the group leaves of 8, and the codes go from the registers they are unpacked in straight into the tile:
 // - S^T = K Q^T. A lane holds 16 codes of 2 keys; a pair of codes becomes the f16 subnormals u 2^-24, u = q + 8, by one
 //   logical operation (and u 2^-20 for the next nibble, whose q is divided by 16); the sum of a group of 64 starts at
-//   -8 sum(q). The key's scale multiplies the group's sum in f32.
+//   -8 sum(q). The key's scale multiplies the group's sum in f32. A row of q is held over the power of two of its largest
+//   value; what is below 2^-36 of that is lost.
 // - O^T = V^T P^T. Two keys' words are interleaved by byte permutations, so that a pair is the same dim of two keys; p
 //   times the key's scale of v, times a power of two that keeps it in f16's range (2^15 at most), is the other operand,
 //   turned by movmatrix from S^T's layout. The offset 8 is taken out at the end with the sum of those weights, which one
@@ -255,8 +256,8 @@ __global__ void kv4_advance_kernel(int32_t* lengths, int64_t batch, int32_t toke
 namespace kv {
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int CLUSTER = 8;    // CTAs that share a run of keys and merge over distributed shared memory
-// Steps in a warp's ring (a power of two): 35 KB a CTA, four of which an SM holds with their 128 registers a thread. With two
-// steps whatever their size, 5 tokens over 3333 keys of 64 in f32, out of memory, took 14.0 us instead of 12.0.
+// Steps in a warp's ring (a power of two): 35 KB a CTA, so that registers say how many an SM holds. With two steps whatever
+// their size, 5 tokens over 3333 keys of 64 in f32, out of memory, took 14.0 us instead of 12.0.
 template <int D, int KT>
 constexpr int ring_depth() {
   return 512 / (KT * D);

@@ -141,7 +141,7 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t v, uint32_t mask, int odd
   return as_u32(__hadd2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(odd ? -1152.f : -1032.f)));
 }
 
-// XT: type of x; NT: tiles of 8 columns; RT: row tiles of 16 channels of a warp; PER_SM: CTAs that fit an SM. Columns 2 t
+// XT: type of x; NT: tiles of 8 columns; RT: row tiles of 16 channels of a warp; WARPS: of a CTA, one an SM. Columns 2 t
 // and 2 t + 1 are the two groups of a chunk for piece t / m (f32: the leading bits, the following ones) of token t % m.
 template <int XT, int NT, int RT, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 1) matvec_mma_kernel(const void* __restrict__ x, const uint8_t* __restrict__ w,

@@ -220,7 +220,9 @@ int we_cross_attention(we_ctx* ctx, const we_cross_desc* desc) {
   if (d.tq > 0x7fffffff / group) return we_ctx_fail(ctx, WE_EINVAL, "cross attention: tq * heads / kv_heads must fit 31 bits");
   // From 9 rows (tokens x heads of a group) on the tcgen05 kernel: its steps cost the same for 1 to 128 rows, the tiles' for
   // 1 to 8. us, tiles / tcgen05: 8 x 4096 keys, 24 heads, 8 rows 73.7 / 80.7, 9 rows 93.0 / 80.9; 4 x 1500 keys, 4 groups of
-  // 4 heads, 8 rows 10.1 / 11.4, 16 rows 19.1 / 12.6.
+  // 4 heads, 8 rows 10.1 / 11.4, 16 rows 19.1 / 12.6. Calls of few heads and many keys would take tiles up to 16 rows: 2 x 512
+  // keys, 16 heads, 9 rows 8.5 / 9.5 (dim 64: 6.9 / 8.6), 1500 keys 10.9 / 13.9 (8.5 / 12.3), 77 keys 8.1 / 7.2 (6.4 / 6.3), and
+  // with 32 rows 15.8 / 11.4, 21.3 / 15.4 and 14.7 / 7.3.
   if (d.tq * group >= 9 && we::cross_flash_supported(d)) {
     const cudaError_t e = we::launch_cross_flash(d, we_ctx_dev_err(ctx), we_num_sms(ctx), we_ctx_stream(ctx));
     if (e != cudaErrorNotSupported) {

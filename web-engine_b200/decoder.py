@@ -144,7 +144,8 @@ class Decoder:
     # ---- one token of every sequence ----
     def step(self, x=None) -> Buffer:
         """The next token of every sequence: x [batch, hidden] f32 (host array; None: `self.x` holds it already).
-        Returns self.x, the last layer's output, in stream order."""
+        Returns self.x, the last layer's output, in stream order. Every sequence takes part: a full one is an error for
+        all of them, and `reset` empties them together."""
         g, cfg = self.graph, self.cfg
         self._ready()
         if max(self.lengths) >= self.tokens:

@@ -323,8 +323,8 @@ def cross_attention(graph: Graph, q, k, v, out, batch: int, tq: int, tk: int, he
                     **kw) -> None:
     """out = softmax(scale q k^T) v per head, the keys and values another sequence's (we_cross_attention): q, out
     [batch, tq, heads, dim], k, v [batch, tk, kv_heads, dim]. key_lengths: int32 [batch]; key_mask: bytes [batch, tk],
-    0 = unseen; a row that sees nothing gives zeros. scale 0 = 1 / sqrt(dim). Strides are values from a token to the
-    next (0 = contiguous)."""
+    0 = unseen; a row that sees nothing gives zeros. scale 0 = 1 / sqrt(dim), else of either sign. Strides are values from
+    a token to the next (0 = contiguous). bf16 inputs: the weights are rounded to bf16 before their product with v."""
     cross_attention_call(graph, q, k, v, out, batch, tq, tk, heads, kv_heads, dim, **kw)()
 
 

@@ -99,7 +99,8 @@ def attention_call(graph: Graph, cache: Cache, q, out, tokens: int, heads: int, 
 def attention(graph: Graph, cache: Cache, q, out, tokens: int, heads: int, dtype: str = "bf16", out_dtype: str = "bf16",
               q_stride: int = 0, out_stride: int = 0, scale: float = 0.0) -> None:
     """softmax(scale q k^T) v of each sequence's newest tokens over its cache: q, out [batch, tokens, heads, dim]; query i
-    sees keys 0 .. lengths[b] + i (appended before). scale 0 = 1 / sqrt(dim). Idle sequences give zeros."""
+    sees keys 0 .. lengths[b] + i (appended before). scale 0 = 1 / sqrt(dim), else of either sign. Idle sequences give
+    zeros; a group of 64 values that held a NaN when it was appended gives NaN."""
     attention_call(graph, cache, q, out, tokens, heads, dtype, out_dtype, q_stride, out_stride, scale)()
 
 
